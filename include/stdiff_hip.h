@@ -37,7 +37,8 @@ enum {
     STDIFF_ERR_SHAPE = -2,    /* shape not supported by the kernels (see each function) */
     STDIFF_ERR_ALIGN = -3,    /* pointer or leading dimension not 16-byte aligned */
     STDIFF_ERR_STATE = -4,    /* handle misuse (graph not captured, ...) */
-    STDIFF_ERR_SCRATCH = -5   /* problem larger than the library's static scratch buffer (stdiff_gemm_static_scratch) */
+    STDIFF_ERR_SCRATCH = -5,  /* problem larger than the library's static scratch buffer (stdiff_gemm_static_scratch) */
+    STDIFF_ERR_WORKSPACE = -6 /* the caller's workspace is missing or too small (each function's *_workspace says the bytes) */
 };
 
 /* GEMM epilogues: v = sum_k A[m,k] W[n,k] + bias[n] */
@@ -492,6 +493,64 @@ long long stdiff_dit_backward_parts(const stdiff_train_weights* w);   /* floats 
 typedef void (*stdiff_bucket_fn)(int bucket, void* user);
 int stdiff_dit_backward(const stdiff_train_weights* w, const stdiff_train_acts* a, void* side_stream,
                         stdiff_bucket_fn after_bucket, void* user, void* stream);
+
+/* ---------------------------------------------------------------- norm, optimizer and 8-bit product beside the DiT
+ * (no counterpart in the reference, which leaves them to torch).  Rows may begin at any element and have any length
+ * unless a function says otherwise; leading dimensions are 64-bit, and those of matrices that are only read may be smaller
+ * than a row (0: one row for all).  None of them allocates; each may be captured.
+ *
+ * LayerNorm over rows of H with a weight and a bias per column (either may be NULL: 1 and 0; both have w_dtype):
+ *   mean = mean x, rstd = 1 / sqrt(mean (x - mean)^2 + eps), y = (x - mean) * rstd * weight + bias
+ * statistics in fp32 from the centred row; mean / rstd (fp32 [R], either may be NULL) are kept for the backward.
+ * y may be x (same dtype and leading dimension). */
+int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, const void* weight, const void* bias, int w_dtype, float eps,
+                      void* y, long long ldy, int y_dtype, float* mean, float* rstd, int R, int H, void* stream);
+/* Its backward from the forward's statistics:  xhat = (x - mean) * rstd, g = dy * weight,
+ *   dx = rstd * (g - mean g - xhat * mean(g * xhat))   in x's dtype (dx may be dy or x where dtype and leading dimension agree)
+ *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy   fp32 [H], either may be NULL; added to what they
+ *   hold when accumulate != 0.  The sums are formed in a fixed order (the same bits every run) from partial sums in
+ *   `workspace` (16-byte aligned, stdiff_layer_norm_bwd_workspace(R, H) bytes; not read when both are NULL). */
+long long stdiff_layer_norm_bwd_workspace(int R, int H);
+int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const void* x, long long ldx, int x_dtype,
+                          const float* mean, const float* rstd, const void* weight, int w_dtype, void* dx, long long lddx,
+                          float* dweight, float* dbias, int accumulate, float* workspace, long long workspace_bytes, int R,
+                          int H, void* stream);
+
+/* AdamW over many tensors at once, the gradients clipped by the norm over all of them:
+ *   g = coef * grad, coef = grad_scale * min(1, max_norm / (norm + 1e-6)), norm = grad_scale * sqrt(sum grad^2)
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * state_bits 32: exp_avg / exp_avg_sq are fp32 [n].  state_bits 8: they are e4m3 codes [n], of m and of the ROOT of v, and every
+ * 256 consecutive elements share exp_avg_scale / exp_avg_sq_scale (fp32 [ceil(n / 256)]): m = scale * code, sqrt v = scale *
+ * code; all zeros is the state before the first step.  A block that holds an infinity or a NaN is NaN from the next step on.
+ * step_dev: int32 [1], the steps done before this call; incremented by it.  max_norm <= 0: no clipping.  norm (may be
+ * NULL): receives the norm.  A norm that is NaN makes every parameter NaN.  The `tensors` array is read during the call
+ * only; the tensors must not overlap.  workspace: stdiff_adamw_multi_workspace(n_tensors) bytes, 4-byte aligned. */
+typedef struct {
+    void* param; const void* grad; void* exp_avg; void* exp_avg_sq; float* exp_avg_scale; float* exp_avg_sq_scale;
+    long long n; int param_dtype; int grad_dtype; float weight_decay; int reserved;
+} stdiff_adamw_tensor;
+typedef struct {
+    const stdiff_adamw_tensor* tensors; int n_tensors; int state_bits;
+    int32_t* step_dev; float* norm; float* workspace; long long workspace_bytes;
+    double lr, beta1, beta2, eps, max_norm, grad_scale;
+} stdiff_adamw_multi_args;
+long long stdiff_adamw_multi_workspace(int n_tensors);
+int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream);
+
+/* Rows in 8 bits:  scale[r] = max |x[r]| / 127, q[r][k] = rint(x[r][k] * (127 / max |x[r]|));  a zero row: zeros and scale 0.
+ * q: int8 [R][ldq], 16-byte aligned, ldq % 16 == 0, ldq >= round_up(K, 16); columns K .. round_up(K, 16) - 1 become
+ * zeros.  A row that holds an infinity or a NaN gets a scale that is not finite. */
+int stdiff_quantize_rows(const void* x, long long ldx, int x_dtype, void* q, long long ldq, float* scale, int R, int K, void* stream);
+/* C[M,N] = (sum_k A[m,k] W[n,k]) * w_scale[n] * a_scale[m] + bias[n]   (A, W int8; the sum exact in int32, K <= 131071;
+ * bias may be NULL; C fp32 or 16-bit).  A and W 16-byte aligned, lda / ldw % 16 == 0 and >= round_up(K, 16): a row is read
+ * up to round_up(K, 16), what stands behind K does not matter. */
+typedef struct {
+    int M, N, K;
+    const void* A; long long lda; const void* W; long long ldw;
+    const float* a_scale; const float* w_scale; const float* bias;
+    void* C; long long ldc; int c_dtype;
+} stdiff_gemm_i8_args;
+int stdiff_gemm_i8(const stdiff_gemm_i8_args* a, void* stream);
 
 /* ---------------------------------------------------------------- hipGraph capture of a reverse step
  * begin/end bracket any sequence of the calls above on `stream`; launch replays it (model/sample.py:67-95 loop body

@@ -121,6 +121,23 @@ class AdamWArgs(C.Structure):
                 ("weight_decay", f32), ("bf16_mirror", vp)]
 
 
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", vp), ("grad", vp), ("exp_avg", vp), ("exp_avg_sq", vp), ("exp_avg_scale", vp),
+                ("exp_avg_sq_scale", vp), ("n", C.c_longlong), ("param_dtype", i32), ("grad_dtype", i32),
+                ("weight_decay", f32), ("reserved", i32)]
+
+
+class AdamWMultiArgs(C.Structure):
+    _fields_ = [("tensors", C.POINTER(AdamWTensor)), ("n_tensors", i32), ("state_bits", i32), ("step_dev", vp), ("norm", vp),
+                ("workspace", vp), ("workspace_bytes", C.c_longlong)] + \
+               [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "max_norm", "grad_scale")]
+
+
+class GemmI8Args(C.Structure):
+    _fields_ = [("M", i32), ("N", i32), ("K", i32), ("A", vp), ("lda", C.c_longlong), ("W", vp), ("ldw", C.c_longlong),
+                ("a_scale", vp), ("w_scale", vp), ("bias", vp), ("C", vp), ("ldc", C.c_longlong), ("c_dtype", i32)]
+
+
 _SIGS = {
     "stdiff_abi_version": (i32, []),
     "stdiff_h16_format": (i32, []),
@@ -171,6 +188,13 @@ _SIGS = {
     "stdiff_dit_train_forward": (i32, [C.POINTER(TrainWeights), C.POINTER(TrainActs), vp, vp, vp]),
     "stdiff_dit_backward": (i32, [C.POINTER(TrainWeights), C.POINTER(TrainActs), vp, BucketFn, vp, vp]),
     "stdiff_dit_backward_parts": (C.c_longlong, [C.POINTER(TrainWeights)]),
+    "stdiff_layer_norm": (i32, [vp, i64, i32, vp, vp, i32, f32, vp, i64, i32, vp, vp, i32, i32, vp]),
+    "stdiff_layer_norm_bwd_workspace": (C.c_longlong, [i32, i32]),
+    "stdiff_layer_norm_bwd": (i32, [vp, i64, i32, vp, i64, i32, vp, vp, vp, i32, vp, i64, vp, vp, i32, vp, i64, i32, i32, vp]),
+    "stdiff_adamw_multi_workspace": (C.c_longlong, [i32]),
+    "stdiff_adamw_multi": (i32, [C.POINTER(AdamWMultiArgs), vp]),
+    "stdiff_quantize_rows": (i32, [vp, i64, i32, vp, i64, vp, i32, i32, vp]),
+    "stdiff_gemm_i8": (i32, [C.POINTER(GemmI8Args), vp]),
     "stdiff_graph_begin": (i32, [vp]),
     "stdiff_graph_end": (i32, [vp, C.POINTER(vp)]),
     "stdiff_graph_launch": (i32, [vp, vp]),
@@ -231,7 +255,7 @@ class StdiffError(RuntimeError):
 def check(rc):
     if rc != 0:
         msg = lib().stdiff_error_string(rc).decode()
-        if rc in (-1, -2, -3, -5):
+        if rc in (-1, -2, -3, -5, -6):
             raise ValueError(f"stdiff_hip: {msg} (status {rc})")
         raise StdiffError(f"stdiff_hip: {msg} (status {rc})")
 

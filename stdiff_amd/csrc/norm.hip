@@ -1,0 +1,453 @@
+// LayerNorm over rows with a weight and a bias per column, forward and backward (the adaLN form, whose shift and scale
+// differ from row to row, is ln_modulate in pointwise.hip / train.hip).
+//   forward :  mu = mean x, var = mean (x - mu)^2, rstd = 1 / sqrt(var + eps), y = (x - mu) * rstd * w + b
+//   backward:  xhat = (x - mu) * rstd, g = dy * w, dx = rstd * (g - mean g - xhat * mean(g * xhat)),
+//              dw = sum over rows of dy * xhat, db = sum over rows of dy
+// A row is read once and stays in registers: V elements (16 bytes of x) per lane and vector, NV vectors per lane, T
+// lanes per row.  The variance is formed from the centred values (a second walk over the registers), so a row whose mean
+// is far larger than its spread keeps its digits.  All statistics and sums are fp32.
+#include "common.h"
+
+namespace {
+
+typedef f32x4 f32x4_u __attribute__((aligned(4)));       // rows may begin at any element: gfx950 loads and stores of
+typedef u32x4 u32x4_u __attribute__((aligned(2)));       // 16 bytes need no alignment in global memory
+typedef u32x2 u32x2_u __attribute__((aligned(2)));
+
+template <int V> __device__ __forceinline__ void ldv(const float* p, float* o) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        const f32x4 v = *(const f32x4_u*)(p + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i + j] = v[j];
+    }
+}
+template <int V> __device__ __forceinline__ void ldv(const bf16_t* p, float* o) {
+    if constexpr (V == 8) {
+        const u32x4 v = *(const u32x4_u*)p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { o[2 * j] = bf_lo(v[j]); o[2 * j + 1] = bf_hi(v[j]); }
+    } else {
+        const u32x2 v = *(const u32x2_u*)p;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { o[2 * j] = bf_lo(v[j]); o[2 * j + 1] = bf_hi(v[j]); }
+    }
+}
+template <int V> __device__ __forceinline__ void stv(float* p, const float* o) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *(f32x4_u*)(p + i) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+}
+template <int V> __device__ __forceinline__ void stv(bf16_t* p, const float* o) {
+    if constexpr (V == 8)
+        *(u32x4_u*)p = u32x4{pack2bf(o[0], o[1]), pack2bf(o[2], o[3]), pack2bf(o[4], o[5]), pack2bf(o[6], o[7])};
+    else
+        *(u32x2_u*)p = u32x2{pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+}
+// V elements at column c of a row of H; what lies behind the row's end reads as `fill` and is not written
+template <int V, typename T> __device__ __forceinline__ void ld_edge(const T* row, int c, int H, float fill, float* o) {
+    if (c + V <= H) return ldv<V>(row + c, o);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = c + j < H ? Elem<T>::ld(row + c + j) : fill;
+}
+template <int V, typename T> __device__ __forceinline__ void st_edge(T* row, int c, int H, const float* o) {
+    if (c + V <= H) return stv<V>(row + c, o);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (c + j < H) Elem<T>::st(row + c + j, o[j]);
+}
+
+// sum over the T lanes of a row, the same bits in all of them; `part`: T / 64 floats per use, not reused before a barrier
+template <int T> __device__ __forceinline__ float row_sum(float v, float* part) {
+    v = wave_sum(v);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < T / 64; ++i) v += part[i];
+    }
+    return v;
+}
+
+template <typename TX, typename TY, typename TW, int V, int NV, int T>
+__global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long ldx, const TW* w, const TW* b, float eps,
+                                                         TY* y, long long ldy, float* mean, float* rstd, int R, int H) {
+    __shared__ float part[2][2][T / 64];
+    constexpr int ROWS = 256 / T;
+    const int t = threadIdx.x % T;
+    float wv[NV][V], bv[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * T + t) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) { wv[i][j] = 1.f; bv[i][j] = 0.f; }
+        if (w) ld_edge<V>(w, c, H, 0.f, wv[i]);
+        if (b) ld_edge<V>(b, c, H, 0.f, bv[i]);
+    }
+    const float inv = 1.0f / (float)H;
+    int odd = 0;
+    for (long long row = (long long)blockIdx.x * ROWS + threadIdx.x / T; row < R; row += (long long)gridDim.x * ROWS, odd ^= 1) {
+        float v[NV][V], s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) ld_edge<V>(x + row * ldx, (i * T + t) * V, H, 0.f, v[i]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += v[i][j];
+        const float mu = row_sum<T>(s, part[odd][0]) * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[i][j] -= mu;
+                if ((i * T + t) * V + j < H) q += v[i][j] * v[i][j];
+            }
+        const float rs = 1.0f / sqrtf(row_sum<T>(q, part[odd][1]) * inv + eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = v[i][j] * rs * wv[i][j] + bv[i][j];
+            st_edge<V>(y + row * ldy, (i * T + t) * V, H, o);
+        }
+        if (t == 0) {
+            if (mean) mean[row] = mu;
+            if (rstd) rstd[row] = rs;
+        }
+    }
+}
+
+// rows too long for the registers: one block per row, the row is read three times (the second and third from the L2)
+template <typename TX, typename TY, typename TW>
+__global__ __launch_bounds__(256) void layer_norm_long_kernel(const TX* x, long long ldx, const TW* w, const TW* b, float eps,
+                                                              TY* y, long long ldy, float* mean, float* rstd, int R, int H) {
+    __shared__ float part[2][2][4];
+    const float inv = 1.0f / (float)H;
+    int odd = 0;
+    for (long long row = blockIdx.x; row < R; row += gridDim.x, odd ^= 1) {
+        const TX* xr = x + row * ldx;
+        TY* yr = y + row * ldy;
+        float s = 0.f, q = 0.f;
+        for (int c = threadIdx.x * 4; c < H; c += 1024) {
+            float v[4];
+            ld_edge<4>(xr, c, H, 0.f, v);
+            s += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        const float mu = row_sum<256>(s, part[odd][0]) * inv;
+        for (int c = threadIdx.x * 4; c < H; c += 1024) {
+            float v[4];
+            ld_edge<4>(xr, c, H, mu, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q += (v[j] - mu) * (v[j] - mu);
+        }
+        const float rs = 1.0f / sqrtf(row_sum<256>(q, part[odd][1]) * inv + eps);
+        for (int c = threadIdx.x * 4; c < H; c += 1024) {
+            float v[4], wv[4] = {1.f, 1.f, 1.f, 1.f}, bv[4] = {0.f, 0.f, 0.f, 0.f};
+            ld_edge<4>(xr, c, H, 0.f, v);
+            if (w) ld_edge<4>(w, c, H, 0.f, wv);
+            if (b) ld_edge<4>(b, c, H, 0.f, bv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (v[j] - mu) * rs * wv[j] + bv[j];
+            st_edge<4>(yr, c, H, v);
+        }
+        if (threadIdx.x == 0) {
+            if (mean) mean[row] = mu;
+            if (rstd) rstd[row] = rs;
+        }
+    }
+}
+
+// ws (or NULL: no weight gradient is asked for): [gridDim.x][2][ldp] partial sums of (dy * xhat, dy), one pair per block
+template <typename TX, typename TD, typename TW, int V, int NV, int T>
+__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
+                                                             const float* mean, const float* rstd, const TW* w, TX* dx,
+                                                             long long lddx, float* ws, int ldp, int R, int H) {
+    __shared__ float part[2][2][T / 64];
+    __shared__ float comb[T == 64 ? 64 * V * NV : 1];
+    constexpr int ROWS = 256 / T;
+    const int t = threadIdx.x % T;
+    float wv[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) { wv[i][j] = 1.f; aw[i][j] = ab[i][j] = 0.f; }
+        if (w) ld_edge<V>(w, (i * T + t) * V, H, 0.f, wv[i]);
+    }
+    const float inv = 1.0f / (float)H;
+    int odd = 0;
+    for (long long row = (long long)blockIdx.x * ROWS + threadIdx.x / T; row < R; row += (long long)gridDim.x * ROWS, odd ^= 1) {
+        float d[NV][V], h[NV][V], sg = 0.f, sgx = 0.f;
+        const float mu = mean[row], rs = rstd[row];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            ld_edge<V>(dy + row * lddy, (i * T + t) * V, H, 0.f, d[i]);     // behind the end dy = 0: nothing is added
+            ld_edge<V>(x + row * ldx, (i * T + t) * V, H, 0.f, h[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                h[i][j] = (h[i][j] - mu) * rs;
+                aw[i][j] += d[i][j] * h[i][j];
+                ab[i][j] += d[i][j];
+                d[i][j] *= wv[i][j];
+                sg += d[i][j];
+                sgx += d[i][j] * h[i][j];
+            }
+        const float mg = row_sum<T>(sg, part[odd][0]) * inv, mgx = row_sum<T>(sgx, part[odd][1]) * inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = rs * (d[i][j] - mg - h[i][j] * mgx);
+            st_edge<V>(dx + row * lddx, (i * T + t) * V, H, o);
+        }
+    }
+    if (!ws) return;
+    float* out = ws + (size_t)blockIdx.x * 2 * ldp;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float(&a)[NV][V] = k ? ab : aw;
+        if constexpr (T == 64) {                     // the block's four waves, added in their order
+            for (int wave = 0; wave < 4; ++wave) {
+                if ((threadIdx.x >> 6) == wave)
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            float& c = comb[(i * V + j) * 64 + t];
+                            c = wave ? c + a[i][j] : a[i][j];
+                            if (wave == 3) a[i][j] = c;
+                        }
+                __syncthreads();
+            }
+            if ((threadIdx.x >> 6) == 3)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) st_edge<V>(out + k * ldp, (i * T + t) * V, H, a[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) st_edge<V>(out + k * ldp, (i * T + t) * V, H, a[i]);
+        }
+    }
+}
+
+// long rows: dx row by row (two walks over the row), and the column sums by a kernel of their own
+template <typename TX, typename TD, typename TW>
+__global__ __launch_bounds__(256) void layer_norm_bwd_long_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
+                                                                  const float* mean, const float* rstd, const TW* w, TX* dx,
+                                                                  long long lddx, int R, int H) {
+    __shared__ float part[2][2][4];
+    const float inv = 1.0f / (float)H;
+    int odd = 0;
+    for (long long row = blockIdx.x; row < R; row += gridDim.x, odd ^= 1) {
+        const float mu = mean[row], rs = rstd[row];
+        float sg = 0.f, sgx = 0.f;
+        for (int c = threadIdx.x * 4; c < H; c += 1024) {
+            float d[4], v[4], wv[4] = {1.f, 1.f, 1.f, 1.f};
+            ld_edge<4>(dy + row * lddy, c, H, 0.f, d);
+            ld_edge<4>(x + row * ldx, c, H, 0.f, v);
+            if (w) ld_edge<4>(w, c, H, 0.f, wv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float g = d[j] * wv[j];
+                sg += g;
+                sgx += g * ((v[j] - mu) * rs);
+            }
+        }
+        const float mg = row_sum<256>(sg, part[odd][0]) * inv, mgx = row_sum<256>(sgx, part[odd][1]) * inv;
+        for (int c = threadIdx.x * 4; c < H; c += 1024) {
+            float d[4], v[4], wv[4] = {1.f, 1.f, 1.f, 1.f};
+            ld_edge<4>(dy + row * lddy, c, H, 0.f, d);
+            ld_edge<4>(x + row * ldx, c, H, 0.f, v);
+            if (w) ld_edge<4>(w, c, H, 0.f, wv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = rs * (d[j] * wv[j] - mg - (v[j] - mu) * rs * mgx);
+            st_edge<4>(dx + row * lddx, c, H, v);
+        }
+    }
+}
+
+template <typename TX, typename TD>
+__global__ __launch_bounds__(256) void layer_norm_bwd_columns_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
+                                                                     const float* mean, const float* rstd, float* ws, int ldp,
+                                                                     int R, int H) {
+    const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
+    float aw[4] = {0.f, 0.f, 0.f, 0.f}, ab[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c >= H) return;
+    for (long long row = blockIdx.y; row < R; row += gridDim.y) {
+        float d[4], v[4];
+        ld_edge<4>(dy + row * lddy, c, H, 0.f, d);
+        ld_edge<4>(x + row * ldx, c, H, 0.f, v);
+        const float mu = mean[row], rs = rstd[row];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            aw[j] += d[j] * ((v[j] - mu) * rs);
+            ab[j] += d[j];
+        }
+    }
+    float* out = ws + (size_t)blockIdx.y * 2 * ldp;
+    st_edge<4>(out, c, H, aw);
+    st_edge<4>(out + ldp, c, H, ab);
+}
+
+// dweight / dbias (+)= the partial sums, in the order of the blocks that left them: 8 lanes of four columns, 32 slots
+__global__ __launch_bounds__(256) void layer_norm_bwd_join_kernel(const float* ws, int ldp, int parts, float* dweight,
+                                                                  float* dbias, int accumulate, int H) {
+    __shared__ f32x4 sum[32][8];
+    const int lane = threadIdx.x & 7, slot = threadIdx.x >> 3, c = (blockIdx.x * 8 + lane) * 4;
+    const float* src = ws + (size_t)blockIdx.y * ldp + c;
+    float* dst = blockIdx.y ? dbias : dweight;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (c < ldp)
+        for (int p = slot; p < parts; p += 32) s += *(const f32x4*)(src + (size_t)p * 2 * ldp);
+    sum[slot][lane] = s;
+    __syncthreads();
+    for (int h = 16; h > 0; h >>= 1) {
+        if (slot < h) sum[slot][lane] += sum[slot + h][lane];
+        __syncthreads();
+    }
+    if (slot || !dst) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (c + j < H) dst[c + j] = accumulate ? dst[c + j] + sum[0][lane][j] : sum[0][lane][j];
+}
+
+__global__ __launch_bounds__(256) void fill_zero_kernel(float* a, float* b, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    if (a) a[i] = 0.f;
+    if (b) b[i] = 0.f;
+}
+
+constexpr int IN_REGISTERS = 8192;        // longest row that the register kernels take
+
+inline int norm_blocks(long long R, int rows_per_block, int per_cu) {
+    return (int)std::min<long long>((R + rows_per_block - 1) / rows_per_block, (long long)per_cu * cu_count());
+}
+inline int lanes_per_row(int H) { return H <= 2048 ? 64 : 256; }
+inline int bwd_parts(int R, int H) {
+    if (H > IN_REGISTERS) return (int)std::min<long long>(R, 64);
+    return norm_blocks(R, 256 / lanes_per_row(H), 2);
+}
+inline int ld_parts(int H) { return (H + 3) / 4 * 4; }
+
+template <typename TX, typename TY, typename TW>
+int launch_ln(const void* x, long long ldx, const void* w, const void* b, float eps, void* y, long long ldy, float* mean,
+              float* rstd, int R, int H, hipStream_t st) {
+    constexpr int V = sizeof(TX) == 2 ? 8 : 4, U = 8 / V;
+#define LN(NV, T)                                                                                                              \
+    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, TW, V, NV, T>), dim3(norm_blocks(R, 256 / T, 8)), dim3(256), 0, st, (const TX*)x, \
+                       ldx, (const TW*)w, (const TW*)b, eps, (TY*)y, ldy, mean, rstd, R, H)
+    if (H <= 512) LN(U, 64);
+    else if (H <= 1024) LN(2 * U, 64);
+    else if (H <= 2048) LN(4 * U, 64);
+    else if (H <= 4096) LN(2 * U, 256);
+    else if (H <= IN_REGISTERS) LN(4 * U, 256);
+    else
+        hipLaunchKernelGGL((layer_norm_long_kernel<TX, TY, TW>), dim3(norm_blocks(R, 1, 8)), dim3(256), 0, st, (const TX*)x, ldx,
+                           (const TW*)w, (const TW*)b, eps, (TY*)y, ldy, mean, rstd, R, H);
+#undef LN
+    STDIFF_LAUNCH_STATUS();
+    return STDIFF_OK;
+}
+
+template <typename TX, typename TD, typename TW>
+int launch_ln_grad(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
+                   const void* w, void* dx, long long lddx, float* ws, int parts, int R, int H, hipStream_t st) {
+    constexpr int V = sizeof(TX) == 2 ? 8 : 4, U = 8 / V;
+    const int ldp = ld_parts(H);
+#define LN(NV, T)                                                                                                               \
+    hipLaunchKernelGGL((layer_norm_bwd_kernel<TX, TD, TW, V, NV, T>), dim3(parts), dim3(256), 0, st, (const TD*)dy, lddy, (const TX*)x, \
+                       ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, ws, ldp, R, H)
+    if (H <= 512) LN(U, 64);
+    else if (H <= 1024) LN(2 * U, 64);
+    else if (H <= 2048) LN(4 * U, 64);
+    else if (H <= 4096) LN(2 * U, 256);
+    else if (H <= IN_REGISTERS) LN(4 * U, 256);
+    else {
+        if (ws)
+            hipLaunchKernelGGL((layer_norm_bwd_columns_kernel<TX, TD>), dim3(cdiv(H, 1024), parts), dim3(256), 0, st, (const TD*)dy,
+                               lddy, (const TX*)x, ldx, mean, rstd, ws, ldp, R, H);
+        hipLaunchKernelGGL((layer_norm_bwd_long_kernel<TX, TD, TW>), dim3(norm_blocks(R, 1, 8)), dim3(256), 0, st, (const TD*)dy,
+                           lddy, (const TX*)x, ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, R, H);
+    }
+#undef LN
+    STDIFF_LAUNCH_STATUS();
+    return STDIFF_OK;
+}
+
+inline bool dtype_ok(int dt) { return dt == STDIFF_F32 || dt == STDIFF_BF16; }
+inline bool at_element(const void* p, int dt) { return ((uintptr_t)p & (dt == STDIFF_BF16 ? 1 : 3)) == 0; }
+
+}  // namespace
+
+extern "C" int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, const void* weight, const void* bias, int w_dtype,
+                                 float eps, void* y, long long ldy, int y_dtype, float* mean, float* rstd, int R, int H,
+                                 void* stream) {
+    STDIFF_CHECK_ARG(R >= 0 && H > 0 && (R == 0 || (x && y)) && ldx >= 0 && ldy >= H && eps >= 0.f);
+    STDIFF_CHECK_ARG(dtype_ok(x_dtype) && dtype_ok(y_dtype) && dtype_ok(w_dtype));
+    if (R == 0) return STDIFF_OK;
+    if (!at_element(x, x_dtype) || !at_element(y, y_dtype) || !at_element(weight, w_dtype) || !at_element(bias, w_dtype) ||
+        !at_element(mean, STDIFF_F32) || !at_element(rstd, STDIFF_F32))
+        return STDIFF_ERR_ALIGN;
+#define LN(TX, TY, TW) launch_ln<TX, TY, TW>(x, ldx, weight, bias, eps, y, ldy, mean, rstd, R, H, (hipStream_t)stream)
+    switch ((x_dtype == STDIFF_BF16) * 4 + (y_dtype == STDIFF_BF16) * 2 + (w_dtype == STDIFF_BF16)) {
+        case 0: return LN(float, float, float);
+        case 1: return LN(float, float, bf16_t);
+        case 2: return LN(float, bf16_t, float);
+        case 3: return LN(float, bf16_t, bf16_t);
+        case 4: return LN(bf16_t, float, float);
+        case 5: return LN(bf16_t, float, bf16_t);
+        case 6: return LN(bf16_t, bf16_t, float);
+        default: return LN(bf16_t, bf16_t, bf16_t);
+    }
+#undef LN
+}
+
+extern "C" long long stdiff_layer_norm_bwd_workspace(int R, int H) {
+    if (R < 0 || H <= 0) return STDIFF_ERR_ARG;
+    return (long long)bwd_parts(R, H) * 2 * ld_parts(H) * 4;
+}
+
+extern "C" int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const void* x, long long ldx, int x_dtype,
+                                     const float* mean, const float* rstd, const void* weight, int w_dtype, void* dx,
+                                     long long lddx, float* dweight, float* dbias, int accumulate, float* workspace,
+                                     long long workspace_bytes, int R, int H, void* stream) {
+    STDIFF_CHECK_ARG(R >= 0 && H > 0 && (R == 0 || (dy && x && mean && rstd && dx)) && lddy >= 0 && ldx >= 0 && lddx >= H);
+    STDIFF_CHECK_ARG(dtype_ok(dy_dtype) && dtype_ok(x_dtype) && dtype_ok(w_dtype));
+    if (!at_element(dy, dy_dtype) || !at_element(x, x_dtype) || !at_element(dx, x_dtype) || !at_element(weight, w_dtype) ||
+        !at_element(mean, STDIFF_F32) || !at_element(rstd, STDIFF_F32) || !at_element(dweight, STDIFF_F32) ||
+        !at_element(dbias, STDIFF_F32) || ((uintptr_t)workspace & 15))
+        return STDIFF_ERR_ALIGN;
+    const bool params = dweight || dbias;
+    hipStream_t st = (hipStream_t)stream;
+    if (R == 0) {
+        if (params && !accumulate) {
+            hipLaunchKernelGGL(fill_zero_kernel, dim3(cdiv(H, 256)), dim3(256), 0, st, dweight, dbias, H);
+            STDIFF_LAUNCH_STATUS();
+        }
+        return STDIFF_OK;
+    }
+    const int parts = bwd_parts(R, H);
+    if (params && (!workspace || workspace_bytes < stdiff_layer_norm_bwd_workspace(R, H))) return STDIFF_ERR_WORKSPACE;
+    float* ws = params ? workspace : nullptr;
+    int rc;
+#define LN(TX, TD, TW) rc = launch_ln_grad<TX, TD, TW>(dy, lddy, x, ldx, mean, rstd, weight, dx, lddx, ws, parts, R, H, st)
+    switch ((x_dtype == STDIFF_BF16) * 4 + (dy_dtype == STDIFF_BF16) * 2 + (w_dtype == STDIFF_BF16)) {
+        case 0: LN(float, float, float); break;
+        case 1: LN(float, float, bf16_t); break;
+        case 2: LN(float, bf16_t, float); break;
+        case 3: LN(float, bf16_t, bf16_t); break;
+        case 4: LN(bf16_t, float, float); break;
+        case 5: LN(bf16_t, float, bf16_t); break;
+        case 6: LN(bf16_t, bf16_t, float); break;
+        default: LN(bf16_t, bf16_t, bf16_t); break;
+    }
+#undef LN
+    if (rc != STDIFF_OK || !params) return rc;
+    hipLaunchKernelGGL(layer_norm_bwd_join_kernel, dim3(cdiv(H, 32), 2), dim3(256), 0, st, workspace, ld_parts(H), parts, dweight,
+                       dbias, accumulate, H);
+    STDIFF_LAUNCH_STATUS();
+    return STDIFF_OK;
+}

@@ -379,6 +379,301 @@ def clip_adamw(p, g, m, v, sumsq, step_dev, scal, lr, max_norm=1.0, grad_scale=1
     check(lib().stdiff_clip_adamw(C.byref(a), stream()))
 
 
+# ---------------------------------------------------------------- norm, optimizer and 8-bit product beside the DiT
+def _one_device(first, *rest):
+    """The device all of these tensors are on (None entries are skipped)."""
+    if not first.is_cuda:
+        require_gpu(first)
+    dev = first.device
+    for t in rest:
+        if t is not None and t.device != dev:
+            require_gpu(t)
+            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+    return dev
+
+
+def _enqueue(dev, call):
+    """check(call(stream)) with the stream that is current on `dev`, `dev` being the current device meanwhile."""
+    if dev.index == torch.cuda.current_device():
+        check(call(torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            check(call(torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _read_ld(t, name, shape=None):
+    """Leading dimension of a matrix that is only read: rows may overlap or be one row broadcast."""
+    if t.dim() != 2 or (shape is not None and t.shape != shape):
+        raise ValueError(f"{name}: a matrix{'' if shape is None else f' of {tuple(shape)}'} is needed, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the elements of a row have to be neighbours, got strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _write_ld(t, name, shape):
+    ld = _read_ld(t, name, shape)
+    if t.shape[0] > 1 and ld < t.shape[1]:
+        raise ValueError(f"{name}: rows of an output may not overlap, got strides {t.stride()}")
+    return ld
+
+
+def _vector(t, name, n, *dtypes):
+    """None, or the address of a contiguous vector of n elements of one of these types."""
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name}: a contiguous vector of {n} elements of {' / '.join(str(d) for d in dtypes)} is needed, "
+                         f"got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _affine(weight, bias, H):
+    """(address, address, dtype code) of a norm's weight and bias, which share one dtype."""
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: one dtype is needed")
+    one = weight if weight is not None else bias
+    return _vector(weight, "weight", H, *_FLOATS), _vector(bias, "bias", H, *_FLOATS), F32 if one is None else dt_of(one)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, mean=None, rstd=None):
+    """LayerNorm of the rows of x [R, H] with a weight and a bias per column (None: 1 and 0; one dtype for both).
+    x and out: fp32 or a 16-bit type, any row stride, any H.  mean / rstd (fp32 [R], optional): receive the statistics
+    that layer_norm_bwd takes.  out may be x."""
+    dev = _one_device(x, weight, bias, out, mean, rstd)
+    ldx = _read_ld(x, "x")
+    R, H = x.shape
+    if out is None:
+        out = torch.empty((R, H), device=dev, dtype=out_dtype or x.dtype)
+    ldy = _write_ld(out, "out", x.shape)
+    w, b, wdt = _affine(weight, bias, H)
+    mp, rp = _vector(mean, "mean", R, torch.float32), _vector(rstd, "rstd", R, torch.float32)
+    fn = lib_for(x, out, weight, bias).stdiff_layer_norm
+    _enqueue(dev, lambda st: fn(x.data_ptr(), ldx, dt_of(x), w, b, wdt, eps, out.data_ptr(), ldy, dt_of(out), mp, rp, R, H, st))
+    return out
+
+
+def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None, accumulate=False, workspace=None):
+    """Backward of layer_norm from its mean / rstd: (dx, dweight, dbias).  dx has x's dtype (allocated unless given; it may be
+    dy or x).  dweight / dbias are fp32 [H]: with a weight both are allocated unless given, without one those that are
+    given are formed (else None); accumulate=True adds to what the given ones hold.  They are sums over the rows in a
+    fixed order: the same bits every run.
+    workspace (fp32, at least layer_norm_bwd_workspace(R, H) floats; allocated unless given): give one of its own to a
+    call that is captured into an ops.Graph."""
+    dev = _one_device(x, dy, mean, rstd, weight, dx, dweight, dbias, workspace)
+    ldx = _read_ld(x, "x")
+    R, H = x.shape
+    lddy = _read_ld(dy, "dy", x.shape)
+    if accumulate and (dweight is None and dbias is None):
+        raise ValueError("accumulate: there is no dweight or dbias to add to")
+    if dx is None:
+        dx = torch.empty((R, H), device=dev, dtype=x.dtype)
+    elif dx.dtype != x.dtype:
+        raise TypeError(f"dx is {dx.dtype}, x {x.dtype}")
+    lddx = _write_ld(dx, "dx", x.shape)
+    if weight is not None and not accumulate:
+        if dweight is None:
+            dweight = torch.empty((H,), device=dev, dtype=torch.float32)
+        if dbias is None:
+            dbias = torch.empty((H,), device=dev, dtype=torch.float32)
+    w, _, wdt = _affine(weight, None, H)
+    if mean is None or rstd is None:
+        raise ValueError("mean and rstd of the forward are needed")
+    mp, rp = _vector(mean, "mean", R, torch.float32), _vector(rstd, "rstd", R, torch.float32)
+    dw, db = _vector(dweight, "dweight", H, torch.float32), _vector(dbias, "dbias", H, torch.float32)
+    lb = lib_for(x, dy, weight)
+    if workspace is None and (dw or db):
+        workspace = torch.empty((layer_norm_bwd_workspace(R, H),), device=dev, dtype=torch.float32)
+    ws, nb = _workspace(workspace)
+    _enqueue(dev, lambda st: lb.stdiff_layer_norm_bwd(
+        dy.data_ptr(), lddy, dt_of(dy), x.data_ptr(), ldx, dt_of(x), mp, rp, w, wdt, dx.data_ptr(), lddx, dw, db,
+        int(accumulate), ws, nb, R, H, st))
+    return dx, dweight, dbias
+
+
+def layer_norm_bwd_workspace(R, H):
+    """Floats that layer_norm_bwd needs as workspace for x [R, H]."""
+    n = lib().stdiff_layer_norm_bwd_workspace(R, H)
+    if n < 0:
+        raise ValueError(f"layer_norm_bwd_workspace: bad size {R} x {H}")
+    return n // 4
+
+
+def _workspace(t):
+    """(address, bytes) of a workspace tensor (None: none)."""
+    if t is None:
+        return None, 0
+    if not t.is_contiguous():
+        raise ValueError("workspace: a contiguous tensor is needed")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+class AdamWTensors:
+    """Parameters and their states as adamw_multi takes them (made by adamw_multi_args; holds the tensors)."""
+
+    def __init__(self, params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, weight_decay):
+        n = len(params)
+        none = [None] * n
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+        self.tensors = [list(params), list(exp_avg), list(exp_avg_sq), list(exp_avg_scale or none), list(exp_avg_sq_scale or none)]
+        if any(len(t) != n for t in self.tensors) or len(decay) != n:
+            raise ValueError("adamw_multi_args: lists of different lengths")
+        self.state_bits = 8 if n and exp_avg[0].dtype == torch.float8_e4m3fn else 32
+        kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
+        self.table = (L.AdamWTensor * max(n, 1))()
+        self.device = params[0].device if n else None
+        self.sizes = [p.numel() for p in params]
+        for i, (p, m, v, ms, vs) in enumerate(zip(*self.tensors)):
+            _one_device(params[0], p, m, v, ms, vs)
+            if m.dtype != kind or v.dtype != kind:
+                raise TypeError(f"tensor {i}: states are {m.dtype} and {v.dtype}, {kind} is needed like in the first")
+            if m.numel() != p.numel() or v.numel() != p.numel():
+                raise ValueError(f"tensor {i}: states of {m.numel()} and {v.numel()} elements for {p.numel()} parameters")
+            for what, t in (("param", p), ("exp_avg", m), ("exp_avg_sq", v)):
+                if not t.is_contiguous():
+                    raise ValueError(f"tensor {i}: {what} is not contiguous")
+            q = self.table[i]
+            if self.state_bits == 8:
+                blocks = round_up(p.numel(), 256) // 256
+                if ms is None or vs is None:
+                    raise ValueError("8-bit states need exp_avg_scale and exp_avg_sq_scale")
+                q.exp_avg_scale = _vector(ms, f"exp_avg_scale[{i}]", blocks, torch.float32)
+                q.exp_avg_sq_scale = _vector(vs, f"exp_avg_sq_scale[{i}]", blocks, torch.float32)
+            elif ms is not None or vs is not None:
+                raise ValueError("32-bit states have no scales")
+            q.param, q.exp_avg, q.exp_avg_sq, q.n = p.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel()
+            q.param_dtype, q.weight_decay = dt_of(p), decay[i]
+        self.half = {p.dtype for p in params} - {torch.float32}
+        if len(self.half) > 1:
+            raise TypeError("float16 and bfloat16 parameters in one adamw_multi")
+
+
+def adamw_multi_args(params, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, weight_decay=0.0):
+    """What adamw_multi updates: lists of contiguous tensors, one entry per parameter (fp32 or one 16-bit type; views into
+    larger buffers are fine).  exp_avg / exp_avg_sq: fp32, or torch.float8_e4m3fn with a vector of
+    ceil(numel / 256) fp32 scales per tensor in exp_avg_scale / exp_avg_sq_scale (adamw8_state makes all four).
+    weight_decay: one number, or one per tensor.  The states are read and written in place by every step."""
+    return AdamWTensors(params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, weight_decay)
+
+
+def adamw8_state(param):
+    """8-bit state of one parameter before its first step: (exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale), all
+    zero.  exp_avg.float() * scale (of its block of 256) is the first moment, exp_avg_sq.float() * scale the ROOT of
+    the second."""
+    require_gpu(param)
+    blocks = round_up(param.numel(), 256) // 256
+    m, v = (torch.zeros(param.shape, device=param.device, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+    ms, vs = (torch.zeros((blocks,), device=param.device, dtype=torch.float32) for _ in range(2))
+    return m, v, ms, vs
+
+
+def adamw_multi_workspace(n_tensors):
+    """Floats that adamw_multi needs as workspace for this many tensors."""
+    n = lib().stdiff_adamw_multi_workspace(n_tensors)
+    if n < 0:
+        raise ValueError(f"adamw_multi_workspace: {n_tensors} tensors")
+    return n // 4
+
+
+def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=(0.9, 0.999), eps=1e-8, norm=None, workspace=None):
+    """One AdamW step over all tensors of `args` (adamw_multi_args).  grads: one contiguous tensor per parameter, fp32 or a
+    16-bit type, or None (that parameter and its state stay as they are).  step_dev: int32 [1] on the device, the steps
+    done so far; incremented.  max_norm: clip by the norm over all gradients (None: no clipping); norm (fp32 [1],
+    optional) receives that norm; grad_scale multiplies every gradient first (1 / world size, 1 / loss scale).
+    workspace (fp32, at least adamw_multi_workspace(len(grads)) floats; allocated unless given): give one of its own to a
+    call that is captured into an ops.Graph.  A captured step keeps lr and the other numbers it was captured with."""
+    table, n = args.table, len(args.sizes)
+    if len(grads) != n:
+        raise ValueError(f"adamw_multi: {len(grads)} gradients for {n} parameters")
+    dev = args.device if n else step_dev.device
+    _one_device(step_dev, norm, workspace)
+    kinds = set(args.half)
+    for q, g, size in zip(table, grads, args.sizes):
+        if g is None:
+            q.n = 0
+            continue
+        if g.numel() != size or g.device != dev or not g.is_contiguous():
+            raise ValueError(f"adamw_multi: a contiguous gradient of {size} elements on {dev} is needed, got {tuple(g.shape)} on {g.device}")
+        dt = g.dtype
+        if dt != torch.float32:
+            kinds.add(dt)
+        q.grad, q.grad_dtype, q.n = g.data_ptr(), dt_of(g), size
+    if step_dev.device != dev:
+        raise ValueError(f"step_dev on {step_dev.device}, the parameters on {dev}")
+    if len(kinds) > 1:
+        raise TypeError("float16 and bfloat16 tensors in one adamw_multi")
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError(f"max_norm has to be positive (or None), got {max_norm}")
+    if workspace is None:
+        workspace = torch.empty((adamw_multi_workspace(n),), device=dev, dtype=torch.float32)
+    a = L.AdamWMultiArgs()
+    a.tensors, a.n_tensors, a.state_bits = table, n, args.state_bits
+    a.step_dev, a.norm = _vector(step_dev, "step_dev", 1, torch.int32), _vector(norm, "norm", 1, torch.float32)
+    a.workspace, a.workspace_bytes = _workspace(workspace)
+    a.lr, a.beta1, a.beta2, a.eps = lr, betas[0], betas[1], eps
+    a.max_norm, a.grad_scale = max_norm or 0.0, grad_scale
+    fn = lib(torch.float16 in kinds).stdiff_adamw_multi
+    _enqueue(dev, lambda st: fn(C.byref(a), st))
+
+
+def quantize_rows(x, out=None, scale=None):
+    """(q, scale): the rows of x [R, K] (fp32 or a 16-bit type) as int8 with one fp32 scale each, scale = max |x| / 127 and
+    q = rint(x * (127 / max |x|)).  q is a [R, K] view of rows that begin on 16-byte borders, zeros behind K, as gemm_i8
+    takes them (a given `out` has to be such a view).  A row that holds an infinity or a NaN gets a scale that is not
+    finite."""
+    dev = _one_device(x, out, scale)
+    ldx = _read_ld(x, "x")
+    R, K = x.shape
+    if out is None:
+        out = torch.empty((R, round_up(K, 16)), device=dev, dtype=torch.int8)[:, :K]
+    ldq = _rows16(out, "out", (R, K))
+    if scale is None:
+        scale = torch.empty((R,), device=dev, dtype=torch.float32)
+    sp = _vector(scale, "scale", R, torch.float32)
+    fn = lib_for(x).stdiff_quantize_rows
+    _enqueue(dev, lambda st: fn(x.data_ptr(), ldx, dt_of(x), out.data_ptr(), ldq, sp, R, K, st))
+    return out, scale
+
+
+def _rows16(t, name, shape=None):
+    """Leading dimension of an int8 matrix whose rows begin on 16-byte borders and may be touched up to the next border."""
+    if t.dtype != torch.int8:
+        raise TypeError(f"{name}: int8 is needed, got {t.dtype}")
+    ld = _read_ld(t, name, shape)
+    rows, kp = t.shape[0], round_up(t.shape[1], 16)
+    ld = ld if rows > 1 else kp
+    if rows and (ld % 16 or ld < kp or t.data_ptr() % 16 or
+                 t.storage_offset() + (rows - 1) * ld + kp > t.untyped_storage().nbytes()):
+        raise ValueError(f"{name}: rows have to begin on 16-byte borders and to reach the next border behind their end in memory, "
+                         f"as quantize_rows lays them out; got shape {tuple(t.shape)}, strides {t.stride()}")
+    return ld
+
+
+def gemm_i8(A, a_scale, W, w_scale, bias=None, out=None, out_dtype=torch.float32):
+    """out[M, N] = (A[M, K] @ W[N, K]^T) * a_scale[M, None] * w_scale[N] + bias: int8 operands as quantize_rows makes them,
+    the sum over K exact in int32 (K <= 131071), scales and bias fp32, out fp32 or a 16-bit type."""
+    dev = _one_device(A, a_scale, W, w_scale, bias, out)
+    lda, ldw = _rows16(A, "A"), _rows16(W, "W")
+    (M, K), N = A.shape, W.shape[0]
+    if W.shape[1] != K:
+        raise ValueError(f"A has {K} columns, W {W.shape[1]}")
+    if a_scale is None or w_scale is None:
+        raise ValueError("a_scale and w_scale are needed")
+    if out is None:
+        out = torch.empty((M, N), device=dev, dtype=out_dtype)
+    a = L.GemmI8Args()
+    a.M, a.N, a.K = M, N, K
+    a.A, a.lda, a.W, a.ldw = A.data_ptr(), lda, W.data_ptr(), ldw
+    a.a_scale, a.w_scale = _vector(a_scale, "a_scale", M, torch.float32), _vector(w_scale, "w_scale", N, torch.float32)
+    a.bias = _vector(bias, "bias", N, torch.float32)
+    a.C, a.ldc, a.c_dtype = out.data_ptr(), _write_ld(out, "out", (M, N)), dt_of(out)
+    fn = lib_for(out).stdiff_gemm_i8
+    _enqueue(dev, lambda st: fn(C.byref(a), st))
+    return out
+
+
 class Graph:
     """hipGraph capture of everything enqueued on the current stream between begin() and end()."""
 

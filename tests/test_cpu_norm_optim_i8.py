@@ -1,0 +1,167 @@
+"""CPU: what the entry points of the layer norm, AdamW and 8-bit product refuse before they launch anything (through the C
+ABI with addresses that are never read), their workspace sizes, their structs, and the checks of the Python layer."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ARG, SHAPE, ALIGN, WORKSPACE = -1, -2, -3, -6
+AT = 1 << 20                                            # an aligned address that nothing lies at
+
+
+@pytest.fixture(scope="module", params=[False, True], ids=["bf16", "fp16"])
+def lib(request):
+    from stdiff_amd import _lib
+    return _lib.lib(request.param)
+
+
+def test_layer_norm_refuses(lib):
+    def fwd(x=AT, ldx=64, xd=0, w=AT, b=AT, wd=0, eps=1e-6, y=AT, ldy=64, yd=0, mean=None, rstd=None, R=4, H=64):
+        return lib.stdiff_layer_norm(x, ldx, xd, w, b, wd, eps, y, ldy, yd, mean, rstd, R, H, None)
+    for kw in (dict(x=None), dict(y=None), dict(R=-1), dict(H=0), dict(ldx=-1), dict(ldy=63), dict(eps=-1.0), dict(eps=float("nan")),
+               dict(xd=2), dict(yd=-1), dict(wd=7)):
+        assert fwd(**kw) == ARG, kw
+    for kw in (dict(x=AT + 2), dict(y=AT + 1, yd=1), dict(w=AT + 3), dict(mean=AT + 2), dict(rstd=AT + 1)):
+        assert fwd(**kw) == ALIGN, kw
+    assert fwd(R=0, x=None, y=None) == 0
+
+
+def test_layer_norm_bwd_refuses(lib):
+    need = lib.stdiff_layer_norm_bwd_workspace(100, 1001)
+    assert need > 0 and lib.stdiff_layer_norm_bwd_workspace(-1, 5) == ARG and lib.stdiff_layer_norm_bwd_workspace(5, 0) == ARG
+    assert lib.stdiff_layer_norm_bwd_workspace(0, 5) >= 0
+
+    def bwd(dy=AT, ldd=1001, dd=0, x=AT, ldx=1001, xd=0, mean=AT, rstd=AT, w=AT, wd=0, dx=AT, lddx=1001, dw=AT, db=AT, ws=AT, nb=need, R=100, H=1001):
+        return lib.stdiff_layer_norm_bwd(dy, ldd, dd, x, ldx, xd, mean, rstd, w, wd, dx, lddx, dw, db, 0, ws, nb, R, H, None)
+    for kw in (dict(dy=None), dict(x=None), dict(mean=None), dict(rstd=None), dict(dx=None), dict(lddx=1000), dict(ldd=-1), dict(R=-2), dict(H=-1),
+               dict(dd=2), dict(xd=3), dict(wd=-1)):
+        assert bwd(**kw) == ARG, kw
+    for kw in (dict(dy=AT + 1), dict(dx=AT + 2), dict(dw=AT + 2), dict(ws=AT + 4)):
+        assert bwd(**kw) == ALIGN, kw
+    for kw in (dict(ws=None), dict(nb=need - 1), dict(nb=0), dict(db=None, nb=0)):
+        assert bwd(**kw) == WORKSPACE, kw
+    assert bwd(R=0, dw=None, db=None, ws=None, nb=0, dy=None, x=None, dx=None, mean=None, rstd=None) == 0
+
+
+def test_adamw_multi_refuses(lib):
+    from stdiff_amd import _lib as L
+    need = lib.stdiff_adamw_multi_workspace(2)
+    assert need > 0 and lib.stdiff_adamw_multi_workspace(-1) == ARG
+    assert lib.stdiff_adamw_multi_workspace(500) > need
+
+    def step(bits=32, n=2, change=None, **kw):
+        t = (L.AdamWTensor * 2)()
+        for q in t:
+            q.param = q.grad = q.exp_avg = q.exp_avg_sq = q.exp_avg_scale = q.exp_avg_sq_scale = AT
+            q.n = 1000
+        for k, v in (change or {}).items():
+            setattr(t[1], k, v)
+        a = L.AdamWMultiArgs()
+        a.tensors, a.n_tensors, a.state_bits = t, n, bits
+        a.step_dev, a.workspace, a.workspace_bytes = AT, AT, need
+        a.lr, a.beta1, a.beta2, a.eps, a.max_norm, a.grad_scale = 1e-3, 0.9, 0.999, 1e-8, 1.0, 1.0
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.stdiff_adamw_multi(C.byref(a), None)
+    assert lib.stdiff_adamw_multi(None, None) == ARG
+    for kw in (dict(bits=16), dict(n=-1), dict(step_dev=None), dict(workspace=None), dict(beta1=1.0), dict(beta2=-0.1), dict(beta1=float("nan")),
+               dict(eps=-1e-8), dict(lr=-1.0), dict(lr=float("nan")), dict(max_norm=float("nan"))):
+        assert step(**kw) == ARG, kw
+    for ch in (dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(n=-1), dict(param_dtype=2), dict(grad_dtype=9)):
+        assert step(change=ch) == ARG, ch
+    for ch in (dict(exp_avg_scale=None), dict(exp_avg_sq_scale=None)):
+        assert step(bits=8, change=ch) == ARG, ch
+    for ch in (dict(param=AT + 2), dict(grad=AT + 1), dict(exp_avg=AT + 2)):
+        assert step(change=ch) == ALIGN, ch
+    assert step(bits=8, change=dict(exp_avg_sq_scale=AT + 2)) == ALIGN
+    assert step(workspace_bytes=need - 1) == WORKSPACE
+    assert step(change=dict(n=1 << 45)) == SHAPE
+
+
+def test_product_refuses(lib):
+    from stdiff_amd import _lib as L
+
+    def prod(**kw):
+        a = L.GemmI8Args()
+        a.M, a.N, a.K = 10, 20, 100
+        a.A = a.W = a.a_scale = a.w_scale = a.bias = a.C = AT
+        a.lda = a.ldw = 112
+        a.ldc = 20
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.stdiff_gemm_i8(C.byref(a), None)
+    assert lib.stdiff_gemm_i8(None, None) == ARG
+    for kw in (dict(A=None), dict(W=None), dict(a_scale=None), dict(w_scale=None), dict(C=None), dict(M=-1), dict(N=-5), dict(K=0), dict(lda=96),
+               dict(ldw=96), dict(ldc=19), dict(c_dtype=2)):
+        assert prod(**kw) == ARG, kw
+    for kw in (dict(lda=120), dict(ldw=113), dict(A=AT + 8), dict(W=AT + 1), dict(C=AT + 2), dict(bias=AT + 2), dict(a_scale=AT + 1)):
+        assert prod(**kw) == ALIGN, kw
+    assert prod(K=131072, lda=131072, ldw=131072) == SHAPE and prod(lda=1 << 24) == SHAPE
+    assert prod(M=0, A=None, C=None) == 0 and prod(N=0) == 0
+
+    def quant(x=AT, ldx=100, xd=0, q=AT, ldq=112, s=AT, R=3, K=100):
+        return lib.stdiff_quantize_rows(x, ldx, xd, q, ldq, s, R, K, None)
+    for kw in (dict(x=None), dict(q=None), dict(s=None), dict(R=-1), dict(K=0), dict(ldx=-1), dict(ldq=100), dict(ldq=96), dict(xd=2)):
+        assert quant(**kw) == ARG, kw
+    for kw in (dict(ldq=120), dict(q=AT + 8), dict(x=AT + 2), dict(s=AT + 2)):
+        assert quant(**kw) == ALIGN, kw
+    assert quant(R=0, x=None, q=None, s=None) == 0
+
+
+def test_structs_match_the_header(tmp_path):
+    """sizes and offsets of the new structs as a C compiler lays them out"""
+    import subprocess
+    from stdiff_amd import _lib as L
+    pairs = (("stdiff_adamw_tensor", L.AdamWTensor), ("stdiff_adamw_multi_args", L.AdamWMultiArgs), ("stdiff_gemm_i8_args", L.GemmI8Args))
+    src = ['#include <stdio.h>', '#include <stddef.h>', '#include "stdiff_hip.h"', 'int main(void) {']
+    for name, cls in pairs:
+        src.append(f'printf("%zu\\n", sizeof({name}));')
+        src += [f'printf("%zu\\n", offsetof({name}, {f[0]}));' for f in cls._fields_]
+    (tmp_path / "t.c").write_text("\n".join(src + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(tmp_path / "t.c"), "-o", str(tmp_path / "t")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "t")], check=True, capture_output=True, text=True).stdout.split()]
+    want = []
+    for _, cls in pairs:
+        want += [C.sizeof(cls)] + [getattr(cls, f[0]).offset for f in cls._fields_]
+    assert got == want
+
+
+def test_python_checks():
+    from stdiff_amd import ops
+    t = torch.zeros(4, 6)
+    assert ops._read_ld(t, "t") == 6 and ops._read_ld(t[:, 1:4], "t") == 6 and ops._read_ld(t[:1].expand(3, 6), "t") == 0
+    assert ops._read_ld(torch.zeros(1, 6).expand(1, 6), "t") == 6
+    for bad in (t.t(), t[:, ::2], t[0], t[None]):
+        with pytest.raises(ValueError):
+            ops._read_ld(bad, "t")
+    with pytest.raises(ValueError, match="overlap"):
+        ops._write_ld(t[:1].expand(3, 6), "t", (3, 6))
+    with pytest.raises(ValueError):
+        ops._write_ld(t, "t", (4, 5))
+    assert ops._vector(None, "v", 3, torch.float32) is None
+    for bad in (torch.zeros(2), torch.zeros(6)[::2], torch.zeros(3, 1), torch.zeros(3).double()):
+        with pytest.raises(ValueError):
+            ops._vector(bad, "v", 3, torch.float32)
+    q = torch.zeros(5, 48, dtype=torch.int8)
+    base = q.data_ptr() % 16
+    if base == 0:
+        assert ops._rows16(q, "q") == 48 and ops._rows16(q[:, :40], "q") == 48 and ops._rows16(q[:1, :3], "q") == 16
+        assert ops._rows16(q[4:, 32:40], "q") == 16
+    for bad in (q[:, 1:20], torch.zeros(5, 40, dtype=torch.int8), torch.zeros(4 * 48 + 40, dtype=torch.int8).as_strided((5, 40), (48, 1))):
+        with pytest.raises(ValueError, match="borders"):
+            ops._rows16(bad, "q")
+    with pytest.raises(TypeError):
+        ops._rows16(q.float(), "q")
+
+
+def test_no_cpu_path():
+    from stdiff_amd import ops
+    x, q, s = torch.zeros(4, 16), torch.zeros(4, 16, dtype=torch.int8), torch.zeros(4)
+    p = torch.zeros(8)
+    for call in (lambda: ops.layer_norm(x), lambda: ops.layer_norm_bwd(x, x, s, s), lambda: ops.quantize_rows(x), lambda: ops.gemm_i8(q, s, q, s),
+                 lambda: ops.adamw_multi_args([p], [p], [p]), lambda: ops.adamw8_state(p)):
+        with pytest.raises(RuntimeError, match="MI355X"):
+            call()

@@ -1,0 +1,721 @@
+"""GPU: layer norm with its gradients, AdamW over many tensors and the 8-bit product against plain statements of the same
+operators in float64 on the CPU.
+
+Tolerances count roundings: u = 2^-24 is half a step of fp32; a sum of n terms in fp32 is off by at most (longest chain of
+additions) * u * (sum of magnitudes).  A row's sums pass at most 32 additions in a lane, 6 in a wave, 4 over waves and
+some more for longer rows: 64 is above all of them for H <= 20000.  A 16-bit result adds one rounding of its own."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+U = 2.0 ** -24
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from stdiff_amd import ops as _ops
+    return _ops
+
+
+def rnd(*shape, seed=0, scale=1.0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale
+
+
+def half_step(t):
+    return torch.finfo(t.dtype).eps / 2 if t.dtype != torch.float32 else U
+
+
+def within(got, want, tol, what):
+    got, want = got.detach().cpu().double(), want.double()
+    assert got.shape == want.shape
+    off = (got - want).abs() - tol
+    assert bool((off <= 0).all()), f"{what}: off by up to {float(off.max()):.3e} more than the tolerance"
+
+
+# ---------------------------------------------------------------- layer norm
+SIZES = [(1, 1), (1, 7), (3, 64), (5, 257), (130, 512), (2, 513), (7, 1001), (9, 1024), (3, 1025), (4, 2048), (3, 2051), (2, 4096),
+         (3, 4099), (2, 8192), (3, 8193), (2, 20000)]
+KINDS = [("fp32", "fp32", "fp32"), ("fp32", "bf16", "fp32"), ("bf16", "bf16", "fp32"), ("bf16", "fp32", "bf16"), ("fp16", "fp16", "fp16"),
+         ("fp32", "fp16", "fp16")]
+
+
+def norm64(x, w, b, eps):
+    x = x.double()
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    y = (x - mean) * rstd
+    if w is not None:
+        y = y * w.double()
+    return (y if b is None else y + b.double()), mean, rstd
+
+
+def norm_tol(x, w, b, mean, rstd):
+    """(x - mean) is off by 65 u of the row's magnitudes, rstd by 130 u of itself / 2, two products and a sum follow"""
+    x = x.double()
+    size = (x.abs() + x.abs().mean(1, keepdim=True) + (x - mean).abs()) * rstd
+    size = size * (1 if w is None else w.double().abs())
+    return 70 * U * size + U * (0 if b is None else b.double().abs()) + 1e-12
+
+
+@pytest.mark.parametrize("R,H", SIZES)
+@pytest.mark.parametrize("xt,yt,wt", KINDS)
+def test_layer_norm(ops, R, H, xt, yt, wt):
+    x = (rnd(R, H, seed=1) * 2 + rnd(R, 1, seed=2, scale=3.0)).to(DT[xt])
+    w, b = (1 + rnd(H, seed=3, scale=0.2)).to(DT[wt]), rnd(H, seed=4).to(DT[wt])
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    y = ops.layer_norm(x.to(DEV), w.to(DEV), b.to(DEV), eps=1e-5, out_dtype=DT[yt], mean=mean, rstd=rstd)
+    want, m64, r64 = norm64(x, w, b, 1e-5)
+    assert y.dtype == DT[yt]
+    within(y, want, norm_tol(x, w, b, m64, r64) * 1.01 + half_step(y) * want.abs() * 1.01, "y")
+    within(mean.view(-1, 1), m64, 65 * U * x.double().abs().mean(1, keepdim=True) + U * m64.abs(), "mean")
+    # relative error of rstd: half of the variance's; the variance of a row of one element is zero
+    within(rstd.view(-1, 1), r64, 70 * U * r64 + r64 ** 3 * 65 * U * x.double().abs().mean(1, keepdim=True) ** 2, "rstd")
+
+
+def test_layer_norm_without_parameters_and_strides(ops):
+    big = rnd(6, 300, seed=5).to(DEV)
+    x = big[::2, 3:260]                                       # rows 600 apart, first element at 12 bytes
+    for w, b in ((None, None), (rnd(257, seed=6), None), (None, rnd(257, seed=7))):
+        out = torch.full((3, 400), 7.0, device=DEV)
+        got = ops.layer_norm(x, None if w is None else w.to(DEV), None if b is None else b.to(DEV), out=out[:, 1:258])
+        assert got.data_ptr() == out[:, 1:258].data_ptr()
+        want, m, r = norm64(x.cpu(), w, b, 1e-6)
+        within(got, want, norm_tol(x.cpu(), w, b, m, r) + U * want.abs(), "strided")
+        assert bool((out[:, 0] == 7).all()) and bool((out[:, 258:] == 7).all())
+    one = rnd(1, 96, seed=8).to(DEV)
+    wide = ops.layer_norm(one.expand(5, 96))                  # one row for all
+    assert torch.equal(wide, ops.layer_norm(one).expand(5, 96))
+    for H in (96, 3000, 9000):
+        x = rnd(3, H, seed=9).to(DEV)
+        want = ops.layer_norm(x, eps=1e-6)
+        assert torch.equal(ops.layer_norm(x, out=x), want) and torch.equal(x, want)
+    assert ops.layer_norm(torch.empty(0, 64, device=DEV)).shape == (0, 64)
+
+
+def test_layer_norm_far_mean_and_special_rows(ops):
+    x = rnd(4, 1024, seed=10) + torch.tensor([[0.0], [1e4], [0.0], [0.0]])
+    x[2] = 3.25                                                # no spread: y is the bias
+    x[3, 17] = float("nan")
+    b = rnd(1024, seed=11)
+    y = ops.layer_norm(x.to(DEV), None, b.to(DEV)).cpu()
+    want, m, r = norm64(x, None, b, 1e-6)
+    # row 1: the mean's own error (65 u * 1e4) moves all elements alike, the spread keeps its digits
+    within(y[:3], want[:3], norm_tol(x, None, b, m, r)[:3] + U * want[:3].abs(), "far mean")
+    assert torch.equal(y[2], b) and bool(torch.isnan(y[3]).all()) and bool(torch.isfinite(y[:3]).all())
+
+
+GRAD_KINDS = [("fp32", "fp32", "fp32"), ("fp32", "bf16", "fp32"), ("bf16", "bf16", "bf16"), ("fp16", "fp16", "fp32"), ("bf16", "fp32", "fp32")]
+
+
+def grad64(dy, x, mean, rstd, w):
+    dy, x, mean, rstd = dy.double(), x.double(), mean.double().view(-1, 1), rstd.double().view(-1, 1)
+    hat = (x - mean) * rstd
+    g = dy if w is None else dy * w.double()
+    dx = rstd * (g - g.mean(1, keepdim=True) - hat * (g * hat).mean(1, keepdim=True))
+    return dx, (dy * hat).sum(0), dy.sum(0), hat, g
+
+
+def grad_tol(dy, rstd, hat, g):
+    """dx: sums of at most 65 additions over products of 3 roundings; columns: a chain of the rows of a wave and the joins"""
+    dy, rstd = dy.double(), rstd.double().view(-1, 1)
+    dx = rstd * (4 * g.abs() + 70 * g.abs().mean(1, keepdim=True) + 76 * hat.abs() * (g * hat).abs().mean(1, keepdim=True)) * U
+    chain = dy.shape[0] / 64 + 64
+    return dx + 1e-14, (chain + 4) * U * (dy * hat).abs().sum(0) + 1e-14, chain * U * dy.abs().sum(0) + 1e-14
+
+
+@pytest.mark.parametrize("R,H", SIZES + [(1500, 320), (2077, 1001), (40, 9001)])
+@pytest.mark.parametrize("xt,dt,wt", GRAD_KINDS)
+def test_layer_norm_bwd(ops, R, H, xt, dt, wt):
+    x = (rnd(R, H, seed=20) + rnd(R, 1, seed=21)).to(DT[xt])
+    dy, w = rnd(R, H, seed=22, scale=0.1).to(DT[dt]), (1 + rnd(H, seed=23, scale=0.2)).to(DT[wt])
+    _, mean, rstd = norm64(x, None, None, 1e-5)
+    mean, rstd = mean.view(-1).float(), rstd.view(-1).float()
+    dx, dw, db = ops.layer_norm_bwd(dy.to(DEV), x.to(DEV), mean.to(DEV), rstd.to(DEV), w.to(DEV))
+    wx, ww, wb, hat, g = grad64(dy, x, mean, rstd, w)
+    tx, tw, tb = grad_tol(dy, rstd, hat, g)
+    assert dx.dtype == x.dtype and dw.dtype == db.dtype == torch.float32
+    within(dx, wx, tx * 1.01 + half_step(dx) * wx.abs() * 1.01 + (2.0 ** -25 if xt == "fp16" else 0), "dx")   # fp16: half of its last step
+    within(dw, ww, tw, "dweight")
+    within(db, wb, tb, "dbias")
+
+
+@pytest.mark.parametrize("H", [48, 1024, 3000, 8200])
+def test_layer_norm_bwd_options(ops, H):
+    R = 37
+    big, bigdy = rnd(R, H + 5, seed=30).to(DEV), rnd(R, H + 3, seed=31).to(DEV)
+    x, dy, w = big[:, 2:H + 2], bigdy[:, 1:H + 1], rnd(H, seed=32).to(DEV)
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    ops.layer_norm(x, w, mean=mean, rstd=rstd)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    # the formulas' own statistics: against differences of the forward, in float64
+    wx, ww, wb, hat, g = grad64(dy.cpu(), x.cpu(), mean.cpu(), rstd.cpu(), w.cpu())
+    tx, tw, tb = grad_tol(dy.cpu(), rstd.cpu(), hat, g)
+    within(dx, wx, tx + U * wx.abs(), "strided dx")
+    again = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))           # a fixed order of additions
+    # accumulate, only one of the two, and none
+    dw2, db2 = dw.clone(), db.clone()
+    ops.layer_norm_bwd(dy, x, mean, rstd, w, dweight=dw2, dbias=db2, accumulate=True)
+    assert torch.equal(dw2, dw + dw) and torch.equal(db2, db + db)
+    only = torch.empty(H, device=DEV)
+    r = ops.layer_norm_bwd(dy, x, mean, rstd, None, dbias=only)
+    assert r[1] is None and torch.equal(only, db)
+    plain = ops.layer_norm_bwd(dy, x, mean, rstd)
+    assert plain[1] is None and plain[2] is None
+    within(plain[0], grad64(dy.cpu(), x.cpu(), mean.cpu(), rstd.cpu(), None)[0], grad_tol(dy.cpu(), rstd.cpu(), hat, dy.cpu().double())[0] + U, "no weight")
+    # in place of dy and of x, with a workspace of its own
+    ws = torch.full((ops.layer_norm_bwd_workspace(R, H),), float("nan"), device=DEV)
+    for which in ("dy", "x"):
+        a, c = dy.clone(), x.clone()
+        got = ops.layer_norm_bwd(a, c, mean, rstd, w, dx=a if which == "dy" else c, workspace=ws)
+        assert torch.equal(got[0], dx) and torch.equal(got[1], dw) and torch.equal(got[2], db)
+    # one gradient row for all rows, as the backward of a sum gives it
+    row = rnd(1, H, seed=33).to(DEV)
+    a = ops.layer_norm_bwd(row.expand(R, H), x, mean, rstd, w)
+    b = ops.layer_norm_bwd(row.expand(R, H).contiguous(), x, mean, rstd, w)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    e = torch.empty(0, H, device=DEV)
+    z = torch.empty(0, device=DEV)
+    r = ops.layer_norm_bwd(e, e, z, z, w)
+    assert r[0].shape == (0, H) and float(r[1].abs().sum()) == 0 and float(r[2].abs().sum()) == 0
+
+
+def test_layer_norm_gradient_against_differences(ops):
+    """d(sum(c * y)) by x, w and b: central differences of the forward in float64 against the kernel's gradients."""
+    R, H, h = 3, 20, 1e-5
+    x, c = rnd(R, H, seed=40).double(), rnd(R, H, seed=41).double()
+    w, b = rnd(H, seed=42).double(), rnd(H, seed=43).double()
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    ops.layer_norm(x.float().to(DEV), w.float().to(DEV), b.float().to(DEV), mean=mean, rstd=rstd)
+    got = ops.layer_norm_bwd(c.float().to(DEV), x.float().to(DEV), mean, rstd, w.float().to(DEV))
+
+    def f(x_, w_, b_):
+        return float((norm64(x_, w_, b_, 1e-6)[0] * c).sum())
+    args = [x, w, b]
+    for k in range(3):
+        d = torch.zeros_like(args[k])
+        for i in range(d.numel()):
+            e = torch.zeros_like(d).view(-1)
+            e[i] = h
+            e = e.view_as(d)
+            d.view(-1)[i] = (f(*[a + e if j == k else a for j, a in enumerate(args)]) - f(*[a - e if j == k else a for j, a in enumerate(args)])) / (2 * h)
+        # h^2 times a third derivative of order 100, and float32 inputs: far below 1e-4
+        assert float((got[k].cpu().double() - d).abs().max()) < 1e-4 * max(1.0, float(d.abs().max())), k
+
+
+# ---------------------------------------------------------------- AdamW
+def blocks_of(x):
+    n = x.numel()
+    k = -(-n // 256)
+    out = torch.zeros(k * 256, dtype=x.dtype)
+    out[:n] = x.reshape(-1)
+    return out.view(k, 256)
+
+
+def code8(x, root):
+    """e4m3 codes and scales of a tensor as the operator defines them, in float32 operation by operation"""
+    b = blocks_of(x)
+    top = b.abs().amax(1, keepdim=True)
+    top = torch.where(top > 0, top.clamp_min(1e-30), top)
+    f = torch.where(top > 0, torch.full_like(top, 448.0) / top, torch.zeros_like(top))
+    z = b * f
+    if root:
+        z = torch.where(b > 0, z.clamp_min(2.0 ** -9), z)
+    return z.to(torch.float8_e4m3fn).view(-1)[:x.numel()], (top / torch.full_like(top, 448.0)).view(-1)
+
+
+def held8(code, scale):
+    return code.float().reshape(-1) * scale.repeat_interleave(256)[:code.numel()]
+
+
+class Oracle:
+    """the state and step of one tensor, states held in float32 (or 8 bits), arithmetic in `dt`"""
+
+    def __init__(self, p, bits, wd, dt):
+        self.p, self.bits, self.wd, self.dt = p.clone(), bits, wd, dt
+        n = p.numel()
+        self.m, self.v = torch.zeros(n), torch.zeros(n)
+        if bits == 8:
+            self.m, self.ms = code8(self.m, False)
+            self.v, self.vs = code8(self.v, True)
+
+    def step(self, g, t, lr, coef, b1, b2, eps):
+        dt = self.dt
+        g = (g.reshape(-1).to(dt) * torch.tensor(coef, dtype=dt))
+        if self.bits == 8:
+            m, r = held8(self.m, self.ms).to(dt), held8(self.v, self.vs).to(dt)
+            v = r * r
+        else:
+            m, v = self.m.to(dt), self.v.to(dt)
+        m = m * b1 + g * (1 - b1)
+        v = v * b2 + g * g * (1 - b2)
+        # by way of float64: torch's float32 square root on the CPU is not the correctly rounded one on every host, and the
+        # root of a float32 rounded to float64 and then to float32 is (53 >= 2 * 24 + 2 bits)
+        root = torch.sqrt(v.double()).to(dt)
+        one = torch.ones((), dtype=dt)
+        den = root / (one * math.sqrt(1 - b2 ** t)) + eps
+        p = self.p.reshape(-1).to(dt)
+        p = p * (one - lr * (one * self.wd)) - (one * (lr / (1 - b1 ** t))) * (m / den)
+        self.p = p.to(self.p.dtype).view(self.p.shape)
+        self.raw = m, root
+        if self.bits == 8:
+            self.m, self.ms = code8(m.float(), False)
+            self.v, self.vs = code8(root.float(), True)
+        else:
+            self.m, self.v = m.float(), v.float()
+
+
+LENGTHS = [(1,), (3,), (255,), (256,), (257,), (64, 64), (0,), (4096,), (4097,), (333, 77), (5, 4099)]
+
+
+def make(ops, shapes, bits, pt, wd, seed=0):
+    ps = [rnd(*s, seed=seed + i, scale=0.1).to(DT[pt]) for i, s in enumerate(shapes)]
+    dp = [p.to(DEV) for p in ps]
+    if bits == 8:
+        st = [ops.adamw8_state(p) for p in dp]
+        args = ops.adamw_multi_args(dp, [s[0] for s in st], [s[1] for s in st], [s[2] for s in st], [s[3] for s in st], weight_decay=wd)
+    else:
+        st = [(torch.zeros_like(p, dtype=torch.float32), torch.zeros_like(p, dtype=torch.float32)) for p in dp]
+        args = ops.adamw_multi_args(dp, [s[0] for s in st], [s[1] for s in st], weight_decay=wd)
+    return ps, dp, st, args
+
+
+def gradients(shapes, gt, seed, scale=1e-2):
+    out = []
+    for i, s in enumerate(shapes):
+        g = rnd(*s, seed=seed + i, scale=scale * 10 ** (i % 3 - 1))
+        g.view(-1)[::7] = 0                                       # elements whose gradient is exactly zero
+        if i % 4 == 3:
+            g[:] = 0                                              # a whole tensor without one
+        out.append(g.to(DT[gt]))
+    return out
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("pt,gt", [("fp32", "fp32"), ("fp32", "bf16"), ("bf16", "bf16"), ("fp16", "fp32")])
+def test_adamw_multi_steps(ops, bits, pt, gt):
+    """Several steps without clipping: states bit for bit what the formulas give operation by operation in float32 (the codes
+    and scales of 8 bits among them), parameters against the same step in float64."""
+    wd = [0.1 if len(s) == 2 else 0.0 for s in LENGTHS]
+    ps, dp, st, args = make(ops, LENGTHS, bits, pt, wd)
+    same = [Oracle(p, bits, w, torch.float32) for p, w in zip(ps, wd)]
+    step = torch.zeros(1, device=DEV, dtype=torch.int32)
+    lr, b1, b2, eps = 1e-3, 0.9, 0.999, 1e-8
+    for t in range(1, 6):
+        gs = gradients(LENGTHS, gt, 100 * t)
+        before = [p.cpu().clone() for p in dp]
+        ops.adamw_multi(args, [g.to(DEV) for g in gs], step, lr, betas=(b1, b2), eps=eps)
+        assert int(step) == t
+        for i, (o, g) in enumerate(zip(same, gs)):
+            o.p = before[i]
+            exact = Oracle(before[i].double(), bits, wd[i], torch.float64)
+            exact.m, exact.v = o.m, o.v
+            if bits == 8:
+                exact.ms, exact.vs = o.ms, o.vs
+            exact.step(g, t, lr, 1.0, b1, b2, eps)
+            o.step(g, t, lr, 1.0, b1, b2, eps)
+            m, v = st[i][0].cpu().view(-1), st[i][1].cpu().view(-1)
+            if bits == 8:
+                assert torch.equal(m.view(torch.uint8), o.m.view(torch.uint8)) and torch.equal(v.view(torch.uint8), o.v.view(torch.uint8)), (t, i)
+                assert torch.equal(st[i][2].cpu(), o.ms) and torch.equal(st[i][3].cpu(), o.vs), (t, i)
+                # against the unrounded state: half a step of e4m3, or half of its smallest step where that is more
+                for code, scale, raw in ((m, o.ms, exact.raw[0]), (v, o.vs, exact.raw[1])):
+                    s = scale.double().repeat_interleave(256)[:raw.numel()]
+                    least = 2.0 ** -9 if code is v else 2.0 ** -10
+                    within(held8(code, scale), raw, raw.abs() * (2.0 ** -4 + 1e-6) + s * least * 1.001, f"state of tensor {i}")
+            else:
+                assert torch.equal(m, o.m) and torch.equal(v, o.v), (t, i)
+            # p: the decayed value and the step, each a handful of roundings
+            upd = (exact.p.view(-1) - before[i].double().view(-1)).abs() + wd[i] * lr * before[i].double().view(-1).abs() + 2 * lr
+            within(dp[i].view(-1), exact.p.view(-1), 12 * U * upd + (2 * U + half_step(dp[i])) * exact.p.view(-1).abs() * 1.001 +
+                   (2.0 ** -25 if pt == "fp16" else 0), f"parameter {i}")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_multi_clips_by_the_norm_of_all(ops, bits):
+    shapes = [(257, 33), (0,), (5000,), (3,)]
+    gs = gradients(shapes, "fp32", 7, scale=1.0)
+    total = math.sqrt(sum(float((g.double() ** 2).sum()) for g in gs))
+    for max_norm, scale in ((1.0, 1.0), (0.5 * total, 1.0), (2 * total, 1.0), (1.0, 0.125), (None, 0.25)):
+        ps, dp, st, args = make(ops, shapes, bits, "fp32", 0.0)
+        step, norm = torch.zeros(1, device=DEV, dtype=torch.int32), torch.zeros(1, device=DEV)
+        ops.adamw_multi(args, [g.to(DEV) for g in gs], step, 1e-3, max_norm=max_norm, grad_scale=scale, norm=norm)
+        assert abs(float(norm) - total * scale) < 100 * U * total * scale
+        coef = scale * (1.0 if max_norm is None else min(1.0, max_norm / (total * scale + 1e-6)))
+        for i, g in enumerate(gs):
+            o = Oracle(ps[i].double(), bits, 0.0, torch.float64)
+            o.step(g, 1, 1e-3, coef, 0.9, 0.999, 1e-8)
+            within(dp[i], o.p, 300 * U * 1e-3 + 3 * U * o.p.abs(), "p")
+            if bits == 32:
+                within(st[i][0].view(-1), o.m, 110 * U * o.m.double().abs(), "m")
+                within(st[i][1].view(-1), o.v, 220 * U * o.v.double().abs(), "v")
+
+
+def test_adamw_multi_more_tensors_than_one_table(ops):
+    """over a hundred tensors, tiny and large ones mixed: the same as each of them alone; a None gradient changes nothing"""
+    shapes = [(i % 9 * 37 + 1,) if i % 10 else (90, 130) for i in range(125)]
+    gs = gradients(shapes, "fp32", 500)
+    for bits in (32, 8):
+        ps, dp, st, args = make(ops, shapes, bits, "fp32", 0.01)
+        step = torch.full((1,), 3, device=DEV, dtype=torch.int32)
+        dg = [g.to(DEV) if i not in (4, 60, 124) else None for i, g in enumerate(gs)]
+        ops.adamw_multi(args, dg, step, 1e-3, norm=torch.zeros(1, device=DEV))
+        assert int(step) == 4
+        for i in range(len(shapes)):
+            if dg[i] is None:
+                assert torch.equal(dp[i].cpu(), ps[i]) and not bool(st[i][0].cpu().view(torch.uint8).any())
+                continue
+            p1, d1, s1, a1 = make(ops, [shapes[i]], bits, "fp32", 0.01, seed=i)
+            ops.adamw_multi(a1, [dg[i]], torch.full((1,), 3, device=DEV, dtype=torch.int32), 1e-3)
+            assert torch.equal(d1[0], dp[i]) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(s1[0], st[i])), i
+    ops.adamw_multi(args, dg, step, 1e-3)                         # and the next call takes the gradient back up
+    ops.adamw_multi(args, [g.to(DEV) for g in gs], step, 1e-3)
+    assert not torch.equal(dp[4].cpu(), ps[4])
+
+
+def test_adamw_multi_unaligned_views(ops):
+    """parameters, gradients and states that begin at any element of larger buffers; nothing beside them is touched"""
+    sizes, at = [1000, 1, 513, 4099], [1, 1003, 1007, 1522]
+    for bits in (32, 8):
+        flat = {k: rnd(6000, seed=60 + i, scale=0.1).to(DEV) for i, k in enumerate("pg")}
+        if bits == 8:
+            flat["m"], flat["v"] = (torch.zeros(6000, device=DEV, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+        else:
+            flat["m"], flat["v"] = torch.zeros(6000, device=DEV), torch.zeros(6000, device=DEV)
+        was = {k: v.clone() for k, v in flat.items()}
+        view = {k: [v[a:a + n] for a, n in zip(at, sizes)] for k, v in flat.items()}
+        sc = [[torch.zeros(-(-n // 256), device=DEV) for n in sizes] for _ in range(2)] if bits == 8 else [None, None]
+        args = ops.adamw_multi_args(view["p"], view["m"], view["v"], *sc)
+        ops.adamw_multi(args, view["g"], torch.zeros(1, device=DEV, dtype=torch.int32), 1e-3, max_norm=1.0)
+        aligned = [t.clone() for t in [was["p"][a:a + n] for a, n in zip(at, sizes)]]
+        st = [ops.adamw8_state(t) if bits == 8 else (torch.zeros_like(t), torch.zeros_like(t)) for t in aligned]
+        a2 = ops.adamw_multi_args(aligned, *[[s[k] for s in st] for k in range(4 if bits == 8 else 2)])
+        ops.adamw_multi(a2, [t.clone() for t in view["g"]], torch.zeros(1, device=DEV, dtype=torch.int32), 1e-3, max_norm=1.0)
+        outside = torch.ones(6000, dtype=torch.bool)
+        for i, (a, n) in enumerate(zip(at, sizes)):
+            outside[a:a + n] = False
+            assert torch.equal(view["p"][i], aligned[i])
+            assert torch.equal(view["m"][i].view(torch.uint8), st[i][0].view(torch.uint8))
+        for k in "pmv":
+            raw = lambda t: t.view(torch.uint8).view(6000, -1)[outside.to(DEV)]  # noqa: E731
+            assert torch.equal(raw(flat[k]), raw(was[k])), k
+
+
+def test_adamw8_extremes(ops):
+    """blocks whose elements span the whole range, tiny and huge gradients, a block without any, one with a NaN"""
+    n = 256 * 6
+    g = torch.zeros(n)
+    g[:256] = 10.0 ** torch.linspace(-18, 2, 256)                 # far below the smallest code beside the largest
+    g[256:512] = 1e-38
+    g[512:768] = 3e18
+    g[1024:1280] = rnd(256, seed=70)
+    g[1100] = float("nan")
+    g[1280:] = rnd(256, seed=71)
+    p = torch.ones(n, device=DEV)
+    m, v, ms, vs = ops.adamw8_state(p)
+    args = ops.adamw_multi_args([p], [m], [v], [ms], [vs])
+    step = torch.zeros(1, device=DEV, dtype=torch.int32)
+    for _ in range(3):
+        ops.adamw_multi(args, [g.to(DEV)], step, 1e-2)
+        q = p.cpu()
+        fine = torch.ones(n, dtype=torch.bool)
+        fine[1024:1280] = False
+        assert bool(torch.isfinite(q[fine]).all())
+        # the step of an element is at most lr * sqrt(1 / (1 - b2)) at the very worst; no element may run away through a
+        # root that was rounded to zero
+        assert float((q[fine] - 1).abs().max()) < 3 * 1e-2 * 32
+    assert torch.equal(p.cpu()[768:1024], torch.ones(256))        # no gradient: nothing moved
+    assert bool(torch.isnan(p.cpu()[1024:1280]).all())            # the NaN took its block, and no other
+    codes = v.cpu().float()
+    assert bool((codes[:256] > 0).all()) and bool((codes[768:1024] == 0).all())
+
+
+# ---------------------------------------------------------------- 8-bit product
+@pytest.mark.parametrize("R,K", [(1, 1), (1, 15), (3, 16), (5, 1000), (2, 1024), (7, 2049), (33, 4096), (2, 9000), (0, 32)])
+@pytest.mark.parametrize("xt", ["fp32", "bf16", "fp16"])
+def test_quantize_rows(ops, R, K, xt):
+    x = (rnd(R, K, seed=80) * torch.exp(rnd(R, 1, seed=81))).to(DT[xt])
+    if R > 2:
+        x[1] = 0
+        x[2, ::3] = 0
+    q, s = ops.quantize_rows(x.to(DEV))
+    f = x.float()
+    top = f.abs().amax(1, keepdim=True) if R else f[:, :1]
+    want = torch.round(f * torch.where(top > 0, torch.full_like(top, 127.0) / top, torch.zeros_like(top)))
+    assert q.shape == (R, K) and torch.equal(q.cpu().float(), want)
+    assert torch.equal(s.cpu(), (top / torch.full_like(top, 127.0)).view(-1))
+    if R:
+        rows = torch.as_strided(q, (R, -(-K // 16) * 16), (q.stride(0) if R > 1 else -(-K // 16) * 16, 1))
+        assert not bool(rows[:, K:].any())
+        # half a step of the scale, and the roundings of the product and the scale
+        within(q.cpu().float() * s.cpu().view(-1, 1), f, s.cpu().double().view(-1, 1) * (0.5 + 200 * U) + 2 * U * f.double().abs(), "value")
+
+
+def test_quantize_rows_special(ops):
+    x = rnd(6, 40, seed=82)
+    x[0] *= 1e-37
+    x[1, 3] = float("inf")
+    x[2, 5] = float("nan")
+    x[3] *= 1e37
+    x[4] = 0
+    big = torch.zeros(6, 50, device=DEV)
+    big[:, 3:43] = x.to(DEV)
+    out = torch.full((6, 64), 9, device=DEV, dtype=torch.int8)
+    q, s = ops.quantize_rows(big[:, 3:43], out=out[:, :40])
+    assert q.data_ptr() == out.data_ptr() and bool((out[:, 48:] == 9).all()) and bool((out[:, 40:48] == 0).all())
+    s = s.cpu()
+    assert math.isinf(float(s[1])) and math.isnan(float(s[2])) and float(s[4]) == 0 and not bool(q[4].any())
+    ok = [0, 3, 5]
+    within(q.cpu().float()[ok] * s[ok].view(-1, 1), x[ok], s[ok].double().view(-1, 1) * 0.501, "value")
+    y = ops.gemm_i8(q, s.to(DEV), *ops.quantize_rows(rnd(8, 40, seed=83).to(DEV))).cpu()
+    assert not bool(torch.isfinite(y[1:3]).any()) and bool(torch.isfinite(y[ok]).all()) and not bool(y[4].any())
+
+
+def operands(M, N, K, seed=0, lo=-127, hi=128):
+    g = torch.Generator().manual_seed(seed)
+    kp = -(-K // 16) * 16
+    A = torch.randint(lo, hi, (M, kp), generator=g, dtype=torch.int8)      # behind K: anything at all
+    W = torch.randint(lo, hi, (N, kp), generator=g, dtype=torch.int8)
+    return A, W, torch.rand(M, generator=g) * 0.01, torch.rand(N, generator=g) * 0.01, torch.randn(N, generator=g)
+
+
+SHAPES8 = [(1, 1, 1), (1, 64, 64), (3, 5, 17), (16, 16, 64), (17, 100, 130), (128, 128, 128), (129, 127, 915), (4, 4096, 1024), (1, 1000, 2048),
+           (33, 65, 4096), (300, 1000, 200), (257, 513, 1040), (64, 200, 8192), (700, 900, 64), (31, 4100, 48), (1030, 770, 333)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES8)
+@pytest.mark.parametrize("ct", ["fp32", "bf16", "fp16"])
+def test_gemm_i8(ops, M, N, K, ct):
+    A, W, sa, sw, b = operands(M, N, K, seed=M + N + K)
+    exact = (A[:, :K].double() @ W[:, :K].double().T)
+    for bias in (b, None):
+        y = ops.gemm_i8(A.to(DEV)[:, :K], sa.to(DEV), W.to(DEV)[:, :K], sw.to(DEV), None if bias is None else bias.to(DEV), out_dtype=DT[ct])
+        prod = exact * sa.double().view(-1, 1) * sw.double()
+        want = prod if bias is None else prod + bias.double()
+        assert y.dtype == DT[ct]
+        within(y, want, 4 * U * (prod.abs() + want.abs()) + half_step(y) * want.abs() * 1.001 + (2.0 ** -25 if ct == "fp16" else 0), "y")
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 3, 131071), (200, 300, 131071), (600, 1024, 2048), (1500, 1300, 1000)])
+def test_gemm_i8_sum_is_exact(ops, M, N, K):
+    """the largest sums that can be: all operands at -128 / 127; with scales of one, C is the rounded whole number"""
+    A, W, _, _, _ = operands(M, N, K, seed=5, lo=-128, hi=128)
+    A[0], W[0], A[-1] = -128, -128, 127
+    one_m, one_n = torch.ones(M, device=DEV), torch.ones(N, device=DEV)
+    y = ops.gemm_i8(A.to(DEV)[:, :K], one_m, W.to(DEV)[:, :K], one_n).cpu()
+    rows, cols = torch.tensor([0, M // 2, M - 1]), torch.tensor([0, N // 2, N - 1])
+    want = (A[rows][:, :K].long() @ W[cols][:, :K].long().T)
+    assert torch.equal(y[rows][:, cols], want.float())
+    if K < 10000:
+        assert torch.equal(y, (A[:, :K].double() @ W[:, :K].double().T).float())
+
+
+def test_gemm_i8_strides_and_edges(ops):
+    """row strides of all operands larger than their rows, an output that begins anywhere; what lies beside is left alone"""
+    for M, N, K in ((5, 7, 33), (130, 250, 300), (520, 1031, 200)):
+        A, W, sa, sw, b = operands(M, N, K, seed=9)
+        bigA = torch.full((M, 1024), 77, device=DEV, dtype=torch.int8)
+        bigW = torch.full((N, 512), -99, device=DEV, dtype=torch.int8)
+        bigA[:, 48:48 + K], bigW[:, 16:16 + K] = A[:, :K].to(DEV), W[:, :K].to(DEV)
+        want = ops.gemm_i8(A.to(DEV)[:, :K], sa.to(DEV), W.to(DEV)[:, :K], sw.to(DEV), b.to(DEV), out_dtype=torch.bfloat16)
+        for dt in (torch.bfloat16, torch.float32):
+            out = torch.full((M, N + 9), 3.0, device=DEV, dtype=dt)
+            got = ops.gemm_i8(bigA[:, 48:48 + K], sa.to(DEV), bigW[:, 16:16 + K], sw.to(DEV), b.to(DEV), out=out[:, 5:5 + N])
+            assert torch.equal(got.bfloat16(), want)
+            assert bool((out[:, :5] == 3).all()) and bool((out[:, 5 + N:] == 3).all())
+    z = ops.gemm_i8(torch.empty(0, 16, device=DEV, dtype=torch.int8), torch.empty(0, device=DEV), W.to(DEV)[:, :16], sw.to(DEV))
+    assert z.shape == (0, N)
+
+
+# ---------------------------------------------------------------- refusals
+def test_refusals(ops):
+    x, w = torch.zeros(4, 32, device=DEV), torch.ones(32, device=DEV)
+    s4, s32 = torch.zeros(4, device=DEV), torch.zeros(32, device=DEV)
+    with pytest.raises(ValueError, match="neighbours"):
+        ops.layer_norm(x.t())
+    with pytest.raises(ValueError, match="weight"):
+        ops.layer_norm(x, w[:31])
+    with pytest.raises(TypeError):
+        ops.layer_norm(x, w, w.bfloat16())
+    with pytest.raises(TypeError):
+        ops.layer_norm(x.half(), w.bfloat16())
+    with pytest.raises(TypeError):
+        ops.layer_norm(x.double())
+    with pytest.raises(ValueError, match="overlap"):
+        ops.layer_norm(x, out=torch.zeros(32, device=DEV).expand(4, 32))
+    with pytest.raises(ValueError):
+        ops.layer_norm(x, eps=-1.0)
+    with pytest.raises(ValueError, match="mean"):
+        ops.layer_norm_bwd(x, x, None, None)
+    with pytest.raises(ValueError, match="accumulate"):
+        ops.layer_norm_bwd(x, x, s4, s4, w, accumulate=True)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.layer_norm_bwd(x, x, s4, s4, w, workspace=torch.zeros(4, device=DEV))
+    with pytest.raises(ValueError, match="dy"):
+        ops.layer_norm_bwd(x[:3], x, s4, s4, w)
+    with pytest.raises(TypeError):
+        ops.layer_norm_bwd(x, x, s4, s4, w, dx=x.bfloat16())
+    p, m, v = (torch.zeros(300, device=DEV) for _ in range(3))
+    args = ops.adamw_multi_args([p], [m], [v])
+    step = torch.zeros(1, device=DEV, dtype=torch.int32)
+    for bad in ([p[:299]], [p.cpu()], [torch.zeros(600, device=DEV)[::2]], [p, p], []):
+        with pytest.raises(ValueError):
+            ops.adamw_multi(args, bad, step, 1e-3)
+    with pytest.raises(TypeError):
+        ops.adamw_multi(args, [p.double()], step, 1e-3)
+    for kw in (dict(max_norm=0.0), dict(max_norm=float("nan")), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(workspace=torch.zeros(3, device=DEV))):
+        with pytest.raises(ValueError):
+            ops.adamw_multi(args, [p], step, 1e-3, **kw)
+    with pytest.raises(ValueError):
+        ops.adamw_multi(args, [p], step, -1e-3)
+    with pytest.raises(ValueError):
+        ops.adamw_multi(args, [p], step.long(), 1e-3)
+    assert int(step) == 0 and not bool(p.any())
+    with pytest.raises(TypeError):
+        ops.adamw_multi_args([p], [m.half()], [v])
+    with pytest.raises(ValueError):
+        ops.adamw_multi_args([p], [m[:7]], [v])
+    c = m.to(torch.float8_e4m3fn)
+    with pytest.raises(ValueError):
+        ops.adamw_multi_args([p], [c], [c])
+    with pytest.raises(ValueError):
+        ops.adamw_multi_args([p], [c], [c], [torch.zeros(1, device=DEV)], [torch.zeros(2, device=DEV)])
+    q = torch.zeros(4, 32, device=DEV, dtype=torch.int8)
+    with pytest.raises(TypeError, match="int8"):
+        ops.gemm_i8(x, s4, q, s4)
+    with pytest.raises(ValueError, match="borders"):
+        ops.gemm_i8(q[:, 3:], s4, q[:, 3:], s4)
+    with pytest.raises(ValueError, match="borders"):
+        ops.gemm_i8(torch.zeros(4, 33, device=DEV, dtype=torch.int8), s4, q, s4)
+    with pytest.raises(ValueError, match="borders"):                 # the last row ends with its memory
+        ops.gemm_i8(torch.zeros(3 * 48 + 33, device=DEV, dtype=torch.int8).as_strided((4, 33), (48, 1)), s4, q, s4)
+    with pytest.raises(ValueError, match="columns"):
+        ops.gemm_i8(q, s4, q[:, :16], s4)
+    with pytest.raises(ValueError, match="a_scale"):
+        ops.gemm_i8(q, s32, q, s4)
+    with pytest.raises(ValueError):
+        ops.gemm_i8(*[torch.zeros(1, 131072, device=DEV, dtype=torch.int8), s4[:1]] * 2)
+    with pytest.raises(TypeError):
+        ops.gemm_i8(q, s4, q, s4, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="borders"):
+        ops.quantize_rows(x[:, :30], out=torch.zeros(4, 30, device=DEV, dtype=torch.int8))
+
+
+# ---------------------------------------------------------------- together, as they are used
+@pytest.mark.parametrize("bits", [32, 8])
+def test_projection_is_trained_and_served(ops, bits):
+    """LayerNorm -> Linear: forward, backward and AdamW on all four tensors for a few steps against autograd and the same
+    optimizer in float64; then the matrix in 8 bits, served one token and many at a time."""
+    R, H, N, lr = 200, 96, 64, 1e-2
+    x, target = rnd(R, H, seed=90) * 2 + 1, rnd(R, N, seed=91)
+    shapes = [(H,), (H,), (N, H), (N,)]
+    init = [torch.ones(H), torch.zeros(H), rnd(N, H, seed=92, scale=0.1), torch.zeros(N)]
+    dp = [p.to(DEV) for p in init]
+    if bits == 8:
+        st = [ops.adamw8_state(p) for p in dp]
+    else:
+        st = [(torch.zeros_like(p), torch.zeros_like(p)) for p in dp]
+    args = ops.adamw_multi_args(dp, *[[s[k] for s in st] for k in range(len(st[0]))], weight_decay=[0, 0, 0.1, 0])
+    step = torch.zeros(1, device=DEV, dtype=torch.int32)
+    oracles = [Oracle(p.double(), bits, w, torch.float64) for p, w in zip(init, (0, 0, 0.1, 0))]
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    dx_, dt_ = x.to(DEV), target.to(DEV)
+    for t in range(1, 4):
+        y = ops.layer_norm(dx_, dp[0], dp[1], mean=mean, rstd=rstd)
+        d = (y @ dp[2].t() + dp[3] - dt_) * (2.0 / (R * N))
+        _, dw, db = ops.layer_norm_bwd(d @ dp[2], dx_, mean, rstd, dp[0])
+        grads = [dw, db, d.t().contiguous() @ y, d.sum(0)]
+        leaves = [o.p.clone().requires_grad_() for o in oracles]
+        out = norm64(x, leaves[0], leaves[1], 1e-6)[0] @ leaves[2].T + leaves[3]
+        ((out - target.double()) ** 2).mean().backward()
+        for g, l in zip(grads, leaves):
+            assert float((g.cpu().double() - l.grad).abs().max()) < 1e-4 * float(l.grad.abs().max())
+        total = math.sqrt(sum(float((l.grad ** 2).sum()) for l in leaves))
+        norm = torch.zeros(1, device=DEV)
+        ops.adamw_multi(args, grads, step, lr, max_norm=0.1, norm=norm)
+        assert abs(float(norm) - total) < 1e-5 * total
+        for o, l in zip(oracles, leaves):
+            o.step(l.grad, t, lr, min(1.0, 0.1 / (total + 1e-6)), 0.9, 0.999, 1e-8)
+        for p, o in zip(dp, oracles):
+            # float32 gradients 1e-6 apart; in 8 bits a state next to a border may fall to the other code, an eighth of a
+            # moment at most, for a few elements
+            off = (p.cpu().double() - o.p).abs()
+            assert float(off.max()) < (0.2 if bits == 8 else 2e-3) * lr * t and float(off.median()) < 1e-4 * lr
+    wq, ws = ops.quantize_rows(dp[2])
+    for rows in (1, R):
+        y = ops.layer_norm(dx_[:rows], dp[0], dp[1], out_dtype=torch.bfloat16)
+        served = ops.gemm_i8(*ops.quantize_rows(y), wq, ws, dp[3], out_dtype=torch.bfloat16)
+        yf, wf = y.cpu().double(), dp[2].cpu().double()
+        want = yf @ wf.T + dp[3].cpu().double()
+        # each operand is off by half of its step: sum over K of (|y| sw + |w| sy) / 2 + sy sw / 4 is above the error
+        sy, sw = yf.abs().amax(1, keepdim=True) / 127, wf.abs().amax(1) / 127
+        tol = (yf.abs().sum(1, keepdim=True) * sw + sy * wf.abs().sum(1)) * 0.501 + H * sy * sw * 0.251 + want.abs() * 2.0 ** -8
+        within(served, want, tol, "served")
+
+
+def test_captured_step_replays(ops):
+    """layer_norm, its backward and the optimizer in one ops.Graph with workspaces of their own, the program's own eager work
+    between the replays: every replay gives what the eager calls give on the same data."""
+    R, H = 70, 200
+    ws = [torch.empty(ops.layer_norm_bwd_workspace(R, H), device=DEV), torch.empty(ops.adamw_multi_workspace(2), device=DEV)]
+    x, dy = torch.empty(R, H, device=DEV), torch.empty(R, H, device=DEV)
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    mean, rstd, dw, db, norm = (torch.empty(n, device=DEV) for n in (R, R, H, H, 1))
+    q, qs = torch.empty(R, 208, device=DEV, dtype=torch.int8)[:, :H], torch.empty(R, device=DEV)
+    out = torch.empty(R, R, device=DEV)
+    for bits in (32, 8):
+        ps, dp, st, args = make(ops, [(H,), (H,)], bits, "fp32", 0.01)
+        ps2, dp2, st2, args2 = make(ops, [(H,), (H,)], bits, "fp32", 0.01)
+        step, step2 = (torch.zeros(1, device=DEV, dtype=torch.int32) for _ in range(2))
+
+        def body():
+            ops.layer_norm(x, dp[0], dp[1], out=y, mean=mean, rstd=rstd)
+            ops.layer_norm_bwd(dy, x, mean, rstd, dp[0], dx=dx, dweight=dw, dbias=db, workspace=ws[0])
+            ops.adamw_multi(args, [dw, db], step, 1e-2, max_norm=1.0, norm=norm, workspace=ws[1])
+            ops.quantize_rows(y, out=q, scale=qs)
+            ops.gemm_i8(q, qs, q, qs, out=out)
+        g = ops.Graph()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            g.begin()
+            body()
+            g.end()
+        torch.cuda.synchronize()
+        assert int(step) == 0
+        for k in range(4):
+            x.copy_(rnd(R, H, seed=200 + k).to(DEV))
+            dy.copy_(rnd(R, H, seed=300 + k).to(DEV))
+            with torch.cuda.stream(s):
+                s.wait_stream(torch.cuda.default_stream())
+                g.launch()
+            torch.cuda.synchronize()
+            m2, r2 = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+            y2 = ops.layer_norm(x, dp2[0], dp2[1], mean=m2, rstd=r2)
+            dx2, dw2, db2 = ops.layer_norm_bwd(dy, x, m2, r2, dp2[0])
+            ops.adamw_multi(args2, [dw2, db2], step2, 1e-2, max_norm=1.0)
+            q2, qs2 = ops.quantize_rows(y2)
+            out2 = ops.gemm_i8(q2, qs2, q2, qs2)
+            for a, b in ((y, y2), (dx, dx2), (dw, dw2), (db, db2), (dp[0], dp2[0]), (dp[1], dp2[1]), (out, out2), (qs, qs2)):
+                assert torch.equal(a, b), (bits, k)
+            assert int(step) == int(step2) == k + 1
+
+
+def test_side_stream(ops):
+    """calls enqueue on the stream that is current, and on no other"""
+    x = rnd(512, 1024, seed=95).to(DEV)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        ops.spin_probe(1, 2000)
+        x.mul_(2)                                                # done after the wait; the calls below have to see it
+        y = ops.layer_norm(x)
+        q, sc = ops.quantize_rows(x)
+        z = ops.gemm_i8(q, sc, q, sc)
+    s.synchronize()
+    assert torch.equal(y, ops.layer_norm(x)) and torch.equal(q, ops.quantize_rows(x)[0]) and torch.equal(z, ops.gemm_i8(q, sc, q, sc))
