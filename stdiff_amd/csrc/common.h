@@ -177,6 +177,38 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// Reductions over a wave without LDS traffic: quad permutes and mirrors inside a row of 16 lanes, then the gfx950 lane swaps
+// between rows.  The same result in all lanes.  (Another order of additions than wave_sum's.)
+#define STDIFF_DPP(v, ctrl) __builtin_amdgcn_update_dpp(0, (int)(v), ctrl, 0xf, 0xf, true)
+typedef unsigned u32x2_swap __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) {
+    v = max(v, (unsigned)STDIFF_DPP(v, 0xb1));        // lanes 1 apart
+    v = max(v, (unsigned)STDIFF_DPP(v, 0x4e));        // 2
+    v = max(v, (unsigned)STDIFF_DPP(v, 0x141));       // mirror of eight
+    v = max(v, (unsigned)STDIFF_DPP(v, 0x140));       // mirror of sixteen
+    u32x2_swap s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(s[0], s[1]);
+    s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(s[0], s[1]);
+}
+__device__ __forceinline__ float wave_sum_dpp(float v) {
+#define STDIFF_DPP_ADD(ctrl) v += __builtin_bit_cast(float, STDIFF_DPP(__builtin_bit_cast(int, v), ctrl))
+    STDIFF_DPP_ADD(0xb1);
+    STDIFF_DPP_ADD(0x4e);
+    STDIFF_DPP_ADD(0x141);
+    STDIFF_DPP_ADD(0x140);
+#undef STDIFF_DPP_ADD
+    // (scalars in between: __builtin_bit_cast of a vector's element takes its first)
+    unsigned b = __builtin_bit_cast(unsigned, v);
+    u32x2_swap s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    unsigned lo = s[0], hi = s[1];
+    v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+    b = __builtin_bit_cast(unsigned, v);
+    s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    lo = s[0], hi = s[1];
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
 static inline int cu_count() {      // CUs of the current device (one process drives one GPU model: cached once)
     static const int n = [] {
         int dev = 0, v = 0;

@@ -37,39 +37,95 @@ __device__ __forceinline__ void ld8(const bf16_t* p, int k, float* o) {
     }
 }
 
-// one workgroup of T threads per row, eight elements per thread and turn; the row is read a second time from the cache.
-// The largest magnitude is found by the bits, so a NaN is above infinity and makes the scale a NaN: with a scale that is
-// not finite the whole row of the product is NaN.  Columns K .. round_up(K, 16) - 1 of q become zeros.
-template <typename TX>
+// The largest magnitude is found by the bits, so a NaN is above infinity and makes the scale a NaN: with a scale that is not
+// finite the whole row of the product is NaN.  Columns K .. round_up(K, 16) - 1 of q become zeros.
+__device__ __forceinline__ float row_factor(unsigned top_bits, float* scale) {
+    const float t = __builtin_bit_cast(float, top_bits);
+    // below 1e-30 the factor 127 / t would leave the range of fp32: such rows are scaled as if their largest were 1e-30
+    const float m = t > 0.f && t < 1e-30f ? 1e-30f : t;
+    *scale = m / 127.0f;
+    return m == 0.f ? 0.f : 127.0f / m;
+}
+__device__ __forceinline__ u32x2 to_i8(const float* v, float f) {
+    unsigned o[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j >> 2] |= ((unsigned)(int)rintf(v[j] * f) & 0xffu) << (8 * (j & 3));
+    return u32x2{o[0], o[1]};
+}
+template <int T> __device__ __forceinline__ unsigned row_max(unsigned top, unsigned* part) {
+    top = wave_umax_dpp(top);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < T / 64; ++i) top = max(top, part[i]);
+    }
+    return top;
+}
+
+// a row stays in the registers of T lanes, eight elements per lane and vector
+template <typename TX, int NV, int T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const TX* x, long long ldx, signed char* q, long long ldq, float* scale,
                                                             int R, int K) {
+    __shared__ unsigned part[2][4];
+    const int t = threadIdx.x % T, kp = (K + 15) / 16 * 16;
+    int odd = 0;
+    for (long long row = (long long)blockIdx.x * (256 / T) + threadIdx.x / T; row < R; row += (long long)gridDim.x * (256 / T), odd ^= 1) {
+        float v[NV][8], s;
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) ld8(x + row * ldx + (i * T + t) * 8, K - (i * T + t) * 8, v[i]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
+        const float f = row_factor(row_max<T>(top, part[odd]), &s);
+        if (t == 0) scale[row] = s;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if ((i * T + t) * 8 < kp) *(u32x2*)(q + row * ldq + (i * T + t) * 8) = to_i8(v[i], f);
+    }
+}
+
+// rows too long for the registers are read a second time, from the cache
+template <typename TX>
+__global__ __launch_bounds__(256) void quantize_rows_long_kernel(const TX* x, long long ldx, signed char* q, long long ldq, float* scale,
+                                                                 int R, int K) {
     __shared__ unsigned part[2][4];
     int odd = 0;
     for (long long row = blockIdx.x; row < R; row += gridDim.x, odd ^= 1) {
         unsigned top = 0;
+        float v[8], s;
         for (int c = threadIdx.x * 8; c < K; c += 2048) {
-            float v[8];
             ld8(x + row * ldx + c, K - c, v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
-        if ((threadIdx.x & 63) == 0) part[odd][threadIdx.x >> 6] = top;
-        __syncthreads();
-        const float t = __builtin_bit_cast(float, max(max(part[odd][0], part[odd][1]), max(part[odd][2], part[odd][3])));
-        // below 1e-30 the factor 127 / t would leave the range of fp32: such rows are scaled as if their largest were 1e-30
-        const float m = t > 0.f && t < 1e-30f ? 1e-30f : t, f = m == 0.f ? 0.f : 127.0f / m;
-        if (threadIdx.x == 0) scale[row] = m / 127.0f;
+        const float f = row_factor(row_max<256>(top, part[odd]), &s);
+        if (threadIdx.x == 0) scale[row] = s;
         for (int c = threadIdx.x * 8; c < (K + 15) / 16 * 16; c += 2048) {
-            float v[8];
             ld8(x + row * ldx + c, K - c, v);
-            unsigned o[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j >> 2] |= ((unsigned)(int)rintf(v[j] * f) & 0xffu) << (8 * (j & 3));
-            *(u32x2*)(q + row * ldq + c) = u32x2{o[0], o[1]};
+            *(u32x2*)(q + row * ldq + c) = to_i8(v, f);
         }
     }
+}
+
+template <typename TX>
+int launch_quantize(const void* x, long long ldx, void* q, long long ldq, float* scale, int R, int K, hipStream_t st) {
+#define QR(NV, T)                                                                                                              \
+    hipLaunchKernelGGL((quantize_rows_kernel<TX, NV, T>), dim3((unsigned)std::min<long long>((R + 256 / T - 1ll) / (256 / T), 8ll * cu_count())), \
+                       dim3(256), 0, st, (const TX*)x, ldx, (signed char*)q, ldq, scale, R, K)
+    if (K <= 512) QR(1, 64);
+    else if (K <= 1024) QR(2, 64);
+    else if (K <= 2048) QR(4, 64);
+    else if (K <= 4096) QR(2, 256);
+    else if (K <= 8192) QR(4, 256);
+    else
+        hipLaunchKernelGGL(quantize_rows_long_kernel<TX>, dim3((unsigned)std::min<long long>(R, 8ll * cu_count())), dim3(256), 0, st,
+                           (const TX*)x, ldx, (signed char*)q, ldq, scale, R, K);
+#undef QR
+    STDIFF_LAUNCH_STATUS();
+    return STDIFF_OK;
 }
 
 // ---------------------------------------------------------------- product
@@ -91,61 +147,428 @@ __device__ __forceinline__ i32x4 before_end(i32x4 v, int k0, int K) {
     return v;
 }
 
-template <typename TC>
-__global__ __launch_bounds__(256) void gemm_i8_kernel(Params8 p) {
-    constexpr int BM = 128, BN = 128, BK = 64, LD = BK + 16;
-    __shared__ __attribute__((aligned(16))) signed char As[BM * LD], Ws[BN * LD];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-    const int wr = wid >> 1, wc = wid & 1, fr = lane & 15, fq = lane >> 4;
-    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
-    i32x4 acc[4][4];
+#define VMCNT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
+#define LGKMCNT0() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
+#define BARRIER()                      \
+    do {                               \
+        __builtin_amdgcn_s_barrier();  \
+        asm volatile("" ::: "memory"); \
+    } while (0)
+
+constexpr int SLAB = 128;                  // bytes of K that are staged at once: one row of a tile image, eight 16-byte pieces
+constexpr unsigned OUTSIDE = 0x80000000u;  // an offset behind every descriptor's range: the load gives zeros
+
+// Rows [first, first + count) of an operand as a buffer whose range ends with the last valid row's last piece: rows behind
+// the matrix read as zeros.  The base moves with the tile, so offsets stay below 2^31 whatever the matrix's size.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const signed char* base, long long ld, int first, int count, int rows, int K) {
+    const int n = min(count, rows - first);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<signed char*>(base + first * ld), 0,
+                                             n > 0 ? (int)((n - 1) * ld) + (K + 15) / 16 * 16 : 0, 0x00020000);
+}
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, unsigned char* dst, unsigned offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
+}
+// columns n .. n + 3 of a vector of N
+__device__ __forceinline__ f32x4 four(const float* v, int n, int N) {
+    if (n + 4 <= N) return *(const f32x4_u*)(v + n);
+    f32x4 o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int e = 0; e < 4; ++e) o[e] = n + e < N ? v[n + e] : 0.f;
+    return o;
+}
+__device__ __forceinline__ f32x4 scaled(i32x4 sum, float as, f32x4 ws, f32x4 b) {
+    f32x4 o;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    for (int k0 = 0; k0 < p.K; k0 += BK) {
-        __syncthreads();
+    for (int e = 0; e < 4; ++e) o[e] = (float)sum[e] * ws[e] * as + b[e];
+    return o;
+}
+__device__ __forceinline__ void put4(float* p, f32x4 v) { *(f32x4*)p = v; }
+__device__ __forceinline__ void put4(bf16_t* p, f32x4 v) { *(u32x2*)p = u32x2{pack2bf(v[0], v[1]), pack2bf(v[2], v[3])}; }
+// 16 bytes of a row of C, which may begin at any element and end inside the piece
+template <bool NT, typename TC> __device__ __forceinline__ void store16(TC* row, int n, int N, u32x4 v) {
+    constexpr int E = 16 / sizeof(TC);
+    if (n + E <= N) {
+        if constexpr (sizeof(TC) == 4) {
+            const f32x4 o = __builtin_bit_cast(f32x4, v);
+            if (NT) __builtin_nontemporal_store(o, (f32x4_u*)(row + n));
+            else *(f32x4_u*)(row + n) = o;
+        } else if (NT) {
+            __builtin_nontemporal_store(v, (u32x4_u*)(row + n));
+        } else {
+            *(u32x4_u*)(row + n) = v;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (n + e < N) {
+                if constexpr (sizeof(TC) == 4) ((unsigned*)row)[n + e] = v[e];
+                else ((bf16_t*)row)[n + e] = (bf16_t)(v[e >> 1] >> (16 * (e & 1)));
+            }
+    }
+}
+__device__ __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int* tm, int* tn) {
+    // workgroups i and i + 8 share an XCD's L2: each XCD gets a contiguous range of tiles, in groups of eight rows of tiles
+    const int n = tiles_m * tiles_n, q = n >> 3, r = n & 7, x = i & 7;
+    const int at = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (i >> 3);
+    const int group = at / (8 * tiles_n), in = at - group * 8 * tiles_n, high = min(tiles_m - group * 8, 8);
+    *tm = group * 8 + in % high;
+    *tn = in / high;
+}
+
+// ---- small outputs: a workgroup owns 16 columns of 16 * MT rows, its eight waves a share of K each, straight from memory into the
+// instruction's operands (a lane holds 16 consecutive bytes of one row); the eight sums meet in LDS.
+template <int MT, typename TC>
+__global__ __launch_bounds__(512) void gemm_i8_rows_kernel(Params8 p) {
+    __shared__ i32x4 sums[8][MT][64];
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+    i32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    const signed char* w = p.W + (long long)min(n0 + fr, p.N - 1) * p.ldw;
+    const signed char* a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) a[i] = p.A + (long long)min(m0 + i * 16 + fr, p.M - 1) * p.lda;    // rows behind the end repeat the last
+    constexpr int U = MT < 4 ? 4 : 2;      // turns whose loads are in flight together
+    for (int k0 = wid * 64; k0 < p.K; k0 += U * 512) {
+        i32x4 wv[U], av[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * 512 + fq * 16;
+            const bool in = k < p.K;
+            wv[u] = in ? *(const i32x4*)(w + k) : i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < MT; ++i) av[u][i] = in ? *(const i32x4*)(a[i] + k) : i32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u], before_end(av[u][i], k0 + u * 512 + fq * 16, p.K), acc[i], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[wid][i][lane] = acc[i];
+    __syncthreads();
+    if (wid >= MT) return;
+    i32x4 s = sums[0][wid][lane];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) s += sums[j][wid][lane];
+    const int m = m0 + wid * 16 + fr, n = n0 + fq * 4;
+    if (m >= p.M || n >= p.N) return;
+    const f32x4 v = scaled(s, p.a_scale[m], four(p.w_scale, n, p.N), p.bias ? four(p.bias, n, p.N) : f32x4{0.f, 0.f, 0.f, 0.f});
+    TC* row = (TC*)p.C + m * p.ldc;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < p.N) Elem<TC>::st(row + n + e, v[e]);
+}
+
+// ---- BM x BN tiles, one per workgroup of NW waves: both operands by LDS-DMA into a ring of four slabs, three ahead, one barrier
+// per slab.  An image row is 128 bytes; its piece c lies in slot c ^ (row & 7) (the swizzle is on the source's side, the
+// DMA writes in lane order), so the 16 rows of a fragment read fall on different banks.
+template <int BM, int BN, int NW, typename TC>
+__global__ __launch_bounds__(NW * 64) void gemm_i8_tile_kernel(Params8 p, int tiles_m, int tiles_n) {
+    constexpr int STAGES = 4, STAGE = (BM + BN) * SLAB, WAVES_N = NW / 2, MT = BM / 2 / 16, NT = BN / WAVES_N / 16;
+    constexpr int DA = BM / 8 / NW, DB = BN / 8 / NW;                   // DMA instructions per wave: eight rows each
+    constexpr int ROW = BN * (int)sizeof(TC) + 16;                      // row of the C image
+    static_assert(DA + DB == 4, "the counted waits below");
+    static_assert(STAGES * STAGE >= BM * ROW, "the C image takes the ring's place");
+    __shared__ __attribute__((aligned(16))) unsigned char smem[STAGES * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wid / WAVES_N, wn = wid % WAVES_N, fr = lane & 15, fq = lane >> 4;
+    int tm, tn;
+    tile_at(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+    const int m0 = tm * BM, n0 = tn * BN, nk = (p.K + SLAB - 1) / SLAB;
+    const __amdgpu_buffer_rsrc_t ra = rows_of(p.A, p.lda, m0, BM, p.M, p.K), rw = rows_of(p.W, p.ldw, n0, BN, p.N, p.K);
+    const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+    auto stage = [&](int slab) {
+        unsigned char* dst = smem + (slab & (STAGES - 1)) * STAGE;
+        const int k = slab * SLAB + piece;
+#pragma unroll
+        for (int j = 0; j < DA; ++j) {
+            const int r = (DA * wid + j) * 8;
+            load_lds(ra, dst + r * SLAB, k < p.K ? (unsigned)((r + (lane >> 3)) * (int)p.lda + k) : OUTSIDE);
+        }
+#pragma unroll
+        for (int j = 0; j < DB; ++j) {
+            const int r = (DB * wid + j) * 8;
+            load_lds(rw, dst + (BM + r) * SLAB, k < p.K ? (unsigned)((r + (lane >> 3)) * (int)p.ldw + k) : OUTSIDE);
+        }
+    };
+    i32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int d = 0; d < STAGES - 1; ++d)
+        if (d < nk) stage(d);
+#pragma unroll 1
+    for (int t = 0; t < nk; ++t) {
+        const int rem = min(STAGES - 2, nk - 1 - t);                    // slabs behind this one that may still be in flight
+        if (rem == 2) VMCNT(8);                                         // four instructions each
+        else if (rem == 1) VMCNT(4);
+        else VMCNT(0);
+        BARRIER();                                                      // slab t is here; every wave is done with slab t - 1
+        if (t + STAGES - 1 < nk) stage(t + STAGES - 1);
+        const unsigned char* img = smem + (t & (STAGES - 1)) * STAGE;
+        i32x4 a[2][MT], w[2][NT];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const int slot = ((ks * 4 + fq) ^ (fr & 7)) * 16;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) a[ks][i] = *(const i32x4*)(img + (wm * (BM / 2) + i * 16 + fr) * SLAB + slot);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) w[ks][j] = *(const i32x4*)(img + (BM + wn * (BN / WAVES_N) + j * 16 + fr) * SLAB + slot);
+        }
+        if (t == nk - 1 && (p.K & 15)) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) a[ks][i] = before_end(a[ks][i], t * SLAB + ks * 64 + fq * 16, p.K);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[ks][j], a[ks][i], acc[i][j], 0, 0, 0);
+    }
+    BARRIER();                                                          // the last slab has been read
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int n = wn * (BN / WAVES_N) + j * 16 + fq * 4;
+        const f32x4 ws = four(p.w_scale, n0 + n, p.N), b = p.bias ? four(p.bias, n0 + n, p.N) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int m = wm * (BM / 2) + i * 16 + fr;
+            put4((TC*)(smem + m * ROW) + n, scaled(acc[i][j], p.a_scale[min(m0 + m, p.M - 1)], ws, b));
+        }
+    }
+    __syncthreads();
+    constexpr int PIECES = BN * (int)sizeof(TC) / 16;
+#pragma unroll 4
+    for (int i = tid; i < BM * PIECES; i += NW * 64) {
+        const int m = i / PIECES, c = i % PIECES;
+        if (m0 + m < p.M) store16<false>((TC*)p.C + (m0 + m) * p.ldc, n0 + c * (16 / (int)sizeof(TC)), p.N, *(const u32x4*)(smem + m * ROW + c * 16));
+    }
+}
+
+// ---- 256 x 256 tiles, eight waves, persistent: the scheme of gemm256q_kernel (gemm.hip).  A slab is four half tiles of 128 rows
+// (A0 A1 W0 W1, 16 KiB each), two buffers of them; a phase multiplies one half of A with both halves of W (32
+// instructions per wave) while the halves that were read last are refilled two slabs ahead; the waits are counted, and
+// waves 4-7 run one barrier behind waves 0-3, so that on every SIMD one wave multiplies while the other reads.  The
+// first loads of the next tile are issued before C leaves through the buffers that they do not use.
+// TAIL: K is no multiple of 16.  (A form of its own: the kernel uses all 256 registers, and the masks cost some.)
+template <typename TC, bool TAIL>
+__global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tiles_m, int tiles_n, int whole, int units) {
+    constexpr int HALF = 128 * SLAB;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[9 * HALF];
+    __shared__ __attribute__((aligned(16))) float scales[3][256];       // a_scale, w_scale and bias of the tile
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wid >> 2, wc = wid & 3, fr = lane & 15, fq = lane >> 4, nk = (p.K + SLAB - 1) / SLAB;
+    const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+    const unsigned va = (unsigned)((16 * wid + (lane >> 3)) * (int)p.lda + piece), vw = (unsigned)((16 * wid + (lane >> 3)) * (int)p.ldw + piece);
+    __amdgpu_buffer_rsrc_t ra, rw;
+    bool full = true;                      // a whole tile; else (the tail of the grid) rows m0 .. m0 + 127 only
+    int m0, n0;
+    float s0, s1;                          // this thread's share of the next tile's scales, on their way
+    auto set_tile = [&](int unit) {
+        int tm, tn, tile = unit, low = 0;
+        full = unit < whole;
+        if (!full) { tile = whole + ((unit - whole) >> 1); low = (unit - whole) & 1; }
+        tile_at(tile, tiles_m, tiles_n, &tm, &tn);
+        m0 = tm * 256 + low * 128;
+        n0 = tn * 256;
+        ra = rows_of(p.A, p.lda, m0, full ? 256 : 128, p.M, p.K);
+        rw = rows_of(p.W, p.ldw, n0, 256, p.N, p.K);
+        const int m = min(m0 + (tid & 255), p.M - 1), n = min(n0 + (tid & 255), p.N - 1);
+        s0 = tid < 256 ? p.a_scale[m] : p.w_scale[n];
+        s1 = p.bias ? p.bias[n] : 0.f;
+    };
+    auto dma = [&](int buf, int slot, int t) {                          // half tile `slot` of slab t into buffer buf
+        unsigned char* dst = smem + (buf * 4 + slot) * HALF + 2 * wid * 1024;
+        const bool in = t * SLAB + piece < p.K;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int piece = tid + 256 * i, row = piece >> 2, k = k0 + (piece & 3) * 16;
-            i32x4 a = {0, 0, 0, 0}, w = {0, 0, 0, 0};
-            if (k < p.K) {
-                if (m0 + row < p.M) a = before_end(*(const i32x4*)(p.A + (m0 + row) * p.lda + k), k, p.K);
-                if (n0 + row < p.N) w = *(const i32x4*)(p.W + (n0 + row) * p.ldw + k);
-            }
-            *(i32x4*)(As + row * LD + (piece & 3) * 16) = a;
-            *(i32x4*)(Ws + row * LD + (piece & 3) * 16) = w;
+            if (slot < 2) load_lds(ra, dst + i * 1024, in ? va + (unsigned)(((slot & 1) * 128 + i * 8) * (int)p.lda + t * SLAB) : OUTSIDE);
+            else load_lds(rw, dst + i * 1024, in ? vw + (unsigned)(((slot & 1) * 128 + i * 8) * (int)p.ldw + t * SLAB) : OUTSIDE);
         }
-        __syncthreads();
-        i32x4 a[4], w[4];
+    };
+    auto prologue = [&]() {                                             // slab 0, and A0 of slab 1
+        dma(0, 0, 0); dma(0, 2, 0); dma(0, 3, 0); dma(0, 1, 0);
+        if (nk > 1) dma(1, 0, 1);
+    };
+    int oa[2], ow[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a[i] = *(const i32x4*)(As + (wr * 64 + i * 16 + fr) * LD + fq * 16);
-            w[i] = *(const i32x4*)(Ws + (wc * 64 + i * 16 + fr) * LD + fq * 16);
-        }
+    for (int ks = 0; ks < 2; ++ks) {
+        const int slot = ((ks * 4 + fq) ^ (fr & 7)) * 16;
+        oa[ks] = (wr * 64 + fr) * SLAB + slot;
+        ow[ks] = (wc * 32 + fr) * SLAB + slot;
+    }
+    i32x4 af[4][2], wf[2][2][2], acc[2][2][4][2];
+    auto load_a = [&](int buf, int mh, int t) {
+        const unsigned char* b = smem + (buf * 4 + mh) * HALF;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], a[i], acc[i][j], 0, 0, 0);
-    }
-    // W stands where the instruction takes its first operand: a lane holds four consecutive n of one m
+            for (int ks = 0; ks < 2; ++ks) af[i][ks] = *(const i32x4*)(b + oa[ks] + i * 16 * SLAB);
+        if (TAIL && t == nk - 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int m = m0 + wr * 64 + i * 16 + fr;
-        if (m >= p.M) continue;
-        const float as = p.a_scale[m];
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + wc * 64 + j * 16 + fq * 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < p.N) {
-                    float v = (float)acc[i][j][e] * p.w_scale[n + e] * as;
-                    if (p.bias) v += p.bias[n + e];
-                    Elem<TC>::st((TC*)p.C + m * p.ldc + n + e, v);
-                }
+                for (int ks = 0; ks < 2; ++ks) af[i][ks] = before_end(af[i][ks], t * SLAB + ks * 64 + fq * 16, p.K);
         }
+    };
+    auto load_w = [&](int buf, int nh) {
+        const unsigned char* b = smem + (buf * 4 + 2 + nh) * HALF;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) wf[nh][j][ks] = *(const i32x4*)(b + ow[ks] + j * 16 * SLAB);
+    };
+#define MMA(MH, NH)                                                                                          \
+    do {                                                                                                     \
+        __builtin_amdgcn_s_setprio(1);                                                                       \
+        _Pragma("unroll") for (int ks = 0; ks < 2; ++ks)                                                     \
+        _Pragma("unroll") for (int i = 0; i < 4; ++i)                                                        \
+        _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                        \
+            acc[MH][NH][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[NH][j][ks], af[i][ks], acc[MH][NH][i][j], 0, 0, 0); \
+        __builtin_amdgcn_s_setprio(0);                                                                       \
+    } while (0)
+
+    int unit = blockIdx.x;
+    set_tile(unit);
+    prologue();
+    while (true) {
+#pragma unroll
+        for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+            for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[mh][nh][i][j] = i32x4{0, 0, 0, 0};
+        BARRIER();                                                      // every wave is done with the C image and the scales
+        scales[tid >> 8][tid & 255] = s0;
+        if (tid >= 256) scales[2][tid & 255] = s1;
+        if (nk > 1) { dma(1, 2, 1); dma(1, 3, 1); VMCNT(4); } else { VMCNT(0); }
+        LGKMCNT0();
+        BARRIER();
+        if (wr == 1) BARRIER();
+        for (int t = 0; t < nk; ++t) {
+            const int b = t & 1, nb = b ^ 1;
+            const bool n1 = t + 1 < nk, n2 = t + 2 < nk;
+            load_w(b, 0);
+            load_w(b, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            load_a(b, 0, t);
+            if (n1) { dma(nb, 1, t + 1); VMCNT(8); } else { VMCNT(0); }                          // A1(t) is here
+            BARRIER();
+            MMA(0, 0);
+            MMA(0, 1);
+            BARRIER();
+            if (full) load_a(b, 1, t);
+            if (n2) { dma(b, 0, t + 2); dma(b, 2, t + 2); dma(b, 3, t + 2); VMCNT(8); }          // A0 W0 W1 (t + 1) are here
+            else if (n1) { VMCNT(2); }
+            BARRIER();
+            if (full) {
+                MMA(1, 0);
+                MMA(1, 1);
+            }
+            BARRIER();
+        }
+        if (wr == 0) BARRIER();                                         // all waves are past their last read of the buffers
+        const int em = m0, en = n0, next = unit + (int)gridDim.x;
+        const bool was_full = full;
+        if (next < units) {
+            set_tile(next);
+            prologue();
+        }
+        // C by quarters of 64 rows (32 of each wave group) through an image in the last four half tiles; 16-bit quarters
+        // alternate between two images, so one barrier per quarter is enough
+        constexpr int ROW = 256 * (int)sizeof(TC), IMAGES = sizeof(TC) == 2 ? 2 : 1;
+        f32x4 ws[2][2], bs[2][2];
+#pragma unroll
+        for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int n = nh * 128 + wc * 32 + j * 16 + fq * 4;
+                ws[nh][j] = *(const f32x4*)&scales[1][n];
+                bs[nh][j] = *(const f32x4*)&scales[2][n];
+            }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (q == 2 && !was_full) break;
+            unsigned char* img = smem + 5 * HALF + (q % IMAGES) * 64 * ROW;
+            if (q && IMAGES == 1) BARRIER();                            // the previous quarter's image has been read
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = wr * 32 + j * 16 + fr, m = (q >> 1) * 128 + wr * 64 + ((q & 1) * 2 + j) * 16 + fr;
+                const float as = scales[0][m];
+#pragma unroll
+                for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+                    for (int jn = 0; jn < 2; ++jn) {
+                        const int c = nh * 32 + wc * 8 + jn * 4 + fq;   // group of four columns
+                        const f32x4 v = scaled(acc[q >> 1][nh][(q & 1) * 2 + j][jn], as, ws[nh][jn], bs[nh][jn]);
+                        if constexpr (sizeof(TC) == 2) put4((TC*)(img + r * ROW + ((c ^ (fr << 1)) << 3)), v);
+                        else put4((TC*)(img + r * ROW + ((c ^ fr) << 4)), v);
+                    }
+            }
+            LGKMCNT0();
+            BARRIER();
+            constexpr int PIECES = ROW / 16;
+#pragma unroll
+            for (int i = 0; i < 64 * PIECES / 512; ++i) {
+                const int r = (tid + 512 * i) / PIECES, c = (tid + 512 * i) % PIECES;
+                const int m = em + (q >> 1) * 128 + (r >> 5) * 64 + (q & 1) * 32 + (r & 31);
+                u32x4 v;
+                if constexpr (sizeof(TC) == 2) v = *(const u32x4*)(img + r * ROW + (((2 * c) ^ ((r & 15) << 1)) << 3));
+                else v = *(const u32x4*)(img + r * ROW + ((c ^ (r & 15)) << 4));
+                if (m < p.M) store16<true>((TC*)p.C + m * p.ldc, en + c * (16 / (int)sizeof(TC)), p.N, v);
+            }
+            LGKMCNT0();
+        }
+        if (next >= units) break;
+        unit = next;
     }
+#undef MMA
+}
+
+template <typename TC> int launch_gemm_i8(const Params8& p, hipStream_t st) {
+    const long long t256 = ((p.M + 255ll) / 256) * ((p.N + 255ll) / 256), t128 = ((p.M + 127ll) / 128) * ((p.N + 127ll) / 128);
+    const long long t64 = ((p.M + 63ll) / 64) * ((p.N + 63ll) / 64);
+    if (t256 > (1 << 28)) return STDIFF_ERR_SHAPE;
+    const int cus = cu_count();
+    // small outputs: bytes of K that the busiest CU reads, a workgroup of 16 x 16 MT against a tile of 64 x 64 (the latter
+    // through LDS, 1.5 times as fast a byte)
+    const auto busiest = [&](int mt) { return ((p.N + 15ll) / 16 * ((p.M + 16ll * mt - 1) / (16 * mt)) + cus - 1) / cus * (16 + 16 * mt) * 3 / 2; };
+    const long long r1 = busiest(1), r2 = busiest(2), r4 = busiest(4), least = std::min(r1, std::min(r2, r4));
+    const int kind = least <= (t64 + cus - 1) / cus * 128 ? 1 : t256 >= cus * 3 / 8 ? 4 : t64 > 2 * cus ? 3 : 2;
+    if (kind == 1) {
+        const int mt = least == r1 ? 1 : least == r2 ? 2 : 4;
+        const dim3 grid(cdiv(p.N, 16), cdiv(p.M, 16 * mt));
+        if (mt == 1) hipLaunchKernelGGL((gemm_i8_rows_kernel<1, TC>), grid, dim3(512), 0, st, p);
+        else if (mt == 2) hipLaunchKernelGGL((gemm_i8_rows_kernel<2, TC>), grid, dim3(512), 0, st, p);
+        else hipLaunchKernelGGL((gemm_i8_rows_kernel<4, TC>), grid, dim3(512), 0, st, p);
+    } else if (kind == 2) {
+        hipLaunchKernelGGL((gemm_i8_tile_kernel<64, 64, 4, TC>), dim3((unsigned)t64), dim3(256), 0, st, p, cdiv(p.M, 64), cdiv(p.N, 64));
+    } else if (kind == 3) {
+        hipLaunchKernelGGL((gemm_i8_tile_kernel<128, 128, 8, TC>), dim3((unsigned)t128), dim3(512), 0, st, p, cdiv(p.M, 128), cdiv(p.N, 128));
+    } else {
+        // a last round of fewer than half the CUs' tiles is cut into half tiles, so that it costs half
+        const int tail = (int)(t256 % cus);
+        const int whole = tail && tail <= cus / 2 ? (int)t256 - tail : (int)t256, units = whole + 2 * ((int)t256 - whole);
+        if (p.K % 16)
+            hipLaunchKernelGGL((gemm_i8_256_kernel<TC, true>), dim3(std::min(units, cus)), dim3(512), 0, st, p, cdiv(p.M, 256),
+                               cdiv(p.N, 256), whole, units);
+        else
+            hipLaunchKernelGGL((gemm_i8_256_kernel<TC, false>), dim3(std::min(units, cus)), dim3(512), 0, st, p, cdiv(p.M, 256),
+                               cdiv(p.N, 256), whole, units);
+    }
+    STDIFF_LAUNCH_STATUS();
+    return STDIFF_OK;
 }
 
 }  // namespace
@@ -157,15 +580,8 @@ extern "C" int stdiff_quantize_rows(const void* x, long long ldx, int x_dtype, v
     if (K > (1 << 30)) return STDIFF_ERR_SHAPE;
     STDIFF_CHECK_ARG(ldq >= (K + 15) / 16 * 16);
     if (ldq % 16 || ((uintptr_t)q & 15) || ((uintptr_t)x & (dtype_size(x_dtype) - 1)) || ((uintptr_t)scale & 3)) return STDIFF_ERR_ALIGN;
-    const dim3 grid((unsigned)std::min<long long>(R, 16ll * cu_count()));
-    if (x_dtype == STDIFF_BF16)
-        hipLaunchKernelGGL(quantize_rows_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, (const bf16_t*)x, ldx,
-                           (signed char*)q, ldq, scale, R, K);
-    else
-        hipLaunchKernelGGL(quantize_rows_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, (const float*)x, ldx,
-                           (signed char*)q, ldq, scale, R, K);
-    STDIFF_LAUNCH_STATUS();
-    return STDIFF_OK;
+    return x_dtype == STDIFF_BF16 ? launch_quantize<bf16_t>(x, ldx, q, ldq, scale, R, K, (hipStream_t)stream)
+                                  : launch_quantize<float>(x, ldx, q, ldq, scale, R, K, (hipStream_t)stream);
 }
 
 extern "C" int stdiff_gemm_i8(const stdiff_gemm_i8_args* a, void* stream) {
@@ -181,13 +597,5 @@ extern "C" int stdiff_gemm_i8(const stdiff_gemm_i8_args* a, void* stream) {
         return STDIFF_ERR_ALIGN;
     Params8 p = {a->M, a->N, a->K, (const signed char*)a->A, a->lda, (const signed char*)a->W, a->ldw, a->a_scale, a->w_scale,
                  a->bias, a->C, a->ldc};
-    const long long ty = ((long long)a->M + 127) / 128;
-    if (ty > 65535) return STDIFF_ERR_SHAPE;
-    const dim3 grid(cdiv(a->N, 128), (unsigned)ty);
-    if (a->c_dtype == STDIFF_BF16)
-        hipLaunchKernelGGL(gemm_i8_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, p);
-    else
-        hipLaunchKernelGGL(gemm_i8_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, p);
-    STDIFF_LAUNCH_STATUS();
-    return STDIFF_OK;
+    return a->c_dtype == STDIFF_BF16 ? launch_gemm_i8<bf16_t>(p, (hipStream_t)stream) : launch_gemm_i8<float>(p, (hipStream_t)stream);
 }

@@ -14,51 +14,62 @@ typedef f32x4 f32x4_u __attribute__((aligned(4)));       // rows may begin at an
 typedef u32x4 u32x4_u __attribute__((aligned(2)));       // 16 bytes need no alignment in global memory
 typedef u32x2 u32x2_u __attribute__((aligned(2)));
 
-template <int V> __device__ __forceinline__ void ldv(const float* p, float* o) {
+// NT: past the caches (for what is used once and is larger than they are)
+template <int V, bool NT = false> __device__ __forceinline__ void ldv(const float* p, float* o) {
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-        const f32x4 v = *(const f32x4_u*)(p + i);
+        const f32x4 v = NT ? __builtin_nontemporal_load((const f32x4_u*)(p + i)) : *(const f32x4_u*)(p + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i + j] = v[j];
     }
 }
-template <int V> __device__ __forceinline__ void ldv(const bf16_t* p, float* o) {
+template <int V, bool NT = false> __device__ __forceinline__ void ldv(const bf16_t* p, float* o) {
     if constexpr (V == 8) {
-        const u32x4 v = *(const u32x4_u*)p;
+        const u32x4 v = NT ? __builtin_nontemporal_load((const u32x4_u*)p) : *(const u32x4_u*)p;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { o[2 * j] = bf_lo(v[j]); o[2 * j + 1] = bf_hi(v[j]); }
     } else {
-        const u32x2 v = *(const u32x2_u*)p;
+        const u32x2 v = NT ? __builtin_nontemporal_load((const u32x2_u*)p) : *(const u32x2_u*)p;
 #pragma unroll
         for (int j = 0; j < 2; ++j) { o[2 * j] = bf_lo(v[j]); o[2 * j + 1] = bf_hi(v[j]); }
     }
 }
-template <int V> __device__ __forceinline__ void stv(float* p, const float* o) {
+template <int V, bool NT = false> __device__ __forceinline__ void stv(float* p, const float* o) {
 #pragma unroll
-    for (int i = 0; i < V; i += 4) *(f32x4_u*)(p + i) = f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+    for (int i = 0; i < V; i += 4) {
+        const f32x4 v = {o[i], o[i + 1], o[i + 2], o[i + 3]};
+        if (NT) __builtin_nontemporal_store(v, (f32x4_u*)(p + i));
+        else *(f32x4_u*)(p + i) = v;
+    }
 }
-template <int V> __device__ __forceinline__ void stv(bf16_t* p, const float* o) {
-    if constexpr (V == 8)
-        *(u32x4_u*)p = u32x4{pack2bf(o[0], o[1]), pack2bf(o[2], o[3]), pack2bf(o[4], o[5]), pack2bf(o[6], o[7])};
-    else
-        *(u32x2_u*)p = u32x2{pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+template <int V, bool NT = false> __device__ __forceinline__ void stv(bf16_t* p, const float* o) {
+    if constexpr (V == 8) {
+        const u32x4 v = {pack2bf(o[0], o[1]), pack2bf(o[2], o[3]), pack2bf(o[4], o[5]), pack2bf(o[6], o[7])};
+        if (NT) __builtin_nontemporal_store(v, (u32x4_u*)p);
+        else *(u32x4_u*)p = v;
+    } else {
+        const u32x2 v = {pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+        if (NT) __builtin_nontemporal_store(v, (u32x2_u*)p);
+        else *(u32x2_u*)p = v;
+    }
 }
 // V elements at column c of a row of H; what lies behind the row's end reads as `fill` and is not written
-template <int V, typename T> __device__ __forceinline__ void ld_edge(const T* row, int c, int H, float fill, float* o) {
-    if (c + V <= H) return ldv<V>(row + c, o);
+template <int V, bool NT = false, typename T> __device__ __forceinline__ void ld_edge(const T* row, int c, int H, float fill, float* o) {
+    if (c + V <= H) return ldv<V, NT>(row + c, o);
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = c + j < H ? Elem<T>::ld(row + c + j) : fill;
 }
-template <int V, typename T> __device__ __forceinline__ void st_edge(T* row, int c, int H, const float* o) {
-    if (c + V <= H) return stv<V>(row + c, o);
+template <int V, bool NT = false, typename T> __device__ __forceinline__ void st_edge(T* row, int c, int H, const float* o) {
+    if (c + V <= H) return stv<V, NT>(row + c, o);
 #pragma unroll
     for (int j = 0; j < V; ++j)
         if (c + j < H) Elem<T>::st(row + c + j, o[j]);
 }
 
 // sum over the T lanes of a row, the same bits in all of them; `part`: T / 64 floats per use, not reused before a barrier
-template <int T> __device__ __forceinline__ float row_sum(float v, float* part) {
-    v = wave_sum(v);
+template <int T, int NTHR = 256> __device__ __forceinline__ float row_sum(float v, float* part) {
+    static_assert(T == 64 || T == NTHR, "a row is one wave's or the whole workgroup's");
+    v = wave_sum_dpp(v);
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -69,7 +80,7 @@ template <int T> __device__ __forceinline__ float row_sum(float v, float* part) 
     return v;
 }
 
-template <typename TX, typename TY, typename TW, int V, int NV, int T>
+template <typename TX, typename TY, typename TW, int V, int NV, int T, bool NT>
 __global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long ldx, const TW* w, const TW* b, float eps,
                                                          TY* y, long long ldy, float* mean, float* rstd, int R, int H) {
     __shared__ float part[2][2][T / 64];
@@ -89,7 +100,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long 
     for (long long row = (long long)blockIdx.x * ROWS + threadIdx.x / T; row < R; row += (long long)gridDim.x * ROWS, odd ^= 1) {
         float v[NV][V], s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) ld_edge<V>(x + row * ldx, (i * T + t) * V, H, 0.f, v[i]);
+        for (int i = 0; i < NV; ++i) ld_edge<V, NT>(x + row * ldx, (i * T + t) * V, H, 0.f, v[i]);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -109,7 +120,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long 
             float o[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = v[i][j] * rs * wv[i][j] + bv[i][j];
-            st_edge<V>(y + row * ldy, (i * T + t) * V, H, o);
+            st_edge<V, NT>(y + row * ldy, (i * T + t) * V, H, o);
         }
         if (t == 0) {
             if (mean) mean[row] = mu;
@@ -158,16 +169,13 @@ __global__ __launch_bounds__(256) void layer_norm_long_kernel(const TX* x, long 
     }
 }
 
-// ws (or NULL: no weight gradient is asked for): [gridDim.x][2][ldp] partial sums of (dy * xhat, dy), one pair per block
-template <typename TX, typename TD, typename TW, int V, int NV, int T>
-__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
-                                                             const float* mean, const float* rstd, const TW* w, TX* dx,
-                                                             long long lddx, float* ws, int ldp, int R, int H) {
-    __shared__ float part[2][2][T / 64];
-    __shared__ float comb[T == 64 ? 64 * V * NV : 1];
-    constexpr int ROWS = 256 / T;
-    const int t = threadIdx.x % T;
-    float wv[NV][V], aw[NV][V], ab[NV][V];
+// dx of the rows first, first + step, ..; SUMS: also this thread's share of sum dy * xhat and sum dy of its columns
+template <typename TX, typename TD, typename TW, int V, int NV, int T, int NTHR, bool SUMS, bool NT>
+__device__ __forceinline__ void norm_bwd_rows(const TD* dy, long long lddy, const TX* x, long long ldx, const float* mean,
+                                              const float* rstd, const TW* w, TX* dx, long long lddx, int R, int H, int t,
+                                              long long first, long long step, float (&aw)[NV][V], float (&ab)[NV][V]) {
+    __shared__ float part[2][2][NTHR / 64];
+    float wv[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
@@ -176,60 +184,131 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const TD* dy, long 
     }
     const float inv = 1.0f / (float)H;
     int odd = 0;
-    for (long long row = (long long)blockIdx.x * ROWS + threadIdx.x / T; row < R; row += (long long)gridDim.x * ROWS, odd ^= 1) {
+    for (long long row = first; row < R; row += step, odd ^= 1) {
         float d[NV][V], h[NV][V], sg = 0.f, sgx = 0.f;
         const float mu = mean[row], rs = rstd[row];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            ld_edge<V>(dy + row * lddy, (i * T + t) * V, H, 0.f, d[i]);     // behind the end dy = 0: nothing is added
-            ld_edge<V>(x + row * ldx, (i * T + t) * V, H, 0.f, h[i]);
+            ld_edge<V, NT>(dy + row * lddy, (i * T + t) * V, H, 0.f, d[i]); // behind the end dy = 0: nothing is added
+            ld_edge<V, NT>(x + row * ldx, (i * T + t) * V, H, 0.f, h[i]);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 h[i][j] = (h[i][j] - mu) * rs;
-                aw[i][j] += d[i][j] * h[i][j];
-                ab[i][j] += d[i][j];
+                if constexpr (SUMS) {
+                    aw[i][j] += d[i][j] * h[i][j];
+                    ab[i][j] += d[i][j];
+                }
                 d[i][j] *= wv[i][j];
                 sg += d[i][j];
                 sgx += d[i][j] * h[i][j];
             }
-        const float mg = row_sum<T>(sg, part[odd][0]) * inv, mgx = row_sum<T>(sgx, part[odd][1]) * inv;
+        const float mg = row_sum<T, NTHR>(sg, part[odd][0]) * inv, mgx = row_sum<T, NTHR>(sgx, part[odd][1]) * inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float o[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = rs * (d[i][j] - mg - h[i][j] * mgx);
-            st_edge<V>(dx + row * lddx, (i * T + t) * V, H, o);
+            st_edge<V, NT>(dx + row * lddx, (i * T + t) * V, H, o);
         }
     }
+}
+
+// Many rows.  Every workgroup walks its rows with the column sums in registers and leaves one pair of partial sums:
+// ws [gridDim.x][2][ldp] of (dy * xhat, dy); ws NULL: dx only.
+template <typename TX, typename TD, typename TW, int V, int NV, int T, bool NT>
+__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
+                                                             const float* mean, const float* rstd, const TW* w, TX* dx,
+                                                             long long lddx, float* ws, int ldp, int R, int H) {
+    constexpr int WIDTH = 64 * V * NV;               // columns that a wave's registers cover (T == 64)
+    __shared__ __attribute__((aligned(16))) float comb[T == 64 ? 4 * WIDTH : 4];
+    constexpr int ROWS = 256 / T;
+    const int t = threadIdx.x % T;
+    float aw[NV][V], ab[NV][V];
+    norm_bwd_rows<TX, TD, TW, V, NV, T, 256, true, NT>(dy, lddy, x, ldx, mean, rstd, w, dx, lddx, R, H, t,
+                                                   (long long)blockIdx.x * ROWS + threadIdx.x / T, (long long)gridDim.x * ROWS, aw, ab);
     if (!ws) return;
     float* out = ws + (size_t)blockIdx.x * 2 * ldp;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        float(&a)[NV][V] = k ? ab : aw;
+        const float(&a)[NV][V] = k ? ab : aw;
         if constexpr (T == 64) {                     // the block's four waves, added in their order
-            for (int wave = 0; wave < 4; ++wave) {
-                if ((threadIdx.x >> 6) == wave)
+            if (k) __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-                        for (int j = 0; j < V; ++j) {
-                            float& c = comb[(i * V + j) * 64 + t];
-                            c = wave ? c + a[i][j] : a[i][j];
-                            if (wave == 3) a[i][j] = c;
-                        }
-                __syncthreads();
+                for (int j = 0; j < V; j += 4)
+                    *(f32x4*)(comb + (threadIdx.x >> 6) * WIDTH + (i * 64 + t) * V + j) = f32x4{a[i][j], a[i][j + 1], a[i][j + 2], a[i][j + 3]};
+            __syncthreads();
+            for (int c = threadIdx.x * 4; c < ldp; c += 1024) {
+                f32x4 s = *(const f32x4*)(comb + c);
+#pragma unroll
+                for (int i = 1; i < 4; ++i) s += *(const f32x4*)(comb + i * WIDTH + c);
+                *(f32x4*)(out + k * ldp + c) = s;
             }
-            if ((threadIdx.x >> 6) == 3)
-#pragma unroll
-                for (int i = 0; i < NV; ++i) st_edge<V>(out + k * ldp, (i * T + t) * V, H, a[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i) st_edge<V>(out + k * ldp, (i * T + t) * V, H, a[i]);
         }
     }
+}
+
+// Few rows, one launch: the column sums need only the statistics, which are there already, so they do not wait for dx.  The
+// first `cols` workgroups own 32 columns each and walk down ALL rows (x and dy are read twice, the second time from the
+// cache); the others own rows and give dx.
+template <typename TX, typename TD, typename TW, int V, int NV, int T>
+__global__ __launch_bounds__(512) void layer_norm_bwd_few_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
+                                                                 const float* mean, const float* rstd, const TW* w, TX* dx,
+                                                                 long long lddx, float* dweight, float* dbias, int accumulate,
+                                                                 int cols, int R, int H) {
+    if ((int)blockIdx.x >= cols) {
+        constexpr int ROWS = 512 / T;
+        float aw[NV][V], ab[NV][V];
+        norm_bwd_rows<TX, TD, TW, V, NV, T, 512, false, false>(dy, lddy, x, ldx, mean, rstd, w, dx, lddx, R, H, threadIdx.x % T,
+                                                        (long long)(blockIdx.x - cols) * ROWS + threadIdx.x / T,
+                                                        (long long)(gridDim.x - cols) * ROWS, aw, ab);
+        return;
+    }
+    constexpr int LANES = 32 / V, SLOTS = 512 / LANES;
+    __shared__ float sums[2][SLOTS][32 + 1];
+    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, c = blockIdx.x * 32 + lane * V;
+    float aw[V], ab[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) aw[j] = ab[j] = 0.f;
+#pragma unroll 4
+    for (int row = slot; row < R; row += SLOTS) {
+        float d[V], h[V];
+        ld_edge<V>(dy + row * lddy, c, H, 0.f, d);
+        ld_edge<V>(x + row * ldx, c, H, 0.f, h);
+        const float mu = mean[row], rs = rstd[row];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            aw[j] += d[j] * ((h[j] - mu) * rs);
+            ab[j] += d[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        sums[0][slot][lane * V + j] = aw[j];
+        sums[1][slot][lane * V + j] = ab[j];
+    }
+    __syncthreads();
+    // 64 sums (two of 32 columns) of SLOTS terms each: eight threads per sum, then their eight in order
+    const int col = threadIdx.x & 31, which = (threadIdx.x >> 5) & 1, share = threadIdx.x >> 6;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < SLOTS / 8; ++i) s += sums[which][share * (SLOTS / 8) + i][col];
+    __syncthreads();
+    sums[which][share][col] = s;
+    __syncthreads();
+    float* dst = which ? dbias : dweight;
+    if (share || !dst || blockIdx.x * 32 + col >= H) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += sums[which][i][col];
+    dst += blockIdx.x * 32 + col;
+    *dst = accumulate ? *dst + s : s;
 }
 
 // long rows: dx row by row (two walks over the row), and the column sums by a kernel of their own
@@ -299,8 +378,10 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_join_kernel(const float* w
     const float* src = ws + (size_t)blockIdx.y * ldp + c;
     float* dst = blockIdx.y ? dbias : dweight;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if (c < ldp)
+    if (c < ldp) {
+#pragma unroll 8
         for (int p = slot; p < parts; p += 32) s += *(const f32x4*)(src + (size_t)p * 2 * ldp);
+    }
     sum[slot][lane] = s;
     __syncthreads();
     for (int h = 16; h > 0; h >>= 1) {
@@ -325,20 +406,32 @@ constexpr int IN_REGISTERS = 8192;        // longest row that the register kerne
 inline int norm_blocks(long long R, int rows_per_block, int per_cu) {
     return (int)std::min<long long>((R + rows_per_block - 1) / rows_per_block, (long long)per_cu * cu_count());
 }
+// A call that moves more than the memory-side cache holds (256 MB) goes past the caches: 131072 x 1024 fp32 -> bf16 146 against
+// 155 us, backward of 32768 x 2048 fp32 139 against 150 us.  Below that the next kernel finds the result in a cache.
+inline bool past_caches(long long bytes) { return bytes > (256ll << 20); }
 inline int lanes_per_row(int H) { return H <= 2048 ? 64 : 256; }
 inline int bwd_parts(int R, int H) {
     if (H > IN_REGISTERS) return (int)std::min<long long>(R, 64);
     return norm_blocks(R, 256 / lanes_per_row(H), 2);
 }
+// Up to 1024 rows the column sums walk down the rows in the launch that gives dx (512 x 1024 bf16: 4.0 us against 8.3 with partial
+// sums and a second launch; 1024 x 1024 fp32: 7.0 against 8.7; 2048 x 1024 fp32: 22 against 11)
+inline bool one_launch(int R, int H) { return R <= 1024 && H <= IN_REGISTERS; }
 inline int ld_parts(int H) { return (H + 3) / 4 * 4; }
 
 template <typename TX, typename TY, typename TW>
 int launch_ln(const void* x, long long ldx, const void* w, const void* b, float eps, void* y, long long ldy, float* mean,
               float* rstd, int R, int H, hipStream_t st) {
     constexpr int V = sizeof(TX) == 2 ? 8 : 4, U = 8 / V;
-#define LN(NV, T)                                                                                                              \
-    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, TW, V, NV, T>), dim3(norm_blocks(R, 256 / T, 8)), dim3(256), 0, st, (const TX*)x, \
+#define LN(NV, T)                                                              \
+    do {                                                                       \
+        if (streams) LN_AT(NV, T, true);                                       \
+        else LN_AT(NV, T, false);                                              \
+    } while (0)
+#define LN_AT(NV, T, NT)                                                                                                           \
+    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, TW, V, NV, T, NT>), dim3(norm_blocks(R, 256 / T, 8)), dim3(256), 0, st, (const TX*)x, \
                        ldx, (const TW*)w, (const TW*)b, eps, (TY*)y, ldy, mean, rstd, R, H)
+    const bool streams = past_caches((long long)R * H * (sizeof(TX) + sizeof(TY)));
     if (H <= 512) LN(U, 64);
     else if (H <= 1024) LN(2 * U, 64);
     else if (H <= 2048) LN(4 * U, 64);
@@ -347,19 +440,52 @@ int launch_ln(const void* x, long long ldx, const void* w, const void* b, float 
     else
         hipLaunchKernelGGL((layer_norm_long_kernel<TX, TY, TW>), dim3(norm_blocks(R, 1, 8)), dim3(256), 0, st, (const TX*)x, ldx,
                            (const TW*)w, (const TW*)b, eps, (TY*)y, ldy, mean, rstd, R, H);
-#undef LN
+#undef LN_AT
     STDIFF_LAUNCH_STATUS();
     return STDIFF_OK;
 }
 
 template <typename TX, typename TD, typename TW>
 int launch_ln_grad(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
-                   const void* w, void* dx, long long lddx, float* ws, int parts, int R, int H, hipStream_t st) {
+                   const void* w, void* dx, long long lddx, float* dweight, float* dbias, int accumulate, float* ws, int R, int H,
+                   hipStream_t st) {
     constexpr int V = sizeof(TX) == 2 ? 8 : 4, U = 8 / V;
-    const int ldp = ld_parts(H);
-#define LN(NV, T)                                                                                                               \
-    hipLaunchKernelGGL((layer_norm_bwd_kernel<TX, TD, TW, V, NV, T>), dim3(parts), dim3(256), 0, st, (const TD*)dy, lddy, (const TX*)x, \
-                       ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, ws, ldp, R, H)
+    const int ldp = ld_parts(H), parts = bwd_parts(R, H);
+    if (!ws && (dweight || dbias)) {                  // few rows
+        const int cols = cdiv(H, 32);
+        const auto meets = [&](const void* p, long long ld, size_t size) {
+            const uintptr_t a = (uintptr_t)p, b = (uintptr_t)dx;
+            return a < b + ((R - 1) * lddx + H) * sizeof(TX) && b < a + ((R - 1) * ld + H) * size;
+        };
+        // dx in the place of x or dy: the columns first, in a launch of their own
+        const bool in_place = meets(x, ldx, sizeof(TX)) || meets(dy, lddy, sizeof(TD));
+#define FEW_AT(GRID, COLS, NV, T)                                                                                                    \
+    hipLaunchKernelGGL((layer_norm_bwd_few_kernel<TX, TD, TW, V, NV, T>), dim3(GRID), dim3(512), 0, st, (const TD*)dy, lddy,          \
+                       (const TX*)x, ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, dweight, dbias, accumulate, COLS, R, H)
+#define FEW(NV, T)                                                    \
+    do {                                                              \
+        const int rows = norm_blocks(R, 512 / T, 4);                  \
+        if (in_place) {                                               \
+            FEW_AT(cols, cols, NV, T);                                \
+            FEW_AT(rows, 0, NV, T);                                   \
+        } else {                                                      \
+            FEW_AT(cols + rows, cols, NV, T);                         \
+        }                                                             \
+    } while (0)
+        if (H <= 512) FEW(U, 64);
+        else if (H <= 1024) FEW(2 * U, 64);
+        else if (H <= 2048) FEW(4 * U, 64);
+        else if (H <= 4096) FEW(U, 512);
+        else FEW(2 * U, 512);
+#undef FEW
+#undef FEW_AT
+        STDIFF_LAUNCH_STATUS();
+        return STDIFF_OK;
+    }
+#define LN_AT(NV, T, NT)                                                                                                       \
+    hipLaunchKernelGGL((layer_norm_bwd_kernel<TX, TD, TW, V, NV, T, NT>), dim3(parts), dim3(256), 0, st, (const TD*)dy, lddy,   \
+                       (const TX*)x, ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, ws, ldp, R, H)
+    const bool streams = past_caches((long long)R * H * (2 * sizeof(TX) + sizeof(TD)));
     if (H <= 512) LN(U, 64);
     else if (H <= 1024) LN(2 * U, 64);
     else if (H <= 2048) LN(4 * U, 64);
@@ -372,8 +498,13 @@ int launch_ln_grad(const void* dy, long long lddy, const void* x, long long ldx,
         hipLaunchKernelGGL((layer_norm_bwd_long_kernel<TX, TD, TW>), dim3(norm_blocks(R, 1, 8)), dim3(256), 0, st, (const TD*)dy,
                            lddy, (const TX*)x, ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, R, H);
     }
+#undef LN_AT
 #undef LN
     STDIFF_LAUNCH_STATUS();
+    if (ws) {
+        hipLaunchKernelGGL(layer_norm_bwd_join_kernel, dim3(cdiv(H, 32), 2), dim3(256), 0, st, ws, ldp, parts, dweight, dbias, accumulate, H);
+        STDIFF_LAUNCH_STATUS();
+    }
     return STDIFF_OK;
 }
 
@@ -407,7 +538,7 @@ extern "C" int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, cons
 
 extern "C" long long stdiff_layer_norm_bwd_workspace(int R, int H) {
     if (R < 0 || H <= 0) return STDIFF_ERR_ARG;
-    return (long long)bwd_parts(R, H) * 2 * ld_parts(H) * 4;
+    return one_launch(R, H) ? 0 : (long long)bwd_parts(R, H) * 2 * ld_parts(H) * 4;
 }
 
 extern "C" int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const void* x, long long ldx, int x_dtype,
@@ -429,25 +560,20 @@ extern "C" int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtyp
         }
         return STDIFF_OK;
     }
-    const int parts = bwd_parts(R, H);
-    if (params && (!workspace || workspace_bytes < stdiff_layer_norm_bwd_workspace(R, H))) return STDIFF_ERR_WORKSPACE;
-    float* ws = params ? workspace : nullptr;
-    int rc;
-#define LN(TX, TD, TW) rc = launch_ln_grad<TX, TD, TW>(dy, lddy, x, ldx, mean, rstd, weight, dx, lddx, ws, parts, R, H, st)
+    const long long need = params ? stdiff_layer_norm_bwd_workspace(R, H) : 0;
+    if (need && (!workspace || workspace_bytes < need)) return STDIFF_ERR_WORKSPACE;
+    float* ws = need ? workspace : nullptr;
+#define LN(TX, TD, TW)                                                                                                            \
+    return launch_ln_grad<TX, TD, TW>(dy, lddy, x, ldx, mean, rstd, weight, dx, lddx, dweight, dbias, accumulate, ws, R, H, st)
     switch ((x_dtype == STDIFF_BF16) * 4 + (dy_dtype == STDIFF_BF16) * 2 + (w_dtype == STDIFF_BF16)) {
-        case 0: LN(float, float, float); break;
-        case 1: LN(float, float, bf16_t); break;
-        case 2: LN(float, bf16_t, float); break;
-        case 3: LN(float, bf16_t, bf16_t); break;
-        case 4: LN(bf16_t, float, float); break;
-        case 5: LN(bf16_t, float, bf16_t); break;
-        case 6: LN(bf16_t, bf16_t, float); break;
-        default: LN(bf16_t, bf16_t, bf16_t); break;
+        case 0: LN(float, float, float);
+        case 1: LN(float, float, bf16_t);
+        case 2: LN(float, bf16_t, float);
+        case 3: LN(float, bf16_t, bf16_t);
+        case 4: LN(bf16_t, float, float);
+        case 5: LN(bf16_t, float, bf16_t);
+        case 6: LN(bf16_t, bf16_t, float);
+        default: LN(bf16_t, bf16_t, bf16_t);
     }
 #undef LN
-    if (rc != STDIFF_OK || !params) return rc;
-    hipLaunchKernelGGL(layer_norm_bwd_join_kernel, dim3(cdiv(H, 32), 2), dim3(256), 0, st, workspace, ld_parts(H), parts, dweight,
-                       dbias, accumulate, H);
-    STDIFF_LAUNCH_STATUS();
-    return STDIFF_OK;
 }

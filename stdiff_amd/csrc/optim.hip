@@ -21,98 +21,105 @@ typedef f32x4 f32x4_u __attribute__((aligned(4)));
 typedef u32x2 u32x2_u __attribute__((aligned(2)));
 typedef unsigned u32_u __attribute__((aligned(1)));
 
-constexpr int TENSORS = 48;               // per launch: the table travels in the kernel's arguments (4 KB at most)
 constexpr int BLOCK = 256;                // elements that share a scale: one wave, four per lane
-constexpr int CHUNK = 4096;               // elements of one turn of a workgroup: four blocks per wave
 constexpr int SCALARS = 4;                // floats at the workspace's head, the partial sums of squares follow
 
-struct tensor_arg {
-    void* p;
-    const void* g;
-    void* m;
-    void* v;
-    float* ms;
-    float* vs;
+// A launch's table of tensors travels in its arguments (4 KB at most): nothing is copied to the device, nothing has to live
+// on, and a captured launch holds its own table.
+struct tensor32 {
+    void* p; const void* g; float* m; float* v;
     long long n;
     float wd;
     int kinds;                            // bit 0: p in 16 bits, bit 1: g in 16 bits
 };
-struct batch_arg {
-    tensor_arg t[TENSORS];
-    int first[TENSORS + 1];               // first chunk of each tensor, then their number
+struct tensor8 {
+    void* p; const void* g; unsigned char* m; unsigned char* v;
+    long long n;
+    float wd;
+    int kinds;
+    float* ms; float* vs;
+};
+struct gradient {
+    const void* g;
+    long long n;                          // elements; their complement where they have 16 bits
+};
+template <typename T, int N> struct batch {
+    T t[N];
+    int first[N + 1];                     // first chunk of each tensor, then their number
     int count;
 };
+typedef batch<tensor32, 76> batch32;
+typedef batch<tensor8, 58> batch8;
+constexpr int GRADIENTS = 190;
+typedef batch<gradient, GRADIENTS> batchg;
 
-__device__ __forceinline__ void ld4e(const float* p, int k, float* o) {
-    if (k >= 4) {
-        const f32x4 v = *(const f32x4_u*)p;
+template <bool WHOLE> __device__ __forceinline__ f32x4 ld4e(const float* p, int k) {
+    if (WHOLE || k >= 4) return __builtin_nontemporal_load((const f32x4_u*)p);
+    f32x4 o;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = j < k ? p[j] : 0.f;
-    }
+    for (int j = 0; j < 4; ++j) o[j] = j < k ? p[j] : 0.f;
+    return o;
 }
-__device__ __forceinline__ void ld4e(const bf16_t* p, int k, float* o) {
-    if (k >= 4) {
-        const u32x2 v = *(const u32x2_u*)p;
-        o[0] = bf_lo(v[0]); o[1] = bf_hi(v[0]); o[2] = bf_lo(v[1]); o[3] = bf_hi(v[1]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = j < k ? bf2f(p[j]) : 0.f;
+template <bool WHOLE> __device__ __forceinline__ f32x4 ld4e(const bf16_t* p, int k) {
+    if (WHOLE || k >= 4) {
+        const u32x2 v = __builtin_nontemporal_load((const u32x2_u*)p);
+        return f32x4{bf_lo(v[0]), bf_hi(v[0]), bf_lo(v[1]), bf_hi(v[1])};
     }
+    f32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = j < k ? bf2f(p[j]) : 0.f;
+    return o;
 }
-__device__ __forceinline__ void st4e(float* p, int k, const float* o) {
-    if (k >= 4) {
-        *(f32x4_u*)p = f32x4{o[0], o[1], o[2], o[3]};
+template <bool WHOLE> __device__ __forceinline__ void st4e(float* p, int k, f32x4 o) {
+    if (WHOLE || k >= 4) {
+        __builtin_nontemporal_store(o, (f32x4_u*)p);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j < k) p[j] = o[j];
     }
 }
-__device__ __forceinline__ void st4e(bf16_t* p, int k, const float* o) {
-    if (k >= 4) {
-        *(u32x2_u*)p = u32x2{pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+template <bool WHOLE> __device__ __forceinline__ void st4e(bf16_t* p, int k, f32x4 o) {
+    if (WHOLE || k >= 4) {
+        const u32x2 v = {pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+        __builtin_nontemporal_store(v, (u32x2_u*)p);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j < k) p[j] = f2bf(o[j]);
     }
 }
-__device__ __forceinline__ unsigned ld_codes(const unsigned char* p, int k) {
-    if (k >= 4) return *(const u32_u*)p;
+template <bool WHOLE> __device__ __forceinline__ unsigned ld_codes(const unsigned char* p, int k) {
+    if (WHOLE || k >= 4) return __builtin_nontemporal_load((const u32_u*)p);
     unsigned v = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (j < k) v |= (unsigned)p[j] << (8 * j);
     return v;
 }
-__device__ __forceinline__ void st_codes(unsigned char* p, int k, unsigned v) {
-    if (k >= 4) {
-        *(u32_u*)p = v;
+template <bool WHOLE> __device__ __forceinline__ void st_codes(unsigned char* p, int k, unsigned v) {
+    if (WHOLE || k >= 4) {
+        __builtin_nontemporal_store(v, (u32_u*)p);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j < k) p[j] = (unsigned char)(v >> (8 * j));
     }
 }
-__device__ __forceinline__ void from_e4m3(unsigned v, float scale, float* o) {
+__device__ __forceinline__ f32x4 from_e4m3(unsigned v, float scale) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)v, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)v, true);
-    o[0] = lo[0] * scale; o[1] = lo[1] * scale; o[2] = hi[0] * scale; o[3] = hi[1] * scale;
+    return f32x4{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
 }
-__device__ __forceinline__ unsigned to_e4m3(const float* v) {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+__device__ __forceinline__ unsigned to_e4m3(f32x4 v) {
+    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r, true);
 }
 // largest magnitude over a wave, by the bits: NaN is above infinity, infinity above every number
-__device__ __forceinline__ float wave_amax(const float* v) {
+__device__ __forceinline__ float wave_amax(f32x4 v) {
     unsigned a = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a = max(a, __builtin_bit_cast(unsigned, v[j]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, o, 64));
-    return __builtin_bit_cast(float, a);
+    for (int j = 0; j < 4; ++j) a = max(a, __builtin_bit_cast(unsigned, (float)v[j]) & 0x7fffffffu);
+    return __builtin_bit_cast(float, wave_umax_dpp(a));
 }
 // scale of a block, and what its elements are multiplied by before they become codes.  Below 1e-30 the factor
 // 448 / largest would leave the range of fp32: such blocks are scaled as if their largest were 1e-30.
@@ -122,8 +129,8 @@ __device__ __forceinline__ float block_scale(float top, float* factor) {
     return top / 448.0f;
 }
 
-__device__ __forceinline__ int tensor_of(const batch_arg& b, int chunk, int t) {
-    while (chunk >= b.first[t + 1]) ++t;
+template <typename B> __device__ __forceinline__ int tensor_of(const B& b, int chunk, int t) {
+    while (chunk < b.first[t]) --t;
     return t;
 }
 
@@ -141,28 +148,42 @@ __global__ void adamw_prepare_kernel(int32_t* step_dev, float* scalars, float* n
 }
 
 // sum of squares of the gradients: one partial sum per workgroup, joined by every workgroup of the update in one order
-__global__ __launch_bounds__(256) void adamw_norm_kernel(batch_arg b, float* parts, int32_t* step_dev, float* scalars, double lr,
+constexpr int NORM_CHUNK = 8192;
+__global__ __launch_bounds__(256) void adamw_norm_kernel(batchg b, float* parts, int32_t* step_dev, float* scalars, double lr,
                                                          double b1, double b2) {
     if (step_dev && blockIdx.x == 0 && threadIdx.x == 0) next_step(step_dev, scalars, lr, b1, b2);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    int t = 0;
-    for (int chunk = blockIdx.x; chunk < b.first[b.count]; chunk += gridDim.x) {
+    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    int t = b.count - 1;
+    for (int chunk = b.first[b.count] - 1 - (int)blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
         t = tensor_of(b, chunk, t);
-        const long long n = b.t[t].n, at = (long long)(chunk - b.first[t]) * CHUNK + threadIdx.x * 4;
-        const bool half = b.t[t].kinds & 2;
+        const bool half = b.t[t].n < 0;
+        const long long n = half ? ~b.t[t].n : b.t[t].n, start = (long long)(chunk - b.first[t]) * NORM_CHUNK;
+        const float* g32 = (const float*)b.t[t].g + start + threadIdx.x * 4;
+        const bf16_t* g16 = (const bf16_t*)b.t[t].g + start + threadIdx.x * 4;
+        f32x4 g[NORM_CHUNK / 1024];
+        if (start + NORM_CHUNK <= n) {
+            if (half) {
 #pragma unroll
-        for (int u = 0; u < CHUNK / 1024; ++u) {
-            const long long i = at + u * 1024;
-            if (i >= n) break;
-            const int k = (int)std::min<long long>(4, n - i);
-            float g[4];
-            if (half) ld4e((const bf16_t*)b.t[t].g + i, k, g);
-            else ld4e((const float*)b.t[t].g + i, k, g);
+                for (int u = 0; u < NORM_CHUNK / 1024; ++u) {
+                    const u32x2 v = *(const u32x2_u*)(g16 + u * 1024);
+                    g[u] = f32x4{bf_lo(v[0]), bf_hi(v[0]), bf_lo(v[1]), bf_hi(v[1])};
+                }
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] += g[j] * g[j];
+                for (int u = 0; u < NORM_CHUNK / 1024; ++u) g[u] = *(const f32x4_u*)(g32 + u * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < NORM_CHUNK / 1024; ++u) {
+                const int k = (int)std::max<long long>(0, std::min<long long>(4, n - start - threadIdx.x * 4 - u * 1024));
+                g[u] = half ? ld4e<false>(g16 + u * 1024, k) : ld4e<false>(g32 + u * 1024, k);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < NORM_CHUNK / 1024; ++u) acc[u & 1] += g[u] * g[u];
     }
-    const float s = wave_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
+    acc[0] += acc[1];
+    const float s = wave_sum_dpp((acc[0][0] + acc[0][1]) + (acc[0][2] + acc[0][3]));
     __shared__ float part[4];
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -177,103 +198,171 @@ struct update_arg {
     float max_norm, grad_scale, lr, b1, b2, omb1, omb2, eps;
 };
 
-template <int BITS>
-__global__ __launch_bounds__(256) void adamw_update_kernel(batch_arg b, update_arg a) {
-    float coef = a.grad_scale;
-    if (a.parts) {
-        __shared__ float part[4];
-        float s = 0.f;
-        for (int i = threadIdx.x; i < a.n_parts; i += 256) s += a.parts[i];
-        s = wave_sum(s);
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-        __syncthreads();
-        const float norm = sqrtf((part[0] + part[1]) + (part[2] + part[3])) * a.grad_scale;
-        if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
-        if (a.max_norm > 0.f) {
-            const float r = a.max_norm / (norm + 1e-6f);
-            coef = (r > 1.f ? 1.f : r) * a.grad_scale;              // a NaN stays one
+// what every gradient is multiplied by; the first workgroup also writes the norm
+__device__ float gradient_factor(const update_arg& a, float* part) {
+    if (!a.parts) return a.grad_scale;
+    float s = 0.f;
+    for (int i = threadIdx.x; i < a.n_parts; i += 256) s += a.parts[i];
+    s = wave_sum_dpp(s);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    const float norm = sqrtf((part[0] + part[1]) + (part[2] + part[3])) * a.grad_scale;
+    if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
+    if (!(a.max_norm > 0.f)) return a.grad_scale;
+    const float r = a.max_norm / (norm + 1e-6f);
+    return (r > 1.f ? 1.f : r) * a.grad_scale;                      // a NaN stays one
+}
+
+struct factors {
+    float coef, step, inv_second;
+    bool known;
+};
+
+// One turn of a workgroup: U * 1024 elements of one tensor, a block of 256 per wave and U.  All loads are issued before anything
+// is computed, on the first turn also before the partial sums of the norm are joined.
+template <int BITS, int U, bool WHOLE, typename TP, typename TG, typename T>
+__device__ __forceinline__ void turn(const T& q, long long start, const update_arg& a, factors& f, float* part) {
+    const long long at = start + threadIdx.x * 4;
+    const float keep = 1.0f - a.lr * q.wd;
+    int k[U];
+    f32x4 p[U], g[U], m[U], v[U];
+    unsigned mc[U], vc[U];
+    float ms[U], vs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long i = at + u * 1024;
+        k[u] = WHOLE ? 4 : (int)std::max<long long>(0, std::min<long long>(4, q.n - i));
+        p[u] = ld4e<WHOLE>((const TP*)q.p + i, k[u]);
+        g[u] = ld4e<WHOLE>((const TG*)q.g + i, k[u]);
+        if constexpr (BITS == 8) {
+            mc[u] = ld_codes<WHOLE>(q.m + i, k[u]);
+            vc[u] = ld_codes<WHOLE>(q.v + i, k[u]);
+            const bool in = WHOLE || i - (threadIdx.x & 63) * 4 < q.n;
+            ms[u] = in ? q.ms[i / BLOCK] : 0.f;
+            vs[u] = in ? q.vs[i / BLOCK] : 0.f;
+        } else {
+            m[u] = ld4e<WHOLE>(q.m + i, k[u]);
+            v[u] = ld4e<WHOLE>(q.v + i, k[u]);
         }
     }
-    const float step = a.scalars[0], second = a.scalars[1];
-    int t = 0;
-    for (int chunk = blockIdx.x; chunk < b.first[b.count]; chunk += gridDim.x) {
-        t = tensor_of(b, chunk, t);
-        const tensor_arg& q = b.t[t];
-        const long long n = q.n, at = (long long)(chunk - b.first[t]) * CHUNK + threadIdx.x * 4;
-        const float keep = 1.0f - a.lr * q.wd;
+    if (!f.known) {
+        f.known = true;
+        f.step = a.scalars[0];
+        f.inv_second = 1.0f / a.scalars[1];
+        f.coef = gradient_factor(a, part);
+    }
 #pragma unroll
-        for (int u = 0; u < CHUNK / 1024; ++u) {
-            const long long i = at + u * 1024;
-            if (i - (threadIdx.x & 63) * 4 >= n) break;             // the whole wave is behind the end
-            const int k = (int)std::max<long long>(0, std::min<long long>(4, n - i));
-            float p[4], g[4], m[4], v[4], r[4];
-            if (q.kinds & 1) ld4e((const bf16_t*)q.p + i, k, p);
-            else ld4e((const float*)q.p + i, k, p);
-            if (q.kinds & 2) ld4e((const bf16_t*)q.g + i, k, g);
-            else ld4e((const float*)q.g + i, k, g);
-            if constexpr (BITS == 8) {
-                from_e4m3(ld_codes((const unsigned char*)q.m + i, k), q.ms[i / BLOCK], m);
-                from_e4m3(ld_codes((const unsigned char*)q.v + i, k), q.vs[i / BLOCK], v);
+    for (int u = 0; u < U; ++u) {
+        const long long i = at + u * 1024;
+        f32x4 r;
+        if constexpr (BITS == 8) {
+            m[u] = from_e4m3(mc[u], ms[u]);
+            v[u] = from_e4m3(vc[u], vs[u]);
+            v[u] = v[u] * v[u];
+        }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = v[j] * v[j];
-            } else {
-                ld4e((const float*)q.m + i, k, m);
-                ld4e((const float*)q.v + i, k, v);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float gr = g[j] * coef;
-                m[j] = m[j] * a.b1 + gr * a.omb1;
-                v[j] = v[j] * a.b2 + gr * gr * a.omb2;
-                r[j] = sqrtf(v[j]);
-                p[j] = p[j] * keep - step * (m[j] / (r[j] / second + a.eps));
-            }
-            if (q.kinds & 1) st4e((bf16_t*)q.p + i, k, p);
-            else st4e((float*)q.p + i, k, p);
-            if constexpr (BITS == 8) {
+        for (int j = 0; j < 4; ++j) {
+            const float gr = g[u][j] * f.coef;
+            m[u][j] = m[u][j] * a.b1 + gr * a.omb1;
+            v[u][j] = v[u][j] * a.b2 + gr * gr * a.omb2;
+            r[j] = sqrtf(v[u][j]);
+            // the quotient by the hardware's reciprocal (off by one unit in the last place): a few 2^-24 of a step that
+            // is itself a small part of p; two full divisions cost a third of this kernel's instructions
+            p[u][j] = p[u][j] * keep - f.step * (m[u][j] * __builtin_amdgcn_rcpf(r[j] * f.inv_second + a.eps));
+        }
+        st4e<WHOLE>((TP*)q.p + i, k[u], p[u]);
+        if constexpr (BITS == 8) {
+            if constexpr (!WHOLE) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (j >= k) m[j] = r[j] = 0.f;                  // behind the end: no part of the block
-                float fm, fr;
-                const float sm = block_scale(wave_amax(m), &fm), sr = block_scale(wave_amax(r), &fr);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    m[j] *= fm;
-                    const float z = r[j] * fr;
-                    r[j] = r[j] > 0.f && z < 0x1p-9f ? 0x1p-9f : z;
-                }
-                st_codes((unsigned char*)q.m + i, k, to_e4m3(m));
-                st_codes((unsigned char*)q.v + i, k, to_e4m3(r));
-                if ((threadIdx.x & 63) == 0) {
-                    q.ms[i / BLOCK] = sm;
-                    q.vs[i / BLOCK] = sr;
-                }
-            } else {
-                st4e((float*)q.m + i, k, m);
-                st4e((float*)q.v + i, k, v);
+                    if (j >= k[u]) m[u][j] = r[j] = 0.f;            // behind the end: no part of the block
             }
+            float fm, fr;
+            const float sm = block_scale(wave_amax(m[u]), &fm), sr = block_scale(wave_amax(r), &fr);
+            f32x4 z;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                z[j] = r[j] * fr;
+                if (r[j] > 0.f && z[j] < 0x1p-9f) z[j] = 0x1p-9f;
+            }
+            st_codes<WHOLE>(q.m + i, k[u], to_e4m3(m[u] * fm));
+            st_codes<WHOLE>(q.v + i, k[u], to_e4m3(z));
+            if ((threadIdx.x & 63) == 0 && k[u] > 0) {
+                q.ms[i / BLOCK] = sm;
+                q.vs[i / BLOCK] = sr;
+            }
+        } else {
+            st4e<WHOLE>(q.m + i, k[u], m[u]);
+            st4e<WHOLE>(q.v + i, k[u], v[u]);
         }
     }
 }
 
-inline bool at_bytes(const void* p, int size) { return ((uintptr_t)p & (size - 1)) == 0; }
-inline int max_blocks() { return 2 * cu_count(); }
+// The norm kernel walks the tensors from the last element to the first, the update from the first: what the norm kernel read
+// last is still in the memory-side cache when the update begins with it.
+template <int BITS, int U, typename B>
+__global__ __launch_bounds__(256) void adamw_update_kernel(B b, update_arg a) {
+    __shared__ float part[4];
+    factors f;
+    f.known = false;
+    int t = 0;
+    for (int chunk = blockIdx.x; chunk < b.first[b.count]; chunk += gridDim.x) {
+        while (chunk >= b.first[t + 1]) ++t;
+        const auto& q = b.t[t];
+        const long long start = (long long)(chunk - b.first[t]) * (U * 1024);
+#define TURN(TP, TG)                                                                                      \
+    do {                                                                                                  \
+        if (start + U * 1024 <= q.n) turn<BITS, U, true, TP, TG>(q, start, a, f, part);                   \
+        else turn<BITS, U, false, TP, TG>(q, start, a, f, part);                                          \
+    } while (0)
+        switch (q.kinds) {
+            case 0: TURN(float, float); break;
+            case 1: TURN(bf16_t, float); break;
+            case 2: TURN(float, bf16_t); break;
+            default: TURN(bf16_t, bf16_t); break;
+        }
+#undef TURN
+    }
+}
 
-// the table of tensors [from, from + TENSORS), without the empty ones
-int fill_batch(const stdiff_adamw_multi_args* a, int from, batch_arg* b) {
+inline bool at_bytes(const void* p, int size) { return ((uintptr_t)p & (size - 1)) == 0; }
+inline int max_blocks() { return 4 * cu_count(); }
+
+void set_tensor(tensor32& t, const stdiff_adamw_tensor& s) {
+    t.p = s.param; t.g = s.grad; t.m = (float*)s.exp_avg; t.v = (float*)s.exp_avg_sq; t.n = s.n; t.wd = s.weight_decay;
+    t.kinds = (s.param_dtype == STDIFF_BF16 ? 1 : 0) | (s.grad_dtype == STDIFF_BF16 ? 2 : 0);
+}
+void set_tensor(tensor8& t, const stdiff_adamw_tensor& s) {
+    t.p = s.param; t.g = s.grad; t.m = (unsigned char*)s.exp_avg; t.v = (unsigned char*)s.exp_avg_sq; t.n = s.n; t.wd = s.weight_decay;
+    t.ms = s.exp_avg_scale; t.vs = s.exp_avg_sq_scale;
+    t.kinds = (s.param_dtype == STDIFF_BF16 ? 1 : 0) | (s.grad_dtype == STDIFF_BF16 ? 2 : 0);
+}
+void set_tensor(gradient& t, const stdiff_adamw_tensor& s) {
+    t.g = s.grad;
+    t.n = s.grad_dtype == STDIFF_BF16 ? ~s.n : s.n;
+}
+
+// Fills a table with the tensors from *at on, without the empty ones, and moves *at behind the last one that found room.
+template <typename T, int N> int fill(const stdiff_adamw_multi_args* a, int* at, int chunk, batch<T, N>* b) {
     b->count = 0;
     b->first[0] = 0;
-    long long chunks = 0;
-    for (int i = from; i < a->n_tensors && i < from + TENSORS; ++i) {
-        const stdiff_adamw_tensor& s = a->tensors[i];
+    for (; *at < a->n_tensors && b->count < N; ++*at) {
+        const stdiff_adamw_tensor& s = a->tensors[*at];
         if (s.n == 0) continue;
-        tensor_arg& t = b->t[b->count++];
-        t.p = s.param; t.g = s.grad; t.m = s.exp_avg; t.v = s.exp_avg_sq; t.ms = s.exp_avg_scale; t.vs = s.exp_avg_sq_scale;
-        t.n = s.n; t.wd = s.weight_decay;
-        t.kinds = (s.param_dtype == STDIFF_BF16 ? 1 : 0) | (s.grad_dtype == STDIFF_BF16 ? 2 : 0);
-        chunks += (s.n + CHUNK - 1) / CHUNK;
-        if (chunks > (1ll << 30)) return STDIFF_ERR_SHAPE;
-        b->first[b->count] = (int)chunks;
+        set_tensor(b->t[b->count], s);
+        b->first[b->count + 1] = b->first[b->count] + (int)((s.n + chunk - 1) / chunk);
+        ++b->count;
+    }
+    return b->first[b->count];
+}
+
+template <int BITS, int U, typename B> int update(const stdiff_adamw_multi_args* a, const update_arg& u, hipStream_t st) {
+    B b;
+    for (int at = 0; at < a->n_tensors;) {
+        const int chunks = fill(a, &at, U * 1024, &b);
+        if (!chunks) continue;
+        hipLaunchKernelGGL((adamw_update_kernel<BITS, U, B>), dim3(std::min(chunks, max_blocks())), dim3(256), 0, st, b, u);
+        STDIFF_LAUNCH_STATUS();
     }
     return STDIFF_OK;
 }
@@ -282,6 +371,7 @@ int check_multi(const stdiff_adamw_multi_args* a) {
     STDIFF_CHECK_ARG(a && a->n_tensors >= 0 && (a->tensors || a->n_tensors == 0) && (a->state_bits == 8 || a->state_bits == 32));
     STDIFF_CHECK_ARG(a->step_dev && a->workspace && a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0 &&
                      a->eps >= 0.0 && a->lr >= 0.0 && a->max_norm == a->max_norm);
+    long long chunks = 0;
     for (int i = 0; i < a->n_tensors; ++i) {
         const stdiff_adamw_tensor& s = a->tensors[i];
         STDIFF_CHECK_ARG(s.n >= 0 && (s.param_dtype == STDIFF_F32 || s.param_dtype == STDIFF_BF16) &&
@@ -293,6 +383,8 @@ int check_multi(const stdiff_adamw_multi_args* a) {
             (a->state_bits == 32 && (!at_bytes(s.exp_avg, 4) || !at_bytes(s.exp_avg_sq, 4))) ||
             (a->state_bits == 8 && (!at_bytes(s.exp_avg_scale, 4) || !at_bytes(s.exp_avg_sq_scale, 4))))
             return STDIFF_ERR_ALIGN;
+        chunks += s.n / 1024 + 1;
+        if (s.n > (1ll << 40) || chunks > (1ll << 30)) return STDIFF_ERR_SHAPE;      // chunks are counted in 32 bits
     }
     if (!at_bytes(a->step_dev, 4) || !at_bytes(a->workspace, 4) || !at_bytes(a->norm, 4)) return STDIFF_ERR_ALIGN;
     if (a->workspace_bytes < stdiff_adamw_multi_workspace(a->n_tensors)) return STDIFF_ERR_WORKSPACE;
@@ -303,16 +395,13 @@ int check_multi(const stdiff_adamw_multi_args* a) {
 
 extern "C" long long stdiff_adamw_multi_workspace(int n_tensors) {
     if (n_tensors < 0) return STDIFF_ERR_ARG;
-    return (SCALARS + (long long)cdiv(n_tensors, TENSORS) * max_blocks()) * 4;
+    return (SCALARS + (long long)cdiv(n_tensors, GRADIENTS) * max_blocks()) * 4;
 }
 
 extern "C" int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream) {
     int rc = check_multi(a);
     if (rc != STDIFF_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
-    batch_arg b;
-    for (int from = 0; from < a->n_tensors; from += TENSORS)       // before the first launch: nothing is half done
-        if ((rc = fill_batch(a, from, &b)) != STDIFF_OK) return rc;
     update_arg u = {};
     u.scalars = a->workspace;
     u.norm = a->norm;
@@ -323,10 +412,11 @@ extern "C" int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream
     bool counted = false;
     if (a->max_norm > 0.0 || a->norm) {
         float* parts = a->workspace + SCALARS;
-        for (int from = 0; from < a->n_tensors; from += TENSORS) {
-            fill_batch(a, from, &b);
-            if (b.first[b.count] == 0) continue;
-            const int grid = std::min(b.first[b.count], max_blocks());
+        batchg b;
+        for (int at = 0; at < a->n_tensors;) {
+            const int chunks = fill(a, &at, NORM_CHUNK, &b);
+            if (!chunks) continue;
+            const int grid = std::min(chunks, max_blocks());
             hipLaunchKernelGGL(adamw_norm_kernel, dim3(grid), dim3(256), 0, st, b, parts + u.n_parts, counted ? nullptr : a->step_dev,
                                a->workspace, a->lr, a->beta1, a->beta2);
             STDIFF_LAUNCH_STATUS();
@@ -336,19 +426,12 @@ extern "C" int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream
         u.parts = parts;
     }
     if (!counted) {
-        hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(64), 0, st, a->step_dev, a->workspace, a->norm, a->lr,
-                           a->beta1, a->beta2);
+        hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(64), 0, st, a->step_dev, a->workspace, a->norm, a->lr, a->beta1, a->beta2);
         STDIFF_LAUNCH_STATUS();
     }
-    for (int from = 0; from < a->n_tensors; from += TENSORS) {
-        fill_batch(a, from, &b);
-        if (b.first[b.count] == 0) continue;
-        const int grid = std::min(b.first[b.count], max_blocks());
-        if (a->state_bits == 8)
-            hipLaunchKernelGGL(adamw_update_kernel<8>, dim3(grid), dim3(256), 0, st, b, u);
-        else
-            hipLaunchKernelGGL(adamw_update_kernel<32>, dim3(grid), dim3(256), 0, st, b, u);
-        STDIFF_LAUNCH_STATUS();
-    }
-    return STDIFF_OK;
+    long long total = 0;
+    for (int i = 0; i < a->n_tensors; ++i) total += a->tensors[i].n;
+    const bool few = total < 4096ll * 2 * cu_count();               // small turns spread the work over all CUs
+    if (a->state_bits == 8) return few ? update<8, 1, batch8>(a, u, st) : update<8, 4, batch8>(a, u, st);
+    return few ? update<32, 1, batch32>(a, u, st) : update<32, 4, batch32>(a, u, st);
 }

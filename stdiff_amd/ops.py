@@ -2,6 +2,7 @@
 Tensors must live on the GPU; outputs are allocated with torch when not supplied."""
 import ctypes as C
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -381,38 +382,51 @@ def clip_adamw(p, g, m, v, sumsq, step_dev, scal, lr, max_norm=1.0, grad_scale=1
 
 # ---------------------------------------------------------------- norm, optimizer and 8-bit product beside the DiT
 def _one_device(first, *rest):
-    """The device all of these tensors are on (None entries are skipped)."""
-    if not first.is_cuda:
-        require_gpu(first)
-    dev = first.device
+    """Index of the device that all of these tensors are on (None entries are skipped)."""
+    dev = first.get_device()
     for t in rest:
-        if t is not None and t.device != dev:
-            require_gpu(t)
-            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+        if t is not None and t.get_device() != dev:
+            require_gpu(first, t)
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+    if dev < 0:
+        require_gpu(first)
     return dev
 
 
-def _enqueue(dev, call):
-    """check(call(stream)) with the stream that is current on `dev`, `dev` being the current device meanwhile."""
-    if dev.index == torch.cuda.current_device():
-        check(call(torch.cuda.current_stream(dev).cuda_stream))
+def _enqueue(dev, fn, *args):
+    """check(fn(*args, stream)) with the stream that is current on device `dev`, `dev` being the current device meanwhile."""
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            check(call(torch.cuda.current_stream(dev).cuda_stream))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc)
+
+
+def _lib_of(*dtypes):
+    """lib_for by dtype."""
+    if torch.float16 in dtypes:
+        if torch.bfloat16 in dtypes:
+            raise TypeError("float16 and bfloat16 tensors in one stdiff_hip call")
+        return lib(True)
+    return lib()
 
 
 def _read_ld(t, name, shape=None):
     """Leading dimension of a matrix that is only read: rows may overlap or be one row broadcast."""
-    if t.dim() != 2 or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name}: a matrix{'' if shape is None else f' of {tuple(shape)}'} is needed, got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    size = t.shape
+    if len(size) != 2 or (shape is not None and size != shape):
+        raise ValueError(f"{name}: a matrix{'' if shape is None else f' of {tuple(shape)}'} is needed, got {tuple(size)}")
+    ld, one = t.stride()
+    if one != 1 and size[1] > 1:
         raise ValueError(f"{name}: the elements of a row have to be neighbours, got strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return ld if size[0] > 1 else size[1]
 
 
 def _write_ld(t, name, shape):
     ld = _read_ld(t, name, shape)
-    if t.shape[0] > 1 and ld < t.shape[1]:
+    if ld < t.shape[1]:
         raise ValueError(f"{name}: rows of an output may not overlap, got strides {t.stride()}")
     return ld
 
@@ -421,7 +435,7 @@ def _vector(t, name, n, *dtypes):
     """None, or the address of a contiguous vector of n elements of one of these types."""
     if t is None:
         return None
-    if t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes or (n > 1 and t.stride(0) != 1):
+    if t.dim() != 1 or t.numel() != n or t.dtype not in dtypes or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous vector of {n} elements of {' / '.join(str(d) for d in dtypes)} is needed, "
                          f"got {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
@@ -431,11 +445,20 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _affine(weight, bias, H):
-    """(address, address, dtype code) of a norm's weight and bias, which share one dtype."""
+    """(address, address, dtype) of a norm's weight and bias, which share one dtype."""
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: one dtype is needed")
     one = weight if weight is not None else bias
-    return _vector(weight, "weight", H, *_FLOATS), _vector(bias, "bias", H, *_FLOATS), F32 if one is None else dt_of(one)
+    return _vector(weight, "weight", H, *_FLOATS), _vector(bias, "bias", H, *_FLOATS), torch.float32 if one is None else one.dtype
+
+
+def _code(dtype):
+    """The C ABI's code of a torch dtype (dt_of by dtype)."""
+    if dtype is torch.float32:
+        return F32
+    if dtype is torch.bfloat16 or dtype is torch.float16:
+        return L.BF16
+    raise TypeError(f"unsupported dtype {dtype}")
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, mean=None, rstd=None):
@@ -446,12 +469,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, me
     ldx = _read_ld(x, "x")
     R, H = x.shape
     if out is None:
-        out = torch.empty((R, H), device=dev, dtype=out_dtype or x.dtype)
-    ldy = _write_ld(out, "out", x.shape)
+        out, ldy = x.new_empty((R, H), dtype=out_dtype), H
+    else:
+        ldy = _write_ld(out, "out", x.shape)
     w, b, wdt = _affine(weight, bias, H)
     mp, rp = _vector(mean, "mean", R, torch.float32), _vector(rstd, "rstd", R, torch.float32)
-    fn = lib_for(x, out, weight, bias).stdiff_layer_norm
-    _enqueue(dev, lambda st: fn(x.data_ptr(), ldx, dt_of(x), w, b, wdt, eps, out.data_ptr(), ldy, dt_of(out), mp, rp, R, H, st))
+    xdt, ydt = x.dtype, out.dtype
+    _enqueue(dev, _lib_of(xdt, ydt, wdt).stdiff_layer_norm, x.data_ptr(), ldx, _code(xdt), w, b, _code(wdt), eps, out.data_ptr(), ldy,
+             _code(ydt), mp, rp, R, H)
     return out
 
 
@@ -460,8 +485,8 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=
     dy or x).  dweight / dbias are fp32 [H]: with a weight both are allocated unless given, without one those that are
     given are formed (else None); accumulate=True adds to what the given ones hold.  They are sums over the rows in a
     fixed order: the same bits every run.
-    workspace (fp32, at least layer_norm_bwd_workspace(R, H) floats; allocated unless given): give one of its own to a
-    call that is captured into an ops.Graph."""
+    workspace (fp32, at least layer_norm_bwd_workspace(R, H) floats, which is none for few rows; allocated unless given):
+    give one of its own to a call that is captured into an ops.Graph."""
     dev = _one_device(x, dy, mean, rstd, weight, dx, dweight, dbias, workspace)
     ldx = _read_ld(x, "x")
     R, H = x.shape
@@ -469,27 +494,30 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=
     if accumulate and (dweight is None and dbias is None):
         raise ValueError("accumulate: there is no dweight or dbias to add to")
     if dx is None:
-        dx = torch.empty((R, H), device=dev, dtype=x.dtype)
+        dx, lddx = x.new_empty((R, H)), H
     elif dx.dtype != x.dtype:
         raise TypeError(f"dx is {dx.dtype}, x {x.dtype}")
-    lddx = _write_ld(dx, "dx", x.shape)
+    else:
+        lddx = _write_ld(dx, "dx", x.shape)
     if weight is not None and not accumulate:
         if dweight is None:
-            dweight = torch.empty((H,), device=dev, dtype=torch.float32)
+            dweight = x.new_empty((H,), dtype=torch.float32)
         if dbias is None:
-            dbias = torch.empty((H,), device=dev, dtype=torch.float32)
+            dbias = x.new_empty((H,), dtype=torch.float32)
     w, _, wdt = _affine(weight, None, H)
     if mean is None or rstd is None:
         raise ValueError("mean and rstd of the forward are needed")
     mp, rp = _vector(mean, "mean", R, torch.float32), _vector(rstd, "rstd", R, torch.float32)
     dw, db = _vector(dweight, "dweight", H, torch.float32), _vector(dbias, "dbias", H, torch.float32)
-    lb = lib_for(x, dy, weight)
-    if workspace is None and (dw or db):
-        workspace = torch.empty((layer_norm_bwd_workspace(R, H),), device=dev, dtype=torch.float32)
+    xdt, ddt = x.dtype, dy.dtype
+    lb = _lib_of(xdt, ddt, wdt)
+    if workspace is None and (dweight is not None or dbias is not None):
+        need = lb.stdiff_layer_norm_bwd_workspace(R, H)
+        if need > 0:
+            workspace = x.new_empty((need // 4,), dtype=torch.float32)
     ws, nb = _workspace(workspace)
-    _enqueue(dev, lambda st: lb.stdiff_layer_norm_bwd(
-        dy.data_ptr(), lddy, dt_of(dy), x.data_ptr(), ldx, dt_of(x), mp, rp, w, wdt, dx.data_ptr(), lddx, dw, db,
-        int(accumulate), ws, nb, R, H, st))
+    _enqueue(dev, lb.stdiff_layer_norm_bwd, dy.data_ptr(), lddy, _code(ddt), x.data_ptr(), ldx, _code(xdt), mp, rp, w, _code(wdt),
+             dx.data_ptr(), lddx, dw, db, int(accumulate), ws, nb, R, H)
     return dx, dweight, dbias
 
 
@@ -523,28 +551,23 @@ class AdamWTensors:
         self.state_bits = 8 if n and exp_avg[0].dtype == torch.float8_e4m3fn else 32
         kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
         self.table = (L.AdamWTensor * max(n, 1))()
-        self.device = params[0].device if n else None
+        self.rows = np.frombuffer(self.table, dtype=np.dtype(L.AdamWTensor))[:n]
+        self.device = _one_device(*[t for k in self.tensors for t in k]) if n else None
         self.sizes = [p.numel() for p in params]
-        for i, (p, m, v, ms, vs) in enumerate(zip(*self.tensors)):
-            _one_device(params[0], p, m, v, ms, vs)
+        for i, (p, m, v, ms, vs, size) in enumerate(zip(*self.tensors, self.sizes)):
             if m.dtype != kind or v.dtype != kind:
                 raise TypeError(f"tensor {i}: states are {m.dtype} and {v.dtype}, {kind} is needed like in the first")
-            if m.numel() != p.numel() or v.numel() != p.numel():
-                raise ValueError(f"tensor {i}: states of {m.numel()} and {v.numel()} elements for {p.numel()} parameters")
-            for what, t in (("param", p), ("exp_avg", m), ("exp_avg_sq", v)):
-                if not t.is_contiguous():
-                    raise ValueError(f"tensor {i}: {what} is not contiguous")
-            q = self.table[i]
-            if self.state_bits == 8:
-                blocks = round_up(p.numel(), 256) // 256
-                if ms is None or vs is None:
-                    raise ValueError("8-bit states need exp_avg_scale and exp_avg_sq_scale")
-                q.exp_avg_scale = _vector(ms, f"exp_avg_scale[{i}]", blocks, torch.float32)
-                q.exp_avg_sq_scale = _vector(vs, f"exp_avg_sq_scale[{i}]", blocks, torch.float32)
-            elif ms is not None or vs is not None:
+            if m.numel() != size or v.numel() != size:
+                raise ValueError(f"tensor {i}: states of {m.numel()} and {v.numel()} elements for {size} parameters")
+            if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+                raise ValueError(f"tensor {i}: the parameter or a state of it is not contiguous")
+            if self.state_bits == 32 and (ms is not None or vs is not None):
                 raise ValueError("32-bit states have no scales")
-            q.param, q.exp_avg, q.exp_avg_sq, q.n = p.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel()
-            q.param_dtype, q.weight_decay = dt_of(p), decay[i]
+            if self.state_bits == 8 and (ms is None or vs is None):
+                raise ValueError("8-bit states need exp_avg_scale and exp_avg_sq_scale")
+            blocks = -(-size // 256)
+            self.table[i] = (p.data_ptr(), 0, m.data_ptr(), v.data_ptr(), _vector(ms, "exp_avg_scale", blocks, torch.float32),
+                             _vector(vs, "exp_avg_sq_scale", blocks, torch.float32), size, _code(p.dtype), 0, decay[i], 0)
         self.half = {p.dtype for p in params} - {torch.float32}
         if len(self.half) > 1:
             raise TypeError("float16 and bfloat16 parameters in one adamw_multi")
@@ -584,38 +607,48 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     optional) receives that norm; grad_scale multiplies every gradient first (1 / world size, 1 / loss scale).
     workspace (fp32, at least adamw_multi_workspace(len(grads)) floats; allocated unless given): give one of its own to a
     call that is captured into an ops.Graph.  A captured step keeps lr and the other numbers it was captured with."""
-    table, n = args.table, len(args.sizes)
+    sizes, rows, n = args.sizes, args.rows, len(args.sizes)
     if len(grads) != n:
         raise ValueError(f"adamw_multi: {len(grads)} gradients for {n} parameters")
-    dev = args.device if n else step_dev.device
-    _one_device(step_dev, norm, workspace)
-    kinds = set(args.half)
-    for q, g, size in zip(table, grads, args.sizes):
-        if g is None:
-            q.n = 0
-            continue
-        if g.numel() != size or g.device != dev or not g.is_contiguous():
-            raise ValueError(f"adamw_multi: a contiguous gradient of {size} elements on {dev} is needed, got {tuple(g.shape)} on {g.device}")
-        dt = g.dtype
-        if dt != torch.float32:
-            kinds.add(dt)
-        q.grad, q.grad_dtype, q.n = g.data_ptr(), dt_of(g), size
-    if step_dev.device != dev:
-        raise ValueError(f"step_dev on {step_dev.device}, the parameters on {dev}")
+    dev = args.device if n else step_dev.get_device()
+    if _one_device(step_dev, norm, workspace) != dev:
+        raise ValueError(f"step_dev on {step_dev.device}, the parameters on device {dev}")
+    missing = any(g is None for g in grads)
+    if missing:
+        some = [i for i, g in enumerate(grads) if g is not None]
+        rows["n"] = 0
+        kinds = {grads[i].dtype for i in some}
+        for i in some:
+            _gradients([grads[i]], [sizes[i]], dev, {grads[i].dtype}, args.rows[i:i + 1])
+    else:
+        kinds = {g.dtype for g in grads}
+        if len(kinds) < 2:
+            _gradients(grads, sizes, dev, kinds, rows)
+        else:
+            for i, g in enumerate(grads):
+                _gradients([g], [sizes[i]], dev, {g.dtype}, rows[i:i + 1])
+    kinds = (kinds | args.half) - {torch.float32}
     if len(kinds) > 1:
         raise TypeError("float16 and bfloat16 tensors in one adamw_multi")
     if max_norm is not None and not max_norm > 0:
         raise ValueError(f"max_norm has to be positive (or None), got {max_norm}")
     if workspace is None:
-        workspace = torch.empty((adamw_multi_workspace(n),), device=dev, dtype=torch.float32)
-    a = L.AdamWMultiArgs()
-    a.tensors, a.n_tensors, a.state_bits = table, n, args.state_bits
-    a.step_dev, a.norm = _vector(step_dev, "step_dev", 1, torch.int32), _vector(norm, "norm", 1, torch.float32)
-    a.workspace, a.workspace_bytes = _workspace(workspace)
-    a.lr, a.beta1, a.beta2, a.eps = lr, betas[0], betas[1], eps
-    a.max_norm, a.grad_scale = max_norm or 0.0, grad_scale
-    fn = lib(torch.float16 in kinds).stdiff_adamw_multi
-    _enqueue(dev, lambda st: fn(C.byref(a), st))
+        workspace = step_dev.new_empty((adamw_multi_workspace(n),), dtype=torch.float32)
+    ws, nb = _workspace(workspace)
+    a = L.AdamWMultiArgs(args.table, n, args.state_bits, _vector(step_dev, "step_dev", 1, torch.int32),
+                         _vector(norm, "norm", 1, torch.float32), ws, nb, lr, betas[0], betas[1], eps, max_norm or 0.0, grad_scale)
+    _enqueue(dev, lib(torch.float16 in kinds).stdiff_adamw_multi, C.byref(a))
+
+
+def _gradients(grads, sizes, dev, kind, rows):
+    """Checks gradients of one dtype and enters them into their rows of the table."""
+    if [g.numel() for g in grads] != sizes or {g.get_device() for g in grads} - {dev} or not all([g.is_contiguous() for g in grads]):
+        raise ValueError(f"adamw_multi: contiguous gradients of the parameters' {sizes if len(sizes) < 9 else 'sizes'} elements on device "
+                         f"{dev} are needed")
+    rows["grad"] = [g.data_ptr() for g in grads]
+    rows["n"] = sizes
+    for dtype in kind:
+        rows["grad_dtype"] = _code(dtype)
 
 
 def quantize_rows(x, out=None, scale=None):
@@ -627,13 +660,16 @@ def quantize_rows(x, out=None, scale=None):
     ldx = _read_ld(x, "x")
     R, K = x.shape
     if out is None:
-        out = torch.empty((R, round_up(K, 16)), device=dev, dtype=torch.int8)[:, :K]
-    ldq = _rows16(out, "out", (R, K))
+        ldq = round_up(K, 16)
+        out = x.new_empty((R, ldq), dtype=torch.int8)
+        if ldq != K:
+            out = out[:, :K]
+    else:
+        ldq = _rows16(out, "out", (R, K))
     if scale is None:
-        scale = torch.empty((R,), device=dev, dtype=torch.float32)
+        scale = x.new_empty((R,), dtype=torch.float32)
     sp = _vector(scale, "scale", R, torch.float32)
-    fn = lib_for(x).stdiff_quantize_rows
-    _enqueue(dev, lambda st: fn(x.data_ptr(), ldx, dt_of(x), out.data_ptr(), ldq, sp, R, K, st))
+    _enqueue(dev, _lib_of(x.dtype).stdiff_quantize_rows, x.data_ptr(), ldx, _code(x.dtype), out.data_ptr(), ldq, sp, R, K)
     return out, scale
 
 
@@ -662,15 +698,13 @@ def gemm_i8(A, a_scale, W, w_scale, bias=None, out=None, out_dtype=torch.float32
     if a_scale is None or w_scale is None:
         raise ValueError("a_scale and w_scale are needed")
     if out is None:
-        out = torch.empty((M, N), device=dev, dtype=out_dtype)
-    a = L.GemmI8Args()
-    a.M, a.N, a.K = M, N, K
-    a.A, a.lda, a.W, a.ldw = A.data_ptr(), lda, W.data_ptr(), ldw
-    a.a_scale, a.w_scale = _vector(a_scale, "a_scale", M, torch.float32), _vector(w_scale, "w_scale", N, torch.float32)
-    a.bias = _vector(bias, "bias", N, torch.float32)
-    a.C, a.ldc, a.c_dtype = out.data_ptr(), _write_ld(out, "out", (M, N)), dt_of(out)
-    fn = lib_for(out).stdiff_gemm_i8
-    _enqueue(dev, lambda st: fn(C.byref(a), st))
+        out, ldc = a_scale.new_empty((M, N), dtype=out_dtype), N
+    else:
+        ldc = _write_ld(out, "out", (M, N))
+    a = L.GemmI8Args(M, N, K, A.data_ptr(), lda, W.data_ptr(), ldw, _vector(a_scale, "a_scale", M, torch.float32),
+                     _vector(w_scale, "w_scale", N, torch.float32), _vector(bias, "bias", N, torch.float32), out.data_ptr(), ldc,
+                     _code(out.dtype))
+    _enqueue(dev, _lib_of(out.dtype).stdiff_gemm_i8, C.byref(a))
     return out
 
 

@@ -128,7 +128,7 @@ def grad_tol(dy, rstd, hat, g):
     return dx + 1e-14, (chain + 4) * U * (dy * hat).abs().sum(0) + 1e-14, chain * U * dy.abs().sum(0) + 1e-14
 
 
-@pytest.mark.parametrize("R,H", SIZES + [(1500, 320), (2077, 1001), (40, 9001)])
+@pytest.mark.parametrize("R,H", SIZES + [(700, 320), (1500, 320), (2077, 1001), (40, 9001), (2500, 64), (2100, 1024), (2300, 2051), (2060, 4099), (2200, 8192)])
 @pytest.mark.parametrize("xt,dt,wt", GRAD_KINDS)
 def test_layer_norm_bwd(ops, R, H, xt, dt, wt):
     x = (rnd(R, H, seed=20) + rnd(R, 1, seed=21)).to(DT[xt])
@@ -144,9 +144,8 @@ def test_layer_norm_bwd(ops, R, H, xt, dt, wt):
     within(db, wb, tb, "dbias")
 
 
-@pytest.mark.parametrize("H", [48, 1024, 3000, 8200])
-def test_layer_norm_bwd_options(ops, H):
-    R = 37
+@pytest.mark.parametrize("R,H", [(37, 48), (37, 1024), (37, 3000), (37, 8200), (5000, 48), (2500, 1024)])
+def test_layer_norm_bwd_options(ops, R, H):
     big, bigdy = rnd(R, H + 5, seed=30).to(DEV), rnd(R, H + 3, seed=31).to(DEV)
     x, dy, w = big[:, 2:H + 2], bigdy[:, 1:H + 1], rnd(H, seed=32).to(DEV)
     mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
@@ -554,8 +553,9 @@ def test_refusals(ops):
         ops.layer_norm_bwd(x, x, None, None)
     with pytest.raises(ValueError, match="accumulate"):
         ops.layer_norm_bwd(x, x, s4, s4, w, accumulate=True)
+    many, s9 = torch.zeros(9000, 32, device=DEV), torch.zeros(9000, device=DEV)
     with pytest.raises(ValueError, match="workspace"):
-        ops.layer_norm_bwd(x, x, s4, s4, w, workspace=torch.zeros(4, device=DEV))
+        ops.layer_norm_bwd(many, many, s9, s9, w, workspace=torch.zeros(4, device=DEV))
     with pytest.raises(ValueError, match="dy"):
         ops.layer_norm_bwd(x[:3], x, s4, s4, w)
     with pytest.raises(TypeError):
