@@ -191,6 +191,23 @@ __device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) {
     s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return max(s[0], s[1]);
 }
+// over groups of T lanes
+template <int T> __device__ __forceinline__ float lanes_sum_dpp(float v) {
+    static_assert(T == 8 || T == 16 || T == 32, "");
+#define STDIFF_DPP_ADD(ctrl) v += __builtin_bit_cast(float, STDIFF_DPP(__builtin_bit_cast(int, v), ctrl))
+    STDIFF_DPP_ADD(0xb1);
+    STDIFF_DPP_ADD(0x4e);
+    STDIFF_DPP_ADD(0x141);
+    if (T >= 16) STDIFF_DPP_ADD(0x140);
+#undef STDIFF_DPP_ADD
+    if (T == 32) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        const u32x2_swap s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+        const unsigned lo = s[0], hi = s[1];
+        v = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+    }
+    return v;
+}
 __device__ __forceinline__ float wave_sum_dpp(float v) {
 #define STDIFF_DPP_ADD(ctrl) v += __builtin_bit_cast(float, STDIFF_DPP(__builtin_bit_cast(int, v), ctrl))
     STDIFF_DPP_ADD(0xb1);

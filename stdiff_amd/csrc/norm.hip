@@ -3,9 +3,15 @@
 //   forward :  mu = mean x, var = mean (x - mu)^2, rstd = 1 / sqrt(var + eps), y = (x - mu) * rstd * w + b
 //   backward:  xhat = (x - mu) * rstd, g = dy * w, dx = rstd * (g - mean g - xhat * mean(g * xhat)),
 //              dw = sum over rows of dy * xhat, db = sum over rows of dy
-// A row is read once and stays in registers: V elements (16 bytes of x) per lane and vector, NV vectors per lane, T
-// lanes per row.  The variance is formed from the centred values (a second walk over the registers), so a row whose mean
-// is far larger than its spread keeps its digits.  All statistics and sums are fp32.
+// A row is read once and stays in registers, 16 elements per lane in vectors of 16 bytes of x: 8, 32 or 64 lanes share a row of
+// up to 128, 512 or 1024 elements (a wave holds 8, 2 or 1 of them), longer rows have a workgroup of ceil(H / 1024) waves,
+// up to 16384; beyond that (and below 8) the row is read again from the cache.  Small shares keep many rows in flight: with
+// one row per wave whatever its length, rows of 64 and 300 16-bit elements ran at 1.1 and 3.9 TB/s.
+// The vector that the row's end cuts is moved left until it fits: its lane holds some of its neighbour's columns again, leaves
+// them out of the sums and stores them a second time with the same bits.  (Element by element, the 7 elements at the end
+// of rows of 999 cost 0.8 of the time of all others.)
+// The variance is formed from the centred values (a second walk over the registers), so a row whose mean is far larger
+// than its spread keeps its digits.  All statistics and sums are fp32.
 #include "common.h"
 
 namespace {
@@ -54,57 +60,81 @@ template <int V, bool NT = false> __device__ __forceinline__ void stv(bf16_t* p,
     }
 }
 // V elements at column c of a row of H; what lies behind the row's end reads as `fill` and is not written
-template <int V, bool NT = false, typename T> __device__ __forceinline__ void ld_edge(const T* row, int c, int H, float fill, float* o) {
-    if (c + V <= H) return ldv<V, NT>(row + c, o);
+template <int V, typename T> __device__ __forceinline__ void ld_edge(const T* row, int c, int H, float fill, float* o) {
+    if (c + V <= H) return ldv<V>(row + c, o);
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = c + j < H ? Elem<T>::ld(row + c + j) : fill;
 }
-template <int V, bool NT = false, typename T> __device__ __forceinline__ void st_edge(T* row, int c, int H, const float* o) {
-    if (c + V <= H) return stv<V, NT>(row + c, o);
+template <int V, typename T> __device__ __forceinline__ void st_edge(T* row, int c, int H, const float* o) {
+    if (c + V <= H) return stv<V>(row + c, o);
 #pragma unroll
     for (int j = 0; j < V; ++j)
         if (c + j < H) Elem<T>::st(row + c + j, o[j]);
 }
 
-// sum over the T lanes of a row, the same bits in all of them; `part`: T / 64 floats per use, not reused before a barrier
-template <int T, int NTHR = 256> __device__ __forceinline__ float row_sum(float v, float* part) {
-    static_assert(T == 64 || T == NTHR, "a row is one wave's or the whole workgroup's");
-    v = wave_sum_dpp(v);
-    if constexpr (T > 64) {
+// the columns of a lane's vector that begins at c in a row of H >= V
+template <int V> struct span {
+    int at, skip;                          // the vector is read and written at `at`; its first `skip` elements are not its own
+    __device__ __forceinline__ span() {}
+    __device__ __forceinline__ span(int c, int H) : at(min(c, H - V)), skip(c - at) {}
+    __device__ __forceinline__ float own(float v, int j) const { return j >= skip ? v : 0.f; }
+    __device__ __forceinline__ bool in() const { return skip < V; }
+};
+
+// T lanes share a row; BLOCK and BIG_BLOCK: the whole workgroup does.  For fp32 rows BLOCK has up to 512 threads (held to the 128
+// registers of 1024 threads the backward keeps 25 of its 148 in memory: 199 against 138 us for 32768 x 2048) and BIG_BLOCK
+// up to 1024; for 16-bit rows BLOCK has up to 1024 (6 of 133 in memory, but a fourth wave per SIMD: 96 against 106 us for
+// 16000 x 4096).
+enum { BLOCK = 0, BIG_BLOCK = 1 };
+constexpr int E = 16;                     // elements per lane
+template <int T> __device__ __forceinline__ int row_lanes() { return T > BIG_BLOCK ? T : (int)blockDim.x; }
+template <int T> __device__ __forceinline__ int row_lane() { return T > BIG_BLOCK ? threadIdx.x % (T > BIG_BLOCK ? T : 1) : threadIdx.x; }
+template <int T> __device__ __forceinline__ int row_in_block() { return T > BIG_BLOCK ? threadIdx.x / (T > BIG_BLOCK ? T : 1) : 0; }
+template <int T> constexpr int rows_per_block(int threads) { return T > BIG_BLOCK ? threads / (T > BIG_BLOCK ? T : 1) : 1; }
+template <int T, int V> constexpr int most_threads() { return T > BIG_BLOCK ? 256 : T == BLOCK && V == 4 ? 512 : 1024; }
+
+// sum over the lanes of a row, the same bits in all of them; `part` (a workgroup's row): a float per wave, not used again before another
+// barrier
+template <int T> __device__ __forceinline__ float row_sum(float v, float* part) {
+    if constexpr (T <= BIG_BLOCK || T == 64) v = wave_sum_dpp(v);
+    else v = lanes_sum_dpp<T>(v);
+    if constexpr (T <= BIG_BLOCK) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
         v = 0.f;
-#pragma unroll
-        for (int i = 0; i < T / 64; ++i) v += part[i];
+        for (int i = 0; i < (int)blockDim.x / 64; ++i) v += part[i];
     }
     return v;
 }
 
-template <typename TX, typename TY, typename TW, int V, int NV, int T, bool NT>
-__global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long ldx, const TW* w, const TW* b, float eps,
-                                                         TY* y, long long ldy, float* mean, float* rstd, int R, int H) {
-    __shared__ float part[2][2][T / 64];
-    constexpr int ROWS = 256 / T;
-    const int t = threadIdx.x % T;
+template <typename TX, typename TY, typename TW, int V, int T, bool NT>
+__global__ __launch_bounds__((most_threads<T, V>())) void layer_norm_kernel(const TX* x, long long ldx, const TW* w, const TW* b, float eps,
+                                                                    TY* y, long long ldy, float* mean, float* rstd, int R, int H) {
+    __shared__ float part[2][2][16];
+    constexpr int NV = E / V;
+    constexpr int rows = rows_per_block<T>(256);
+    const int lanes = row_lanes<T>(), t = row_lane<T>();
     float wv[NV][V], bv[NV][V];
+    span<V> col[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * T + t) * V;
+        col[i] = span<V>((i * lanes + t) * V, H);
 #pragma unroll
         for (int j = 0; j < V; ++j) { wv[i][j] = 1.f; bv[i][j] = 0.f; }
-        if (w) ld_edge<V>(w, c, H, 0.f, wv[i]);
-        if (b) ld_edge<V>(b, c, H, 0.f, bv[i]);
+        if (w) ldv<V>(w + col[i].at, wv[i]);
+        if (b) ldv<V>(b + col[i].at, bv[i]);
     }
     const float inv = 1.0f / (float)H;
     int odd = 0;
-    for (long long row = (long long)blockIdx.x * ROWS + threadIdx.x / T; row < R; row += (long long)gridDim.x * ROWS, odd ^= 1) {
+    for (long long row = (long long)blockIdx.x * rows + row_in_block<T>(); row < R;
+         row += (long long)gridDim.x * rows, odd ^= 1) {
         float v[NV][V], s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) ld_edge<V, NT>(x + row * ldx, (i * T + t) * V, H, 0.f, v[i]);
+        for (int i = 0; i < NV; ++i) ldv<V, NT>(x + row * ldx + col[i].at, v[i]);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += v[i][j];
+            for (int j = 0; j < V; ++j) s += col[i].own(v[i][j], j);
         const float mu = row_sum<T>(s, part[odd][0]) * inv;
         float q = 0.f;
 #pragma unroll
@@ -112,7 +142,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long 
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 v[i][j] -= mu;
-                if ((i * T + t) * V + j < H) q += v[i][j] * v[i][j];
+                q += col[i].own(v[i][j] * v[i][j], j);
             }
         const float rs = 1.0f / sqrtf(row_sum<T>(q, part[odd][1]) * inv + eps);
 #pragma unroll
@@ -120,7 +150,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long 
             float o[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = v[i][j] * rs * wv[i][j] + bv[i][j];
-            st_edge<V, NT>(y + row * ldy, (i * T + t) * V, H, o);
+            if (col[i].in()) stv<V, NT>(y + row * ldy + col[i].at, o);
         }
         if (t == 0) {
             if (mean) mean[row] = mu;
@@ -133,7 +163,7 @@ __global__ __launch_bounds__(256) void layer_norm_kernel(const TX* x, long long 
 template <typename TX, typename TY, typename TW>
 __global__ __launch_bounds__(256) void layer_norm_long_kernel(const TX* x, long long ldx, const TW* w, const TW* b, float eps,
                                                               TY* y, long long ldy, float* mean, float* rstd, int R, int H) {
-    __shared__ float part[2][2][4];
+    __shared__ float part[2][2][16];
     const float inv = 1.0f / (float)H;
     int odd = 0;
     for (long long row = blockIdx.x; row < R; row += gridDim.x, odd ^= 1) {
@@ -145,14 +175,14 @@ __global__ __launch_bounds__(256) void layer_norm_long_kernel(const TX* x, long 
             ld_edge<4>(xr, c, H, 0.f, v);
             s += (v[0] + v[1]) + (v[2] + v[3]);
         }
-        const float mu = row_sum<256>(s, part[odd][0]) * inv;
+        const float mu = row_sum<BLOCK>(s, part[odd][0]) * inv;
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float v[4];
             ld_edge<4>(xr, c, H, mu, v);
 #pragma unroll
             for (int j = 0; j < 4; ++j) q += (v[j] - mu) * (v[j] - mu);
         }
-        const float rs = 1.0f / sqrtf(row_sum<256>(q, part[odd][1]) * inv + eps);
+        const float rs = 1.0f / sqrtf(row_sum<BLOCK>(q, part[odd][1]) * inv + eps);
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float v[4], wv[4] = {1.f, 1.f, 1.f, 1.f}, bv[4] = {0.f, 0.f, 0.f, 0.f};
             ld_edge<4>(xr, c, H, 0.f, v);
@@ -170,17 +200,21 @@ __global__ __launch_bounds__(256) void layer_norm_long_kernel(const TX* x, long 
 }
 
 // dx of the rows first, first + step, ..; SUMS: also this thread's share of sum dy * xhat and sum dy of its columns
-template <typename TX, typename TD, typename TW, int V, int NV, int T, int NTHR, bool SUMS, bool NT>
+template <typename TX, typename TD, typename TW, int V, int T, bool SUMS, bool NT>
 __device__ __forceinline__ void norm_bwd_rows(const TD* dy, long long lddy, const TX* x, long long ldx, const float* mean,
                                               const float* rstd, const TW* w, TX* dx, long long lddx, int R, int H, int t,
-                                              long long first, long long step, float (&aw)[NV][V], float (&ab)[NV][V]) {
-    __shared__ float part[2][2][NTHR / 64];
+                                              long long first, long long step, float (&aw)[E / V][V], float (&ab)[E / V][V]) {
+    __shared__ float part[2][2][16];
+    constexpr int NV = E / V;
+    const int lanes = row_lanes<T>();
     float wv[NV][V];
+    span<V> col[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+        col[i] = span<V>((i * lanes + t) * V, H);
 #pragma unroll
         for (int j = 0; j < V; ++j) { wv[i][j] = 1.f; aw[i][j] = ab[i][j] = 0.f; }
-        if (w) ld_edge<V>(w, (i * T + t) * V, H, 0.f, wv[i]);
+        if (w) ldv<V>(w + col[i].at, wv[i]);
     }
     const float inv = 1.0f / (float)H;
     int odd = 0;
@@ -189,8 +223,8 @@ __device__ __forceinline__ void norm_bwd_rows(const TD* dy, long long lddy, cons
         const float mu = mean[row], rs = rstd[row];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            ld_edge<V, NT>(dy + row * lddy, (i * T + t) * V, H, 0.f, d[i]); // behind the end dy = 0: nothing is added
-            ld_edge<V, NT>(x + row * ldx, (i * T + t) * V, H, 0.f, h[i]);
+            ldv<V, NT>(dy + row * lddy + col[i].at, d[i]);
+            ldv<V, NT>(x + row * ldx + col[i].at, h[i]);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -198,59 +232,67 @@ __device__ __forceinline__ void norm_bwd_rows(const TD* dy, long long lddy, cons
             for (int j = 0; j < V; ++j) {
                 h[i][j] = (h[i][j] - mu) * rs;
                 if constexpr (SUMS) {
-                    aw[i][j] += d[i][j] * h[i][j];
-                    ab[i][j] += d[i][j];
+                    const float own = col[i].own(d[i][j], j);
+                    aw[i][j] += own * h[i][j];
+                    ab[i][j] += own;
                 }
                 d[i][j] *= wv[i][j];
-                sg += d[i][j];
-                sgx += d[i][j] * h[i][j];
+                const float g = col[i].own(d[i][j], j);
+                sg += g;
+                sgx += g * h[i][j];
             }
-        const float mg = row_sum<T, NTHR>(sg, part[odd][0]) * inv, mgx = row_sum<T, NTHR>(sgx, part[odd][1]) * inv;
+        const float mg = row_sum<T>(sg, part[odd][0]) * inv, mgx = row_sum<T>(sgx, part[odd][1]) * inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float o[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = rs * (d[i][j] - mg - h[i][j] * mgx);
-            st_edge<V, NT>(dx + row * lddx, (i * T + t) * V, H, o);
+            if (col[i].in()) stv<V, NT>(dx + row * lddx + col[i].at, o);
         }
     }
 }
 
 // Many rows.  Every workgroup walks its rows with the column sums in registers and leaves one pair of partial sums:
 // ws [gridDim.x][2][ldp] of (dy * xhat, dy); ws NULL: dx only.
-template <typename TX, typename TD, typename TW, int V, int NV, int T, bool NT>
-__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
-                                                             const float* mean, const float* rstd, const TW* w, TX* dx,
-                                                             long long lddx, float* ws, int ldp, int R, int H) {
-    constexpr int WIDTH = 64 * V * NV;               // columns that a wave's registers cover (T == 64)
-    __shared__ __attribute__((aligned(16))) float comb[T == 64 ? 4 * WIDTH : 4];
-    constexpr int ROWS = 256 / T;
-    const int t = threadIdx.x % T;
+template <typename TX, typename TD, typename TW, int V, int T, bool NT>
+__global__ __launch_bounds__((most_threads<T, V>())) void layer_norm_bwd_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
+                                                                        const float* mean, const float* rstd, const TW* w, TX* dx,
+                                                                        long long lddx, float* ws, int ldp, int R, int H) {
+    constexpr int NV = E / V, ROWS = rows_per_block<T>(256), WIDTH = T * E;        // WIDTH: columns of a row's lanes
+    __shared__ __attribute__((aligned(16))) float comb[T > BIG_BLOCK ? ROWS * WIDTH : 4];
+    const int t = row_lane<T>(), r = row_in_block<T>();
     float aw[NV][V], ab[NV][V];
-    norm_bwd_rows<TX, TD, TW, V, NV, T, 256, true, NT>(dy, lddy, x, ldx, mean, rstd, w, dx, lddx, R, H, t,
-                                                   (long long)blockIdx.x * ROWS + threadIdx.x / T, (long long)gridDim.x * ROWS, aw, ab);
+    norm_bwd_rows<TX, TD, TW, V, T, true, NT>(dy, lddy, x, ldx, mean, rstd, w, dx, lddx, R, H, t, (long long)blockIdx.x * ROWS + r,
+                                              (long long)gridDim.x * ROWS, aw, ab);
     if (!ws) return;
     float* out = ws + (size_t)blockIdx.x * 2 * ldp;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const float(&a)[NV][V] = k ? ab : aw;
-        if constexpr (T == 64) {                     // the block's four waves, added in their order
+        if constexpr (T > BIG_BLOCK) {               // the workgroup's rows, added in their order
             if (k) __syncthreads();
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int j = 0; j < V; j += 4)
-                    *(f32x4*)(comb + (threadIdx.x >> 6) * WIDTH + (i * 64 + t) * V + j) = f32x4{a[i][j], a[i][j + 1], a[i][j + 2], a[i][j + 3]};
+                    *(f32x4*)(comb + r * WIDTH + (i * T + t) * V + j) = f32x4{a[i][j], a[i][j + 1], a[i][j + 2], a[i][j + 3]};
             __syncthreads();
-            for (int c = threadIdx.x * 4; c < ldp; c += 1024) {
-                f32x4 s = *(const f32x4*)(comb + c);
+            const int whole = H / V * V, shift = (V - H % V) % V;        // the last vector's own elements are its last ones
+            for (int c = threadIdx.x; c < H; c += 256) {
+                const float* e = comb + c + (c >= whole ? shift : 0);
+                float s = e[0];
 #pragma unroll
-                for (int i = 1; i < 4; ++i) s += *(const f32x4*)(comb + i * WIDTH + c);
-                *(f32x4*)(out + k * ldp + c) = s;
+                for (int i = 1; i < ROWS; ++i) s += e[i * WIDTH];
+                out[k * ldp + c] = s;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) st_edge<V>(out + k * ldp, (i * T + t) * V, H, a[i]);
+            for (int i = 0; i < NV; ++i) {
+                const span<V> col((i * (int)blockDim.x + t) * V, H);
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j >= col.skip) out[k * ldp + col.at + j] = a[i][j];
+            }
         }
     }
 }
@@ -258,30 +300,31 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(const TD* dy, long 
 // Few rows, one launch: the column sums need only the statistics, which are there already, so they do not wait for dx.  The
 // first `cols` workgroups own 32 columns each and walk down ALL rows (x and dy are read twice, the second time from the
 // cache); the others own rows and give dx.
-template <typename TX, typename TD, typename TW, int V, int NV, int T>
+template <typename TX, typename TD, typename TW, int V, int T>
 __global__ __launch_bounds__(512) void layer_norm_bwd_few_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
                                                                  const float* mean, const float* rstd, const TW* w, TX* dx,
                                                                  long long lddx, float* dweight, float* dbias, int accumulate,
                                                                  int cols, int R, int H) {
     if ((int)blockIdx.x >= cols) {
-        constexpr int ROWS = 512 / T;
-        float aw[NV][V], ab[NV][V];
-        norm_bwd_rows<TX, TD, TW, V, NV, T, 512, false, false>(dy, lddy, x, ldx, mean, rstd, w, dx, lddx, R, H, threadIdx.x % T,
-                                                        (long long)(blockIdx.x - cols) * ROWS + threadIdx.x / T,
-                                                        (long long)(gridDim.x - cols) * ROWS, aw, ab);
+        constexpr int ROWS = rows_per_block<T>(512);
+        float aw[E / V][V], ab[E / V][V];
+        norm_bwd_rows<TX, TD, TW, V, T, false, false>(dy, lddy, x, ldx, mean, rstd, w, dx, lddx, R, H,
+                                                      row_lane<T>(), (long long)(blockIdx.x - cols) * ROWS + row_in_block<T>(),
+                                                      (long long)(gridDim.x - cols) * ROWS, aw, ab);
         return;
     }
     constexpr int LANES = 32 / V, SLOTS = 512 / LANES;
     __shared__ float sums[2][SLOTS][32 + 1];
-    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, c = blockIdx.x * 32 + lane * V;
+    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+    const span<V> at(blockIdx.x * 32 + lane * V, H);
     float aw[V], ab[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) aw[j] = ab[j] = 0.f;
 #pragma unroll 4
     for (int row = slot; row < R; row += SLOTS) {
         float d[V], h[V];
-        ld_edge<V>(dy + row * lddy, c, H, 0.f, d);
-        ld_edge<V>(x + row * ldx, c, H, 0.f, h);
+        ldv<V>(dy + row * lddy + at.at, d);
+        ldv<V>(x + row * ldx + at.at, h);
         const float mu = mean[row], rs = rstd[row];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -297,9 +340,10 @@ __global__ __launch_bounds__(512) void layer_norm_bwd_few_kernel(const TD* dy, l
     __syncthreads();
     // 64 sums (two of 32 columns) of SLOTS terms each: eight threads per sum, then their eight in order
     const int col = threadIdx.x & 31, which = (threadIdx.x >> 5) & 1, share = threadIdx.x >> 6;
+    const int from = min(col + (blockIdx.x * 32 + col >= H / V * V ? (V - H % V) % V : 0), 31);
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < SLOTS / 8; ++i) s += sums[which][share * (SLOTS / 8) + i][col];
+    for (int i = 0; i < SLOTS / 8; ++i) s += sums[which][share * (SLOTS / 8) + i][from];
     __syncthreads();
     sums[which][share][col] = s;
     __syncthreads();
@@ -316,7 +360,7 @@ template <typename TX, typename TD, typename TW>
 __global__ __launch_bounds__(256) void layer_norm_bwd_long_kernel(const TD* dy, long long lddy, const TX* x, long long ldx,
                                                                   const float* mean, const float* rstd, const TW* w, TX* dx,
                                                                   long long lddx, int R, int H) {
-    __shared__ float part[2][2][4];
+    __shared__ float part[2][2][16];
     const float inv = 1.0f / (float)H;
     int odd = 0;
     for (long long row = blockIdx.x; row < R; row += gridDim.x, odd ^= 1) {
@@ -334,7 +378,7 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_long_kernel(const TD* dy, 
                 sgx += g * ((v[j] - mu) * rs);
             }
         }
-        const float mg = row_sum<256>(sg, part[odd][0]) * inv, mgx = row_sum<256>(sgx, part[odd][1]) * inv;
+        const float mg = row_sum<BLOCK>(sg, part[odd][0]) * inv, mgx = row_sum<BLOCK>(sgx, part[odd][1]) * inv;
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float d[4], v[4], wv[4] = {1.f, 1.f, 1.f, 1.f};
             ld_edge<4>(dy + row * lddy, c, H, 0.f, d);
@@ -401,7 +445,8 @@ __global__ __launch_bounds__(256) void fill_zero_kernel(float* a, float* b, int 
     if (b) b[i] = 0.f;
 }
 
-constexpr int IN_REGISTERS = 8192;        // longest row that the register kernels take
+constexpr int IN_REGISTERS = 16384;       // longest row that the register kernels take; the shortest is a vector
+inline bool in_registers(int H) { return H >= 8 && H <= IN_REGISTERS; }
 
 inline int norm_blocks(long long R, int rows_per_block, int per_cu) {
     return (int)std::min<long long>((R + rows_per_block - 1) / rows_per_block, (long long)per_cu * cu_count());
@@ -409,37 +454,53 @@ inline int norm_blocks(long long R, int rows_per_block, int per_cu) {
 // A call that moves more than the memory-side cache holds (256 MB) goes past the caches: 131072 x 1024 fp32 -> bf16 146 against
 // 155 us, backward of 32768 x 2048 fp32 139 against 150 us.  Below that the next kernel finds the result in a cache.
 inline bool past_caches(long long bytes) { return bytes > (256ll << 20); }
-inline int lanes_per_row(int H) { return H <= 2048 ? 64 : 256; }
-inline int bwd_parts(int R, int H) {
-    if (H > IN_REGISTERS) return (int)std::min<long long>(R, 64);
-    return norm_blocks(R, 256 / lanes_per_row(H), 2);
-}
+inline int lanes_of(int H) { return H <= 128 ? 8 : H <= 512 ? 32 : H <= 1024 ? 64 : BLOCK; }
+inline int threads_of(int H) { return H <= 1024 ? 256 : cdiv(H, 1024) * 64; }
+inline int rows_of_block(int H) { return H <= 1024 ? 256 / lanes_of(H) : 1; }
 // Up to 1024 rows the column sums walk down the rows in the launch that gives dx (512 x 1024 bf16: 4.0 us against 8.3 with partial
 // sums and a second launch; 1024 x 1024 fp32: 7.0 against 8.7; 2048 x 1024 fp32: 22 against 11)
-inline bool one_launch(int R, int H) { return R <= 1024 && H <= IN_REGISTERS; }
+inline bool one_launch(int R, int H) { return R <= 1024 && H >= 8 && H <= 8192; }
+// Workgroups of the backward: 16 waves per CU for rows of 16 bits, 8 for fp32 rows, which have as many bytes in flight (65536 x 1024
+// bf16: 8 waves 106 us, 16 waves 75; 32768 x 2048 fp32: 139 and 143 us, and twice the partial sums), and two rows at least
+// for each, so that the partial sums stay small beside the rows.
+inline int bwd_parts(int R, int H, int size) {
+    if (!in_registers(H)) return (int)std::min<long long>(R, 64);
+    return norm_blocks(R, rows_of_block(H) * 2, std::max(1, (size == 2 ? 1024 : 512) / threads_of(H)));
+}
 inline int ld_parts(int H) { return (H + 3) / 4 * 4; }
+
+#define NORM_LANES(CALL)                                  \
+    switch (lanes_of(H)) {                                \
+        case 8: CALL(8); break;                           \
+        case 32: CALL(32); break;                         \
+        case 64: CALL(64); break;                         \
+        default:                                          \
+            if constexpr (V == 4) {                       \
+                if (H > 8192) { CALL(BIG_BLOCK); break; } \
+            }                                             \
+            CALL(BLOCK);                                  \
+    }
 
 template <typename TX, typename TY, typename TW>
 int launch_ln(const void* x, long long ldx, const void* w, const void* b, float eps, void* y, long long ldy, float* mean,
               float* rstd, int R, int H, hipStream_t st) {
-    constexpr int V = sizeof(TX) == 2 ? 8 : 4, U = 8 / V;
-#define LN(NV, T)                                                              \
-    do {                                                                       \
-        if (streams) LN_AT(NV, T, true);                                       \
-        else LN_AT(NV, T, false);                                              \
-    } while (0)
-#define LN_AT(NV, T, NT)                                                                                                           \
-    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, TW, V, NV, T, NT>), dim3(norm_blocks(R, 256 / T, 8)), dim3(256), 0, st, (const TX*)x, \
-                       ldx, (const TW*)w, (const TW*)b, eps, (TY*)y, ldy, mean, rstd, R, H)
+    constexpr int V = sizeof(TX) == 2 ? 8 : 4;
     const bool streams = past_caches((long long)R * H * (sizeof(TX) + sizeof(TY)));
-    if (H <= 512) LN(U, 64);
-    else if (H <= 1024) LN(2 * U, 64);
-    else if (H <= 2048) LN(4 * U, 64);
-    else if (H <= 4096) LN(2 * U, 256);
-    else if (H <= IN_REGISTERS) LN(4 * U, 256);
-    else
+    const dim3 grid(norm_blocks(R, rows_of_block(H), 2048 / threads_of(std::min(H, IN_REGISTERS)))), block(threads_of(H));
+#define LN_AT(T, NT)                                                                                                           \
+    hipLaunchKernelGGL((layer_norm_kernel<TX, TY, TW, V, T, NT>), grid, block, 0, st, (const TX*)x, ldx, (const TW*)w, (const TW*)b, eps, \
+                       (TY*)y, ldy, mean, rstd, R, H)
+#define LN(T)                                                                  \
+    do {                                                                       \
+        if (streams) LN_AT(T, true);                                           \
+        else LN_AT(T, false);                                                  \
+    } while (0)
+    if (!in_registers(H))
         hipLaunchKernelGGL((layer_norm_long_kernel<TX, TY, TW>), dim3(norm_blocks(R, 1, 8)), dim3(256), 0, st, (const TX*)x, ldx,
                            (const TW*)w, (const TW*)b, eps, (TY*)y, ldy, mean, rstd, R, H);
+    else
+        NORM_LANES(LN)
+#undef LN
 #undef LN_AT
     STDIFF_LAUNCH_STATUS();
     return STDIFF_OK;
@@ -449,57 +510,56 @@ template <typename TX, typename TD, typename TW>
 int launch_ln_grad(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
                    const void* w, void* dx, long long lddx, float* dweight, float* dbias, int accumulate, float* ws, int R, int H,
                    hipStream_t st) {
-    constexpr int V = sizeof(TX) == 2 ? 8 : 4, U = 8 / V;
-    const int ldp = ld_parts(H), parts = bwd_parts(R, H);
+    constexpr int V = sizeof(TX) == 2 ? 8 : 4;
+    const int ldp = ld_parts(H), parts = bwd_parts(R, H, sizeof(TX));
     if (!ws && (dweight || dbias)) {                  // few rows
-        const int cols = cdiv(H, 32);
+        const int cols = cdiv(H, 32), rows = norm_blocks(R, H <= 1024 ? 8 : 1, 4);
         const auto meets = [&](const void* p, long long ld, size_t size) {
             const uintptr_t a = (uintptr_t)p, b = (uintptr_t)dx;
             return a < b + ((R - 1) * lddx + H) * sizeof(TX) && b < a + ((R - 1) * ld + H) * size;
         };
         // dx in the place of x or dy: the columns first, in a launch of their own
         const bool in_place = meets(x, ldx, sizeof(TX)) || meets(dy, lddy, sizeof(TD));
-#define FEW_AT(GRID, COLS, NV, T)                                                                                                    \
-    hipLaunchKernelGGL((layer_norm_bwd_few_kernel<TX, TD, TW, V, NV, T>), dim3(GRID), dim3(512), 0, st, (const TD*)dy, lddy,          \
-                       (const TX*)x, ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, dweight, dbias, accumulate, COLS, R, H)
-#define FEW(NV, T)                                                    \
-    do {                                                              \
-        const int rows = norm_blocks(R, 512 / T, 4);                  \
-        if (in_place) {                                               \
-            FEW_AT(cols, cols, NV, T);                                \
-            FEW_AT(rows, 0, NV, T);                                   \
-        } else {                                                      \
-            FEW_AT(cols + rows, cols, NV, T);                         \
-        }                                                             \
+#define FEW(GRID, COLS, T)                                                                                                        \
+    hipLaunchKernelGGL((layer_norm_bwd_few_kernel<TX, TD, TW, V, T>), dim3(GRID), dim3(512), 0, st, (const TD*)dy, lddy, (const TX*)x, \
+                       ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, dweight, dbias, accumulate, COLS, R, H)
+#define FEW_AT(GRID, COLS)                        \
+    do {                                          \
+        if (H <= 1024) FEW(GRID, COLS, 64);       \
+        else FEW(GRID, COLS, BLOCK);              \
     } while (0)
-        if (H <= 512) FEW(U, 64);
-        else if (H <= 1024) FEW(2 * U, 64);
-        else if (H <= 2048) FEW(4 * U, 64);
-        else if (H <= 4096) FEW(U, 512);
-        else FEW(2 * U, 512);
+        if (in_place) {
+            FEW_AT(cols, cols);
+            FEW_AT(rows, 0);
+        } else {
+            FEW_AT(cols + rows, cols);
+        }
 #undef FEW
 #undef FEW_AT
         STDIFF_LAUNCH_STATUS();
         return STDIFF_OK;
     }
-#define LN_AT(NV, T, NT)                                                                                                       \
-    hipLaunchKernelGGL((layer_norm_bwd_kernel<TX, TD, TW, V, NV, T, NT>), dim3(parts), dim3(256), 0, st, (const TD*)dy, lddy,   \
-                       (const TX*)x, ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, ws, ldp, R, H)
     const bool streams = past_caches((long long)R * H * (2 * sizeof(TX) + sizeof(TD)));
-    if (H <= 512) LN(U, 64);
-    else if (H <= 1024) LN(2 * U, 64);
-    else if (H <= 2048) LN(4 * U, 64);
-    else if (H <= 4096) LN(2 * U, 256);
-    else if (H <= IN_REGISTERS) LN(4 * U, 256);
-    else {
+    const dim3 grid(parts), block(threads_of(H));
+#define LN_AT(T, NT)                                                                                                          \
+    hipLaunchKernelGGL((layer_norm_bwd_kernel<TX, TD, TW, V, T, NT>), grid, block, 0, st, (const TD*)dy, lddy, (const TX*)x, ldx, mean, \
+                       rstd, (const TW*)w, (TX*)dx, lddx, ws, ldp, R, H)
+#define LN(T)                                                                  \
+    do {                                                                       \
+        if (streams) LN_AT(T, true);                                           \
+        else LN_AT(T, false);                                                  \
+    } while (0)
+    if (!in_registers(H)) {
         if (ws)
             hipLaunchKernelGGL((layer_norm_bwd_columns_kernel<TX, TD>), dim3(cdiv(H, 1024), parts), dim3(256), 0, st, (const TD*)dy,
                                lddy, (const TX*)x, ldx, mean, rstd, ws, ldp, R, H);
         hipLaunchKernelGGL((layer_norm_bwd_long_kernel<TX, TD, TW>), dim3(norm_blocks(R, 1, 8)), dim3(256), 0, st, (const TD*)dy,
                            lddy, (const TX*)x, ldx, mean, rstd, (const TW*)w, (TX*)dx, lddx, R, H);
+    } else {
+        NORM_LANES(LN)
     }
-#undef LN_AT
 #undef LN
+#undef LN_AT
     STDIFF_LAUNCH_STATUS();
     if (ws) {
         hipLaunchKernelGGL(layer_norm_bwd_join_kernel, dim3(cdiv(H, 32), 2), dim3(256), 0, st, ws, ldp, parts, dweight, dbias, accumulate, H);
@@ -538,7 +598,7 @@ extern "C" int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, cons
 
 extern "C" long long stdiff_layer_norm_bwd_workspace(int R, int H) {
     if (R < 0 || H <= 0) return STDIFF_ERR_ARG;
-    return one_launch(R, H) ? 0 : (long long)bwd_parts(R, H) * 2 * ld_parts(H) * 4;
+    return one_launch(R, H) ? 0 : (long long)bwd_parts(R, H, 2) * 2 * ld_parts(H) * 4;
 }
 
 extern "C" int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const void* x, long long ldx, int x_dtype,

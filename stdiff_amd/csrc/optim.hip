@@ -121,12 +121,17 @@ __device__ __forceinline__ float wave_amax(f32x4 v) {
     for (int j = 0; j < 4; ++j) a = max(a, __builtin_bit_cast(unsigned, (float)v[j]) & 0x7fffffffu);
     return __builtin_bit_cast(float, wave_umax_dpp(a));
 }
-// scale of a block, and what its elements are multiplied by before they become codes.  Below 1e-30 the factor
-// 448 / largest would leave the range of fp32: such blocks are scaled as if their largest were 1e-30.
-__device__ __forceinline__ float block_scale(float top, float* factor) {
-    if (top > 0.f && top < 1e-30f) top = 1e-30f;
-    *factor = top == 0.f ? 0.f : 448.0f / top;
-    return top / 448.0f;
+// Scales of a wave's blocks, and what their elements are multiplied by before they become codes.  One division for up to eight of
+// them: lanes k and 8 + k (of every 16) come with the k-th block's largest magnitude t, lane k leaves with 448 / t, lane 8 + k
+// with t / 448.  Below 1e-30 the factor would leave the range of fp32: such blocks are scaled as if t were 1e-30.
+__device__ __forceinline__ float block_scales(float t) {
+    const bool scale = threadIdx.x & 8;
+    if (t > 0.f && t < 1e-30f) t = 1e-30f;
+    const float q = (scale ? t : 448.0f) / (scale ? 448.0f : t);
+    return t == 0.f ? 0.f : q;
+}
+__device__ __forceinline__ float of_lane(float v, int k) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), k));
 }
 
 template <typename B> __device__ __forceinline__ int tensor_of(const B& b, int chunk, int t) {
@@ -251,10 +256,10 @@ __device__ __forceinline__ void turn(const T& q, long long start, const update_a
         f.inv_second = 1.0f / a.scalars[1];
         f.coef = gradient_factor(a, part);
     }
+    f32x4 r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const long long i = at + u * 1024;
-        f32x4 r;
         if constexpr (BITS == 8) {
             m[u] = from_e4m3(mc[u], ms[u]);
             v[u] = from_e4m3(vc[u], vs[u]);
@@ -265,36 +270,48 @@ __device__ __forceinline__ void turn(const T& q, long long start, const update_a
             const float gr = g[u][j] * f.coef;
             m[u][j] = m[u][j] * a.b1 + gr * a.omb1;
             v[u][j] = v[u][j] * a.b2 + gr * gr * a.omb2;
-            r[j] = sqrtf(v[u][j]);
+            r[u][j] = sqrtf(v[u][j]);
             // the quotient by the hardware's reciprocal (off by one unit in the last place): a few 2^-24 of a step that
             // is itself a small part of p; two full divisions cost a third of this kernel's instructions
-            p[u][j] = p[u][j] * keep - f.step * (m[u][j] * __builtin_amdgcn_rcpf(r[j] * f.inv_second + a.eps));
+            p[u][j] = p[u][j] * keep - f.step * (m[u][j] * __builtin_amdgcn_rcpf(r[u][j] * f.inv_second + a.eps));
         }
         st4e<WHOLE>((TP*)q.p + i, k[u], p[u]);
-        if constexpr (BITS == 8) {
-            if constexpr (!WHOLE) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j >= k[u]) m[u][j] = r[j] = 0.f;            // behind the end: no part of the block
-            }
-            float fm, fr;
-            const float sm = block_scale(wave_amax(m[u]), &fm), sr = block_scale(wave_amax(r), &fr);
-            f32x4 z;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                z[j] = r[j] * fr;
-                if (r[j] > 0.f && z[j] < 0x1p-9f) z[j] = 0x1p-9f;
-            }
-            st_codes<WHOLE>(q.m + i, k[u], to_e4m3(m[u] * fm));
-            st_codes<WHOLE>(q.v + i, k[u], to_e4m3(z));
-            if ((threadIdx.x & 63) == 0 && k[u] > 0) {
-                q.ms[i / BLOCK] = sm;
-                q.vs[i / BLOCK] = sr;
-            }
-        } else {
+        if constexpr (BITS == 32) {
             st4e<WHOLE>(q.m + i, k[u], m[u]);
             st4e<WHOLE>(q.v + i, k[u], v[u]);
         }
+    }
+    if constexpr (BITS == 8) {
+        const int slot = threadIdx.x & 7;
+        float top = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if constexpr (!WHOLE) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j >= k[u]) m[u][j] = r[u][j] = 0.f;         // behind the end: no part of the block
+            }
+            const float tm = wave_amax(m[u]), tr = wave_amax(r[u]);
+            if (slot == 2 * u) top = tm;
+            if (slot == 2 * u + 1) top = tr;
+        }
+        const float scales = block_scales(top);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float fr = of_lane(scales, 2 * u + 1);
+            f32x4 z;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                z[j] = r[u][j] * fr;
+                if (r[u][j] > 0.f && z[j] < 0x1p-9f) z[j] = 0x1p-9f;
+            }
+            st_codes<WHOLE>(q.m + at + u * 1024, k[u], to_e4m3(m[u] * of_lane(scales, 2 * u)));
+            st_codes<WHOLE>(q.v + at + u * 1024, k[u], to_e4m3(z));
+        }
+        // lanes 8 .. 8 + 2 U - 1 hold the scales
+        const int lane = threadIdx.x & 63, own = lane - 8, u = own >> 1;
+        const long long first = start + (threadIdx.x - lane) * 4 + u * 1024;          // first element of this lane's block
+        if (own >= 0 && own < 2 * U && (WHOLE || first < q.n)) (own & 1 ? q.vs : q.ms)[first / BLOCK] = scales;
     }
 }
 
@@ -327,6 +344,9 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(B b, update_arg a) {
 
 inline bool at_bytes(const void* p, int size) { return ((uintptr_t)p & (size - 1)) == 0; }
 inline int max_blocks() { return 4 * cu_count(); }
+// Workgroups per CU of the update: four, for what is larger than the caches by far two, whose fewer streams suit the memory
+// better (8-bit states, 30 M elements: four 99, two 113 us; 479 M: 1515 and 1436 us; 32-bit, 120 M: 649 and 645 us)
+inline int update_blocks(long long elements) { return (elements > (1ll << 26) ? 2 : 4) * cu_count(); }
 
 void set_tensor(tensor32& t, const stdiff_adamw_tensor& s) {
     t.p = s.param; t.g = s.grad; t.m = (float*)s.exp_avg; t.v = (float*)s.exp_avg_sq; t.n = s.n; t.wd = s.weight_decay;
@@ -356,12 +376,12 @@ template <typename T, int N> int fill(const stdiff_adamw_multi_args* a, int* at,
     return b->first[b->count];
 }
 
-template <int BITS, int U, typename B> int update(const stdiff_adamw_multi_args* a, const update_arg& u, hipStream_t st) {
+template <int BITS, int U, typename B> int update(const stdiff_adamw_multi_args* a, const update_arg& u, long long total, hipStream_t st) {
     B b;
     for (int at = 0; at < a->n_tensors;) {
         const int chunks = fill(a, &at, U * 1024, &b);
         if (!chunks) continue;
-        hipLaunchKernelGGL((adamw_update_kernel<BITS, U, B>), dim3(std::min(chunks, max_blocks())), dim3(256), 0, st, b, u);
+        hipLaunchKernelGGL((adamw_update_kernel<BITS, U, B>), dim3(std::min(chunks, update_blocks(total))), dim3(256), 0, st, b, u);
         STDIFF_LAUNCH_STATUS();
     }
     return STDIFF_OK;
@@ -432,6 +452,6 @@ extern "C" int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream
     long long total = 0;
     for (int i = 0; i < a->n_tensors; ++i) total += a->tensors[i].n;
     const bool few = total < 4096ll * 2 * cu_count();               // small turns spread the work over all CUs
-    if (a->state_bits == 8) return few ? update<8, 1, batch8>(a, u, st) : update<8, 4, batch8>(a, u, st);
-    return few ? update<32, 1, batch32>(a, u, st) : update<32, 4, batch32>(a, u, st);
+    if (a->state_bits == 8) return few ? update<8, 1, batch8>(a, u, total, st) : update<8, 4, batch8>(a, u, total, st);
+    return few ? update<32, 1, batch32>(a, u, total, st) : update<32, 4, batch32>(a, u, total, st);
 }

@@ -393,13 +393,16 @@ def _one_device(first, *rest):
     return dev
 
 
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _enqueue(dev, fn, *args):
     """check(fn(*args, stream)) with the stream that is current on device `dev`, `dev` being the current device meanwhile."""
-    if dev == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if dev == _current_device():
+        rc = fn(*args, _current_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            rc = fn(*args, _current_stream(dev))
     if rc:
         check(rc)
 
@@ -431,13 +434,13 @@ def _write_ld(t, name, shape):
     return ld
 
 
-def _vector(t, name, n, *dtypes):
-    """None, or the address of a contiguous vector of n elements of one of these types."""
+def _vector(t, name, n, dtype=torch.float32):
+    """None, or the address of a contiguous vector of n elements of this type (or of one of these)."""
     if t is None:
         return None
-    if t.dim() != 1 or t.numel() != n or t.dtype not in dtypes or not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous vector of {n} elements of {' / '.join(str(d) for d in dtypes)} is needed, "
-                         f"got {tuple(t.shape)} {t.dtype}")
+    kind = t.dtype
+    if not (kind is dtype or (dtype is _FLOATS and kind in _FLOATS)) or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous vector of {n} elements of {dtype} is needed, got {tuple(t.shape)} {kind}")
     return t.data_ptr()
 
 
@@ -449,7 +452,7 @@ def _affine(weight, bias, H):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: one dtype is needed")
     one = weight if weight is not None else bias
-    return _vector(weight, "weight", H, *_FLOATS), _vector(bias, "bias", H, *_FLOATS), torch.float32 if one is None else one.dtype
+    return _vector(weight, "weight", H, _FLOATS), _vector(bias, "bias", H, _FLOATS), torch.float32 if one is None else one.dtype
 
 
 def _code(dtype):
@@ -473,7 +476,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, me
     else:
         ldy = _write_ld(out, "out", x.shape)
     w, b, wdt = _affine(weight, bias, H)
-    mp, rp = _vector(mean, "mean", R, torch.float32), _vector(rstd, "rstd", R, torch.float32)
+    mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
     xdt, ydt = x.dtype, out.dtype
     _enqueue(dev, _lib_of(xdt, ydt, wdt).stdiff_layer_norm, x.data_ptr(), ldx, _code(xdt), w, b, _code(wdt), eps, out.data_ptr(), ldy,
              _code(ydt), mp, rp, R, H)
@@ -507,8 +510,8 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=
     w, _, wdt = _affine(weight, None, H)
     if mean is None or rstd is None:
         raise ValueError("mean and rstd of the forward are needed")
-    mp, rp = _vector(mean, "mean", R, torch.float32), _vector(rstd, "rstd", R, torch.float32)
-    dw, db = _vector(dweight, "dweight", H, torch.float32), _vector(dbias, "dbias", H, torch.float32)
+    mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
+    dw, db = _vector(dweight, "dweight", H), _vector(dbias, "dbias", H)
     xdt, ddt = x.dtype, dy.dtype
     lb = _lib_of(xdt, ddt, wdt)
     if workspace is None and (dweight is not None or dbias is not None):
@@ -566,8 +569,9 @@ class AdamWTensors:
             if self.state_bits == 8 and (ms is None or vs is None):
                 raise ValueError("8-bit states need exp_avg_scale and exp_avg_sq_scale")
             blocks = -(-size // 256)
-            self.table[i] = (p.data_ptr(), 0, m.data_ptr(), v.data_ptr(), _vector(ms, "exp_avg_scale", blocks, torch.float32),
-                             _vector(vs, "exp_avg_sq_scale", blocks, torch.float32), size, _code(p.dtype), 0, decay[i], 0)
+            self.table[i] = (p.data_ptr(), 0, m.data_ptr(), v.data_ptr(), _vector(ms, "exp_avg_scale", blocks),
+                             _vector(vs, "exp_avg_sq_scale", blocks), size, _code(p.dtype), 0, decay[i], 0)
+        self.partial = False                  # the last step left tensors out
         self.half = {p.dtype for p in params} - {torch.float32}
         if len(self.half) > 1:
             raise TypeError("float16 and bfloat16 parameters in one adamw_multi")
@@ -613,14 +617,16 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     dev = args.device if n else step_dev.get_device()
     if _one_device(step_dev, norm, workspace) != dev:
         raise ValueError(f"step_dev on {step_dev.device}, the parameters on device {dev}")
-    missing = any(g is None for g in grads)
-    if missing:
+    if any([g is None for g in grads]):
+        args.partial, rows["n"] = True, 0
         some = [i for i, g in enumerate(grads) if g is not None]
-        rows["n"] = 0
-        kinds = {grads[i].dtype for i in some}
         for i in some:
-            _gradients([grads[i]], [sizes[i]], dev, {grads[i].dtype}, args.rows[i:i + 1])
+            _gradients([grads[i]], [sizes[i]], dev, {grads[i].dtype}, rows[i:i + 1])
+            rows["n"][i] = sizes[i]
+        kinds = {grads[i].dtype for i in some}
     else:
+        if args.partial:
+            args.partial, rows["n"] = False, sizes
         kinds = {g.dtype for g in grads}
         if len(kinds) < 2:
             _gradients(grads, sizes, dev, kinds, rows)
@@ -636,7 +642,7 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
         workspace = step_dev.new_empty((adamw_multi_workspace(n),), dtype=torch.float32)
     ws, nb = _workspace(workspace)
     a = L.AdamWMultiArgs(args.table, n, args.state_bits, _vector(step_dev, "step_dev", 1, torch.int32),
-                         _vector(norm, "norm", 1, torch.float32), ws, nb, lr, betas[0], betas[1], eps, max_norm or 0.0, grad_scale)
+                         _vector(norm, "norm", 1), ws, nb, lr, betas[0], betas[1], eps, max_norm or 0.0, grad_scale)
     _enqueue(dev, lib(torch.float16 in kinds).stdiff_adamw_multi, C.byref(a))
 
 
@@ -646,7 +652,6 @@ def _gradients(grads, sizes, dev, kind, rows):
         raise ValueError(f"adamw_multi: contiguous gradients of the parameters' {sizes if len(sizes) < 9 else 'sizes'} elements on device "
                          f"{dev} are needed")
     rows["grad"] = [g.data_ptr() for g in grads]
-    rows["n"] = sizes
     for dtype in kind:
         rows["grad_dtype"] = _code(dtype)
 
@@ -668,7 +673,7 @@ def quantize_rows(x, out=None, scale=None):
         ldq = _rows16(out, "out", (R, K))
     if scale is None:
         scale = x.new_empty((R,), dtype=torch.float32)
-    sp = _vector(scale, "scale", R, torch.float32)
+    sp = _vector(scale, "scale", R)
     _enqueue(dev, _lib_of(x.dtype).stdiff_quantize_rows, x.data_ptr(), ldx, _code(x.dtype), out.data_ptr(), ldq, sp, R, K)
     return out, scale
 
@@ -678,10 +683,11 @@ def _rows16(t, name, shape=None):
     if t.dtype != torch.int8:
         raise TypeError(f"{name}: int8 is needed, got {t.dtype}")
     ld = _read_ld(t, name, shape)
-    rows, kp = t.shape[0], round_up(t.shape[1], 16)
+    rows, k = t.shape
+    kp = round_up(k, 16)
     ld = ld if rows > 1 else kp
     if rows and (ld % 16 or ld < kp or t.data_ptr() % 16 or
-                 t.storage_offset() + (rows - 1) * ld + kp > t.untyped_storage().nbytes()):
+                 (kp > k and t.storage_offset() + (rows - 1) * ld + kp > t.untyped_storage().nbytes())):
         raise ValueError(f"{name}: rows have to begin on 16-byte borders and to reach the next border behind their end in memory, "
                          f"as quantize_rows lays them out; got shape {tuple(t.shape)}, strides {t.stride()}")
     return ld
@@ -701,8 +707,8 @@ def gemm_i8(A, a_scale, W, w_scale, bias=None, out=None, out_dtype=torch.float32
         out, ldc = a_scale.new_empty((M, N), dtype=out_dtype), N
     else:
         ldc = _write_ld(out, "out", (M, N))
-    a = L.GemmI8Args(M, N, K, A.data_ptr(), lda, W.data_ptr(), ldw, _vector(a_scale, "a_scale", M, torch.float32),
-                     _vector(w_scale, "w_scale", N, torch.float32), _vector(bias, "bias", N, torch.float32), out.data_ptr(), ldc,
+    a = L.GemmI8Args(M, N, K, A.data_ptr(), lda, W.data_ptr(), ldw, _vector(a_scale, "a_scale", M),
+                     _vector(w_scale, "w_scale", N), _vector(bias, "bias", N), out.data_ptr(), ldc,
                      _code(out.dtype))
     _enqueue(dev, _lib_of(out.dtype).stdiff_gemm_i8, C.byref(a))
     return out
