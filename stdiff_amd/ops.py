@@ -1,6 +1,7 @@
 """Tensor-level wrappers over the C ABI (one function per entry point of include/stdiff_hip.h).
 Tensors must live on the GPU; outputs are allocated with torch when not supplied."""
 import ctypes as C
+import operator
 
 import numpy as np
 import torch
@@ -439,7 +440,8 @@ def _vector(t, name, n, dtype=torch.float32):
     if t is None:
         return None
     kind = t.dtype
-    if not (kind is dtype or (dtype is _FLOATS and kind in _FLOATS)) or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+    if t.numel() != n or (t.stride() != (1,) and not (t.dim() == 1 and n <= 1)) or \
+            not (kind is dtype or (dtype is _FLOATS and kind in _FLOATS)):
         raise ValueError(f"{name}: a contiguous vector of {n} elements of {dtype} is needed, got {tuple(t.shape)} {kind}")
     return t.data_ptr()
 
@@ -476,7 +478,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, me
     else:
         ldy = _write_ld(out, "out", x.shape)
     w, b, wdt = _affine(weight, bias, H)
-    mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
+    mp = rp = None
+    if mean is not None or rstd is not None:
+        mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
     xdt, ydt = x.dtype, out.dtype
     _enqueue(dev, _lib_of(xdt, ydt, wdt).stdiff_layer_norm, x.data_ptr(), ldx, _code(xdt), w, b, _code(wdt), eps, out.data_ptr(), ldy,
              _code(ydt), mp, rp, R, H)
@@ -502,16 +506,20 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=
         raise TypeError(f"dx is {dx.dtype}, x {x.dtype}")
     else:
         lddx = _write_ld(dx, "dx", x.shape)
-    if weight is not None and not accumulate:
-        if dweight is None:
-            dweight = x.new_empty((H,), dtype=torch.float32)
-        if dbias is None:
-            dbias = x.new_empty((H,), dtype=torch.float32)
-    w, _, wdt = _affine(weight, None, H)
+    dw, db = _vector(dweight, "dweight", H), _vector(dbias, "dbias", H)
+    w, wdt = None, torch.float32
+    if weight is not None:
+        w, wdt = _vector(weight, "weight", H, _FLOATS), weight.dtype
+        if not accumulate:
+            if dweight is None:
+                dweight = x.new_empty((H,), dtype=torch.float32)
+                dw = dweight.data_ptr()
+            if dbias is None:
+                dbias = x.new_empty((H,), dtype=torch.float32)
+                db = dbias.data_ptr()
     if mean is None or rstd is None:
         raise ValueError("mean and rstd of the forward are needed")
     mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
-    dw, db = _vector(dweight, "dweight", H), _vector(dbias, "dbias", H)
     xdt, ddt = x.dtype, dy.dtype
     lb = _lib_of(xdt, ddt, wdt)
     if workspace is None and (dweight is not None or dbias is not None):
@@ -617,22 +625,22 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     dev = args.device if n else step_dev.get_device()
     if _one_device(step_dev, norm, workspace) != dev:
         raise ValueError(f"step_dev on {step_dev.device}, the parameters on device {dev}")
-    if any([g is None for g in grads]):
-        args.partial, rows["n"] = True, 0
-        some = [i for i, g in enumerate(grads) if g is not None]
-        for i in some:
-            _gradients([grads[i]], [sizes[i]], dev, {grads[i].dtype}, rows[i:i + 1])
-            rows["n"][i] = sizes[i]
-        kinds = {grads[i].dtype for i in some}
-    else:
+    try:
+        kinds = set(map(_dtype, grads))
+    except AttributeError:
+        kinds = None                           # some are missing
+    if kinds is not None and len(kinds) == 1:
         if args.partial:
             args.partial, rows["n"] = False, sizes
-        kinds = {g.dtype for g in grads}
-        if len(kinds) < 2:
-            _gradients(grads, sizes, dev, kinds, rows)
-        else:
-            for i, g in enumerate(grads):
+        _gradients(grads, sizes, dev, kinds, rows)
+    else:
+        args.partial, rows["n"] = True, 0
+        kinds = set()
+        for i, g in enumerate(grads):
+            if g is not None:
                 _gradients([g], [sizes[i]], dev, {g.dtype}, rows[i:i + 1])
+                rows["n"][i] = sizes[i]
+                kinds.add(g.dtype)
     kinds = (kinds | args.half) - {torch.float32}
     if len(kinds) > 1:
         raise TypeError("float16 and bfloat16 tensors in one adamw_multi")
@@ -646,12 +654,16 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     _enqueue(dev, lib(torch.float16 in kinds).stdiff_adamw_multi, C.byref(a))
 
 
+_dtype, _numel, _get_device = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.get_device
+_is_contiguous, _data_ptr = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
+
 def _gradients(grads, sizes, dev, kind, rows):
     """Checks gradients of one dtype and enters them into their rows of the table."""
-    if [g.numel() for g in grads] != sizes or {g.get_device() for g in grads} - {dev} or not all([g.is_contiguous() for g in grads]):
+    if list(map(_numel, grads)) != sizes or set(map(_get_device, grads)) != {dev} or not all(map(_is_contiguous, grads)):
         raise ValueError(f"adamw_multi: contiguous gradients of the parameters' {sizes if len(sizes) < 9 else 'sizes'} elements on device "
                          f"{dev} are needed")
-    rows["grad"] = [g.data_ptr() for g in grads]
+    rows["grad"] = list(map(_data_ptr, grads))
     for dtype in kind:
         rows["grad_dtype"] = _code(dtype)
 
@@ -680,14 +692,15 @@ def quantize_rows(x, out=None, scale=None):
 
 def _rows16(t, name, shape=None):
     """Leading dimension of an int8 matrix whose rows begin on 16-byte borders and may be touched up to the next border."""
-    if t.dtype != torch.int8:
+    if t.dtype is not torch.int8:
         raise TypeError(f"{name}: int8 is needed, got {t.dtype}")
     ld = _read_ld(t, name, shape)
     rows, k = t.shape
-    kp = round_up(k, 16)
-    ld = ld if rows > 1 else kp
-    if rows and (ld % 16 or ld < kp or t.data_ptr() % 16 or
-                 (kp > k and t.storage_offset() + (rows - 1) * ld + kp > t.untyped_storage().nbytes())):
+    kp = (k + 15) & ~15
+    if rows == 1:
+        ld = kp
+    if (ld & 15 or ld < kp or t.data_ptr() & 15 or
+            (kp > k and t.storage_offset() + (rows - 1) * ld + kp > t.untyped_storage().nbytes())) and rows:
         raise ValueError(f"{name}: rows have to begin on 16-byte borders and to reach the next border behind their end in memory, "
                          f"as quantize_rows lays them out; got shape {tuple(t.shape)}, strides {t.stride()}")
     return ld
