@@ -193,12 +193,12 @@ __device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) {
 }
 // over groups of T lanes
 template <int T> __device__ __forceinline__ float lanes_sum_dpp(float v) {
-    static_assert(T == 8 || T == 16 || T == 32, "");
+    static_assert(T == 8 || T == 32, "");
 #define STDIFF_DPP_ADD(ctrl) v += __builtin_bit_cast(float, STDIFF_DPP(__builtin_bit_cast(int, v), ctrl))
     STDIFF_DPP_ADD(0xb1);
     STDIFF_DPP_ADD(0x4e);
     STDIFF_DPP_ADD(0x141);
-    if (T >= 16) STDIFF_DPP_ADD(0x140);
+    if (T == 32) STDIFF_DPP_ADD(0x140);
 #undef STDIFF_DPP_ADD
     if (T == 32) {
         const unsigned b = __builtin_bit_cast(unsigned, v);

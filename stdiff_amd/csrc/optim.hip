@@ -9,6 +9,8 @@
 // block keeps fp32 precision through its scale, so a block whose elements grow evenly keeps its codes and none stands
 // still under the slow decay of v.  The step itself uses m and v before they are rounded.
 // A block that holds an infinity or a NaN gets a scale that is not finite: all its elements are NaN from the next step on.
+#include <float.h>
+
 #include "common.h"
 
 namespace {
@@ -425,7 +427,8 @@ extern "C" int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream
     update_arg u = {};
     u.scalars = a->workspace;
     u.norm = a->norm;
-    u.max_norm = (float)a->max_norm; u.grad_scale = (float)a->grad_scale; u.lr = (float)a->lr;
+    u.max_norm = a->max_norm > 0.0 ? std::max((float)a->max_norm, FLT_MIN) : 0.f;     // what is positive stays it
+    u.grad_scale = (float)a->grad_scale; u.lr = (float)a->lr;
     u.b1 = (float)a->beta1; u.b2 = (float)a->beta2; u.eps = (float)a->eps;
     u.omb1 = (float)(1.0 - a->beta1);                               // rounded once: 1 - 0.9f is not 0.1f
     u.omb2 = (float)(1.0 - a->beta2);

@@ -550,22 +550,24 @@ def _workspace(t):
 
 
 class AdamWTensors:
-    """Parameters and their states as adamw_multi takes them (made by adamw_multi_args; holds the tensors)."""
+    """Parameters and their states as adamw_multi takes them (made by adamw_multi_args; holds the tensors and their memory)."""
 
     def __init__(self, params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, weight_decay):
         n = len(params)
         none = [None] * n
         decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
-        self.tensors = [list(params), list(exp_avg), list(exp_avg_sq), list(exp_avg_scale or none), list(exp_avg_sq_scale or none)]
-        if any(len(t) != n for t in self.tensors) or len(decay) != n:
+        lists = [list(params), list(exp_avg), list(exp_avg_sq), list(exp_avg_scale or none), list(exp_avg_sq_scale or none)]
+        if any(len(t) != n for t in lists) or len(decay) != n:
             raise ValueError("adamw_multi_args: lists of different lengths")
+        self.params = lists[0]
         self.state_bits = 8 if n and exp_avg[0].dtype == torch.float8_e4m3fn else 32
         kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
         self.table = (L.AdamWTensor * max(n, 1))()
         self.rows = np.frombuffer(self.table, dtype=np.dtype(L.AdamWTensor))[:n]
-        self.device = _one_device(*[t for k in self.tensors for t in k]) if n else None
-        self.sizes = [p.numel() for p in params]
-        for i, (p, m, v, ms, vs, size) in enumerate(zip(*self.tensors, self.sizes)):
+        every = [t for k in lists for t in k if t is not None]
+        self.device = _one_device(*every) if n else None
+        self.sizes, self.addresses = [p.numel() for p in params], [p.data_ptr() for p in params]
+        for i, (p, m, v, ms, vs, size) in enumerate(zip(*lists, self.sizes)):
             if m.dtype != kind or v.dtype != kind:
                 raise TypeError(f"tensor {i}: states are {m.dtype} and {v.dtype}, {kind} is needed like in the first")
             if m.numel() != size or v.numel() != size:
@@ -577,8 +579,12 @@ class AdamWTensors:
             if self.state_bits == 8 and (ms is None or vs is None):
                 raise ValueError("8-bit states need exp_avg_scale and exp_avg_sq_scale")
             blocks = -(-size // 256)
-            self.table[i] = (p.data_ptr(), 0, m.data_ptr(), v.data_ptr(), _vector(ms, "exp_avg_scale", blocks),
+            self.table[i] = (self.addresses[i], 0, m.data_ptr(), v.data_ptr(), _vector(ms, "exp_avg_scale", blocks),
                              _vector(vs, "exp_avg_sq_scale", blocks), size, _code(p.dtype), 0, decay[i], 0)
+        ranges = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in every if t.numel())
+        if any(at + size > after for (at, size), (after, _) in zip(ranges, ranges[1:])):
+            raise ValueError("adamw_multi_args: two of the parameters and states share memory")
+        self.memory = [t.untyped_storage() for t in every]         # alive even where a tensor is given other memory
         self.partial = False                  # the last step left tensors out
         self.half = {p.dtype for p in params} - {torch.float32}
         if len(self.half) > 1:
@@ -618,10 +624,13 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     done so far; incremented.  max_norm: clip by the norm over all gradients (None: no clipping); norm (fp32 [1],
     optional) receives that norm; grad_scale multiplies every gradient first (1 / world size, 1 / loss scale).
     workspace (fp32, at least adamw_multi_workspace(len(grads)) floats; allocated unless given): give one of its own to a
-    call that is captured into an ops.Graph.  A captured step keeps lr and the other numbers it was captured with."""
+    call that is captured into an ops.Graph.  A captured step keeps lr and the other numbers it was captured with, and its
+    replays do not raise the parameters' version counters: torch.autograd.graph.increment_version does."""
     sizes, rows, n = args.sizes, args.rows, len(args.sizes)
     if len(grads) != n:
         raise ValueError(f"adamw_multi: {len(grads)} gradients for {n} parameters")
+    if list(map(_data_ptr, args.params)) != args.addresses:
+        raise ValueError("adamw_multi: a parameter was given other memory since adamw_multi_args")
     dev = args.device if n else step_dev.get_device()
     if _one_device(step_dev, norm, workspace) != dev:
         raise ValueError(f"step_dev on {step_dev.device}, the parameters on device {dev}")
@@ -652,6 +661,8 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     a = L.AdamWMultiArgs(args.table, n, args.state_bits, _vector(step_dev, "step_dev", 1, torch.int32),
                          _vector(norm, "norm", 1), ws, nb, lr, betas[0], betas[1], eps, max_norm or 0.0, grad_scale)
     _enqueue(dev, lib(torch.float16 in kinds).stdiff_adamw_multi, C.byref(a))
+    if n:
+        torch.autograd.graph.increment_version(args.params)        # who keeps copies of them (DiT_stDiff) sees the change
 
 
 _dtype, _numel, _get_device = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.get_device

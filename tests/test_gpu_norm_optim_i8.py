@@ -580,11 +580,22 @@ def test_refusals(ops):
         ops.adamw_multi_args([p], [m.half()], [v])
     with pytest.raises(ValueError):
         ops.adamw_multi_args([p], [m[:7]], [v])
-    c = m.to(torch.float8_e4m3fn)
+    with pytest.raises(ValueError, match="share"):
+        ops.adamw_multi_args([p, p], [m, torch.zeros_like(m)], [v, torch.zeros_like(v)])
+    with pytest.raises(ValueError, match="share"):
+        ops.adamw_multi_args([p], [m], [m])
+    with pytest.raises(ValueError, match="share"):
+        ops.adamw_multi_args([p[:200], p[199:]], [m[:200], torch.zeros(101, device=DEV)], [v[:200], torch.zeros(101, device=DEV)])
+    moved = torch.nn.Parameter(torch.zeros(300, device=DEV))
+    margs = ops.adamw_multi_args([moved], [m], [v])
+    moved.data = torch.ones(300, device=DEV)
+    with pytest.raises(ValueError, match="memory"):
+        ops.adamw_multi(margs, [p], step, 1e-3)
+    c, c2 = m.to(torch.float8_e4m3fn), m.to(torch.float8_e4m3fn)
     with pytest.raises(ValueError):
-        ops.adamw_multi_args([p], [c], [c])
+        ops.adamw_multi_args([p], [c], [c2])
     with pytest.raises(ValueError):
-        ops.adamw_multi_args([p], [c], [c], [torch.zeros(1, device=DEV)], [torch.zeros(2, device=DEV)])
+        ops.adamw_multi_args([p], [c], [c2], [torch.zeros(1, device=DEV)], [torch.zeros(2, device=DEV)])
     q = torch.zeros(4, 32, device=DEV, dtype=torch.int8)
     with pytest.raises(TypeError, match="int8"):
         ops.gemm_i8(x, s4, q, s4)
@@ -656,6 +667,58 @@ def test_projection_is_trained_and_served(ops, bits):
         sy, sw = yf.abs().amax(1, keepdim=True) / 127, wf.abs().amax(1) / 127
         tol = (yf.abs().sum(1, keepdim=True) * sw + sy * wf.abs().sum(1)) * 0.501 + H * sy * sw * 0.251 + want.abs() * 2.0 ** -8
         within(served, want, tol, "served")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_model_is_trained_by_adamw_multi(ops, bits):
+    """The framework's denoiser through its autograd path, its parameters (condi_emb has no gradient) updated by adamw_multi:
+    states as the formulas give them from the same gradients, and a forward that sees the new weights."""
+    from stdiff_amd.model.stDiff_model import DiT_stDiff
+    torch.manual_seed(3)
+    C_, G, H = 24, 40, 128
+    model = DiT_stDiff(G, H, 1, "dit", 4, 6).to(DEV)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(0.02 * torch.randn_like(p))                  # the output and adaLN layers begin with zeros
+    params = list(model.parameters())
+    decay = [0.01 if p.dim() == 2 else 0.0 for p in params]
+    if bits == 8:
+        st = [ops.adamw8_state(p) for p in params]
+    else:
+        st = [(torch.zeros_like(p), torch.zeros_like(p)) for p in params]
+    x, y, t = rnd(C_, G, seed=1).to(DEV), rnd(C_, G, seed=2).to(DEV), torch.arange(C_, device=DEV)
+    states = [[s[k] for s in st] for k in range(len(st[0]))]
+    early = ops.adamw_multi_args(params, *states, weight_decay=decay)
+    model(x, t, y)                                              # the autograd path gathers the parameters in one buffer
+    step, norm = torch.zeros(1, device=DEV, dtype=torch.int32), torch.zeros(1, device=DEV)
+    with pytest.raises(ValueError, match="memory"):
+        ops.adamw_multi(early, [None] * len(params), step, 1e-2)
+    args = ops.adamw_multi_args(params, *states, weight_decay=decay)
+    own = [Oracle(p.detach().cpu(), bits, w, torch.float32) for p, w in zip(params, decay)]
+    for k in range(1, 4):
+        for p in params:
+            p.grad = None
+        before = model(x, t, y)
+        (before ** 2).mean().backward()
+        grads = [p.grad for p in params]
+        assert sum(g is None for g in grads) == 1
+        was = [p.detach().cpu().clone() for p in params]
+        ops.adamw_multi(args, grads, step, 1e-2, norm=norm)
+        total = math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads if g is not None))
+        assert abs(float(norm) - total) < 100 * U * total
+        for p, o, g, w, s in zip(params, own, grads, was, st):
+            if g is None:
+                assert torch.equal(p.detach().cpu(), w)
+                continue
+            o.p = w
+            o.step(g.cpu(), k, 1e-2, 1.0, 0.9, 0.999, 1e-8)
+            assert torch.equal(s[0].cpu().view(-1).view(torch.uint8), o.m.view(torch.uint8))
+            assert torch.equal(s[1].cpu().view(-1).view(torch.uint8), o.v.view(torch.uint8))
+            within(p, o.p, 16 * U * 3e-2 + 3 * U * o.p.double().abs(), "parameter")
+        fresh = DiT_stDiff(G, H, 1, "dit", 4, 6).to(DEV)
+        fresh.load_state_dict(model.state_dict())
+        with torch.no_grad():
+            assert torch.equal(model(x, t, y), fresh(x, t, y)) and not torch.equal(model(x, t, y), before)
 
 
 def test_captured_step_replays(ops):
