@@ -500,6 +500,25 @@ def test_gemm_i8(ops, M, N, K, ct):
         within(y, want, 4 * U * (prod.abs() + want.abs()) + half_step(y) * want.abs() * 1.001 + (2.0 ** -25 if ct == "fp16" else 0), "y")
 
 
+@pytest.mark.parametrize("M,N", [(1600, 1700), (2600, 2500), (3300, 2900), (5000, 4200)])
+@pytest.mark.parametrize("K", [33, 128, 200, 384, 915, 1040])
+def test_gemm_i8_large_outputs(ops, M, N, K):
+    """sizes of the tiled kernels: 128 x 128 tiles; 256 x 256 tiles cut in halves, whole ones, and more than there are CUs with
+    a last round in halves; one slab of K, two, three and many, whole and cut.  What lies beside C is left alone."""
+    A, W, sa, sw, b = [t.to(DEV) for t in operands(M, N, K, seed=M + K)]
+    prod = A[:, :K].double() @ W[:, :K].double().t().contiguous() * sa.double().view(-1, 1) * sw.double()
+    want = prod + b.double()
+    tol = 4 * U * (prod.abs() + want.abs())
+    for ct in (torch.float32, torch.bfloat16):
+        out = torch.full((M + 1, N + 8), 5.0, device=DEV, dtype=ct)
+        y = ops.gemm_i8(A[:, :K], sa, W[:, :K], sw, b, out=out[:M, 3:3 + N])
+        off = (y.double() - want).abs() - tol - half_step(y) * want.abs() * 1.001
+        assert float(off.max()) <= 0, (ct, float(off.max()))
+        assert bool((out[:, :3] == 5).all()) and bool((out[:, 3 + N:] == 5).all()) and bool((out[M] == 5).all())
+        again = ops.gemm_i8(A[:, :K], sa, W[:, :K], sw, b, out_dtype=ct)
+        assert torch.equal(again, y)
+
+
 @pytest.mark.parametrize("M,N,K", [(2, 3, 131071), (200, 300, 131071), (600, 1024, 2048), (1500, 1300, 1000)])
 def test_gemm_i8_sum_is_exact(ops, M, N, K):
     """the largest sums that can be: all operands at -128 / 127; with scales of one, C is the rounded whole number"""
