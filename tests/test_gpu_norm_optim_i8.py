@@ -550,6 +550,57 @@ def test_gemm_i8_strides_and_edges(ops):
     assert z.shape == (0, N)
 
 
+# ---------------------------------------------------------------- sizes whose offsets pass 32 bits
+def test_far_rows(ops):
+    """rows behind the 2^32-th byte (and the 2^31-th element): the same results as the same rows alone"""
+    H, ld = 1001, 40000
+    R = 2 ** 31 // ld + 100                                     # the last rows begin behind element 2^31
+    far = torch.zeros(R, ld, device=DEV, dtype=torch.bfloat16)
+    last = rnd(50, H, seed=110).to(DEV).bfloat16()
+    far[-50:, 7:7 + H] = last
+    x = far[:, 7:7 + H]
+    w, b = rnd(H, seed=111).to(DEV), rnd(H, seed=112).to(DEV)
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    assert torch.equal(ops.layer_norm(x, w, b, mean=mean, rstd=rstd)[-50:], ops.layer_norm(last, w, b))
+    dx, dw, db = ops.layer_norm_bwd(x, x, mean, rstd, w)
+    one = ops.layer_norm_bwd(last, last, mean[-50:].clone(), rstd[-50:].clone(), w)
+    assert torch.equal(dx[-50:], one[0])
+    scale = last.float().pow(2).sum(0) * float(rstd.max()) + 1
+    assert bool(((dw - one[1]).abs() <= 200 * U * scale).all())   # the other rows add zeros: another order of the same terms
+    q, s = ops.quantize_rows(x)
+    q1, s1 = ops.quantize_rows(last)
+    assert torch.equal(q[-50:], q1) and torch.equal(s[-50:], s1)
+    del x, far, dx, q
+    M, K, N = 2 ** 31 // 8192 + 300, 8192, 300
+    A = torch.zeros(M, K, device=DEV, dtype=torch.int8)
+    A[-300:] = torch.randint(-127, 128, (300, K), device=DEV, dtype=torch.int8)
+    W = torch.randint(-127, 128, (N, K), device=DEV, dtype=torch.int8)
+    sa, sw = torch.rand(M, device=DEV), torch.rand(N, device=DEV)
+    y = ops.gemm_i8(A, sa, W, sw)
+    assert torch.equal(y[-300:], ops.gemm_i8(A[-300:], sa[-300:].clone(), W, sw)) and not bool(y[:-300].any())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_multi_far_elements(ops, bits):
+    """a tensor of more than 2^31 elements: its ends as small tensors of their own give them"""
+    n = 2 ** 31 + 5000
+    p, g = torch.zeros(n, device=DEV, dtype=torch.bfloat16), torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    cut = 2 ** 31 - 2048
+    p[cut:], g[cut:] = rnd(n - cut, seed=120).to(DEV).bfloat16(), rnd(n - cut, seed=121).to(DEV).bfloat16()
+    small = p[cut:].clone()
+    if bits == 8:
+        st, own = ops.adamw8_state(p), ops.adamw8_state(small)
+    else:
+        st, own = [tuple(torch.zeros(t.numel(), device=DEV) for _ in range(2)) for t in (p, small)]
+    step = torch.zeros(2, device=DEV, dtype=torch.int32)
+    for t, s, gr, k in ((p, st, g, 0), (small, own, g[cut:].clone(), 1)):
+        args = ops.adamw_multi_args([t], *[[v] for v in s])
+        ops.adamw_multi(args, [gr], step[k:k + 1], 1e-2)
+    assert torch.equal(p[cut:], small) and not bool(p[:cut].any())
+    assert torch.equal(st[0][cut:].view(torch.uint8), own[0].view(torch.uint8))
+    assert torch.equal(st[1][cut:].view(torch.uint8), own[1].view(torch.uint8))
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals(ops):
     x, w = torch.zeros(4, 32, device=DEV), torch.ones(32, device=DEV)
