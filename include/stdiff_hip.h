@@ -509,9 +509,9 @@ int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, const void* wei
  *   dx = rstd * (g - mean g - xhat * mean(g * xhat))   in x's dtype (dx may be dy or x where dtype and leading dimension agree)
  *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy   fp32 [H], either may be NULL; added to what they
  *   hold when accumulate != 0.  The sums are formed in a fixed order (the same bits every run); where there are many rows
- *   from partial sums in `workspace` (16-byte aligned, stdiff_layer_norm_bwd_workspace(R, H) bytes, which may be 0; not
+ *   from partial sums in `workspace` (16-byte aligned, stdiff_layer_norm_bwd_workspace(..) bytes, which may be 0; not
  *   used when both are NULL). */
-long long stdiff_layer_norm_bwd_workspace(int R, int H);
+long long stdiff_layer_norm_bwd_workspace(int R, int H, int x_dtype, int dy_dtype);
 int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const void* x, long long ldx, int x_dtype,
                           const float* mean, const float* rstd, const void* weight, int w_dtype, void* dx, long long lddx,
                           float* dweight, float* dbias, int accumulate, float* workspace, long long workspace_bytes, int R,

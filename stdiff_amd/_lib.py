@@ -189,7 +189,7 @@ _SIGS = {
     "stdiff_dit_backward": (i32, [C.POINTER(TrainWeights), C.POINTER(TrainActs), vp, BucketFn, vp, vp]),
     "stdiff_dit_backward_parts": (C.c_longlong, [C.POINTER(TrainWeights)]),
     "stdiff_layer_norm": (i32, [vp, i64, i32, vp, vp, i32, f32, vp, i64, i32, vp, vp, i32, i32, vp]),
-    "stdiff_layer_norm_bwd_workspace": (C.c_longlong, [i32, i32]),
+    "stdiff_layer_norm_bwd_workspace": (C.c_longlong, [i32, i32, i32, i32]),
     "stdiff_layer_norm_bwd": (i32, [vp, i64, i32, vp, i64, i32, vp, vp, vp, i32, vp, i64, vp, vp, i32, vp, i64, i32, i32, vp]),
     "stdiff_adamw_multi_workspace": (C.c_longlong, [i32]),
     "stdiff_adamw_multi": (i32, [C.POINTER(AdamWMultiArgs), vp]),

@@ -457,15 +457,22 @@ inline bool past_caches(long long bytes) { return bytes > (256ll << 20); }
 inline int lanes_of(int H) { return H <= 128 ? 8 : H <= 512 ? 32 : H <= 1024 ? 64 : BLOCK; }
 inline int threads_of(int H) { return H <= 1024 ? 256 : cdiv(H, 1024) * 64; }
 inline int rows_of_block(int H) { return H <= 1024 ? 256 / lanes_of(H) : 1; }
-// Up to 1024 rows the column sums walk down the rows in the launch that gives dx (512 x 1024 bf16: 4.0 us against 8.3 with partial
-// sums and a second launch; 1024 x 1024 fp32: 7.0 against 8.7; 2048 x 1024 fp32: 22 against 11)
-inline bool one_launch(int R, int H) { return R <= 1024 && H >= 8 && H <= 8192; }
-// Workgroups of the backward: 16 waves per CU for rows of 16 bits, 8 for fp32 rows, which have as many bytes in flight (65536 x 1024
-// bf16: 8 waves 106 us, 16 waves 75; 32768 x 2048 fp32: 139 and 143 us, and twice the partial sums), and two rows at least
-// for each, so that the partial sums stay small beside the rows.
+// Few rows: the column sums walk down the rows in the launch that gives dx.  A workgroup reads 32 columns of all rows, and a CU draws
+// about 45 GB/s from the L2: up to 320 KB cost 7 us, which is what the second launch, the workspace and the partial sums
+// cost (512 x 1024 bf16: 4.0 us against 8.3; 1024 x 1024 fp32: 7.0 against 8.7; 2077 x 1001 fp16: 11.3 against 9.4, but 13.4
+// against 17.5 where the host launches; 2048 x 1024 fp32: 16 against 10).
+inline bool one_launch(int R, int H, int x_size, int dy_size) {
+    return (long long)R * 32 * (x_size + dy_size) <= 320 << 10 && H >= 8 && H <= 8192;
+}
+// Workgroups of the backward, each of which leaves partial sums as large as two fp32 rows: at least six rows for each (4096 x 2048
+// bf16: two 40, six 26 us).  Eight waves per CU; sixteen for rows of 16 bits, which have half the bytes in flight (65536 x
+// 1024 bf16: 106 against 75 us), but where a workgroup has one row at a time only if that leaves sixteen rows for each
+// (16384 x 2048 bf16: eight waves 48, sixteen 60 us; 32768 x 4096: 177 and 163).
 inline int bwd_parts(int R, int H, int size) {
     if (!in_registers(H)) return (int)std::min<long long>(R, 64);
-    return norm_blocks(R, rows_of_block(H) * 2, std::max(1, (size == 2 ? 1024 : 512) / threads_of(H)));
+    const int wide = std::max(1, 1024 / threads_of(H)), narrow = std::max(1, 512 / threads_of(H));
+    const bool many = size == 2 && (H <= 1024 || R >= 16ll * wide * cu_count());
+    return norm_blocks(R, std::max(rows_of_block(H) * 2, 6), many ? wide : narrow);
 }
 inline int ld_parts(int H) { return (H + 3) / 4 * 4; }
 
@@ -512,7 +519,7 @@ int launch_ln_grad(const void* dy, long long lddy, const void* x, long long ldx,
                    hipStream_t st) {
     constexpr int V = sizeof(TX) == 2 ? 8 : 4;
     const int ldp = ld_parts(H), parts = bwd_parts(R, H, sizeof(TX));
-    if (!ws && (dweight || dbias)) {                  // few rows
+    if (one_launch(R, H, sizeof(TX), sizeof(TD)) && (dweight || dbias)) {
         const int cols = cdiv(H, 32), rows = norm_blocks(R, H <= 1024 ? 8 : 1, 4);
         const auto meets = [&](const void* p, long long ld, size_t size) {
             const uintptr_t a = (uintptr_t)p, b = (uintptr_t)dx;
@@ -596,9 +603,10 @@ extern "C" int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, cons
 #undef LN
 }
 
-extern "C" long long stdiff_layer_norm_bwd_workspace(int R, int H) {
-    if (R < 0 || H <= 0) return STDIFF_ERR_ARG;
-    return one_launch(R, H) ? 0 : (long long)bwd_parts(R, H, 2) * 2 * ld_parts(H) * 4;
+extern "C" long long stdiff_layer_norm_bwd_workspace(int R, int H, int x_dtype, int dy_dtype) {
+    if (R < 0 || H <= 0 || !dtype_ok(x_dtype) || !dtype_ok(dy_dtype)) return STDIFF_ERR_ARG;
+    const int size = (int)dtype_size(x_dtype);
+    return one_launch(R, H, size, (int)dtype_size(dy_dtype)) ? 0 : (long long)bwd_parts(R, H, size) * 2 * ld_parts(H) * 4;
 }
 
 extern "C" int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const void* x, long long ldx, int x_dtype,
@@ -620,7 +628,7 @@ extern "C" int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtyp
         }
         return STDIFF_OK;
     }
-    const long long need = params ? stdiff_layer_norm_bwd_workspace(R, H) : 0;
+    const long long need = params ? stdiff_layer_norm_bwd_workspace(R, H, x_dtype, dy_dtype) : 0;
     if (need && (!workspace || workspace_bytes < need)) return STDIFF_ERR_WORKSPACE;
     float* ws = need ? workspace : nullptr;
 #define LN(TX, TD, TW)                                                                                                            \

@@ -492,7 +492,7 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=
     dy or x).  dweight / dbias are fp32 [H]: with a weight both are allocated unless given, without one those that are
     given are formed (else None); accumulate=True adds to what the given ones hold.  They are sums over the rows in a
     fixed order: the same bits every run.
-    workspace (fp32, at least layer_norm_bwd_workspace(R, H) floats, which is none for few rows; allocated unless given):
+    workspace (fp32, at least layer_norm_bwd_workspace(R, H, ..) floats, none for few rows; allocated unless given):
     give one of its own to a call that is captured into an ops.Graph."""
     dev = _one_device(x, dy, mean, rstd, weight, dx, dweight, dbias, workspace)
     ldx = _read_ld(x, "x")
@@ -520,21 +520,22 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=
     if mean is None or rstd is None:
         raise ValueError("mean and rstd of the forward are needed")
     mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
-    xdt, ddt = x.dtype, dy.dtype
-    lb = _lib_of(xdt, ddt, wdt)
+    xdt, ddt = _code(x.dtype), _code(dy.dtype)
+    lb = _lib_of(x.dtype, dy.dtype, wdt)
     if workspace is None and (dweight is not None or dbias is not None):
-        need = lb.stdiff_layer_norm_bwd_workspace(R, H)
+        need = lb.stdiff_layer_norm_bwd_workspace(R, H, xdt, ddt)
         if need > 0:
             workspace = x.new_empty((need // 4,), dtype=torch.float32)
     ws, nb = _workspace(workspace)
-    _enqueue(dev, lb.stdiff_layer_norm_bwd, dy.data_ptr(), lddy, _code(ddt), x.data_ptr(), ldx, _code(xdt), mp, rp, w, _code(wdt),
+    _enqueue(dev, lb.stdiff_layer_norm_bwd, dy.data_ptr(), lddy, ddt, x.data_ptr(), ldx, xdt, mp, rp, w, _code(wdt),
              dx.data_ptr(), lddx, dw, db, int(accumulate), ws, nb, R, H)
     return dx, dweight, dbias
 
 
-def layer_norm_bwd_workspace(R, H):
-    """Floats that layer_norm_bwd needs as workspace for x [R, H]."""
-    n = lib().stdiff_layer_norm_bwd_workspace(R, H)
+def layer_norm_bwd_workspace(R, H, x_dtype, dy_dtype=None):
+    """Floats that layer_norm_bwd needs as workspace for x [R, H] and dy of these types (dy's is x's unless given)."""
+    x_code = _code(x_dtype)
+    n = lib().stdiff_layer_norm_bwd_workspace(R, H, x_code, x_code if dy_dtype is None else _code(dy_dtype))
     if n < 0:
         raise ValueError(f"layer_norm_bwd_workspace: bad size {R} x {H}")
     return n // 4

@@ -30,9 +30,10 @@ def test_layer_norm_refuses(lib):
 
 
 def test_layer_norm_bwd_refuses(lib):
-    need = lib.stdiff_layer_norm_bwd_workspace(9000, 1001)
-    assert need > 0 and lib.stdiff_layer_norm_bwd_workspace(-1, 5) == ARG and lib.stdiff_layer_norm_bwd_workspace(5, 0) == ARG
-    assert lib.stdiff_layer_norm_bwd_workspace(0, 5) >= 0 and lib.stdiff_layer_norm_bwd_workspace(10, 5) >= 0
+    need = lib.stdiff_layer_norm_bwd_workspace(9000, 1001, 0, 0)
+    for bad in ((-1, 5, 0, 0), (5, 0, 0, 0), (5, 5, 2, 0), (5, 5, 1, -1)):
+        assert lib.stdiff_layer_norm_bwd_workspace(*bad) == ARG
+    assert need > 0 and lib.stdiff_layer_norm_bwd_workspace(0, 5, 1, 1) >= 0 and lib.stdiff_layer_norm_bwd_workspace(10, 5, 0, 1) >= 0
 
     def bwd(dy=AT, ldd=1001, dd=0, x=AT, ldx=1001, xd=0, mean=AT, rstd=AT, w=AT, wd=0, dx=AT, lddx=1001, dw=AT, db=AT, ws=AT, nb=need, R=9000, H=1001):
         return lib.stdiff_layer_norm_bwd(dy, ldd, dd, x, ldx, xd, mean, rstd, w, wd, dx, lddx, dw, db, 0, ws, nb, R, H, None)

@@ -168,7 +168,7 @@ def test_layer_norm_bwd_options(ops, R, H):
     assert plain[1] is None and plain[2] is None
     within(plain[0], grad64(dy.cpu(), x.cpu(), mean.cpu(), rstd.cpu(), None)[0], grad_tol(dy.cpu(), rstd.cpu(), hat, dy.cpu().double())[0] + U, "no weight")
     # in place of dy and of x, with a workspace of its own
-    ws = torch.full((ops.layer_norm_bwd_workspace(R, H),), float("nan"), device=DEV)
+    ws = torch.full((ops.layer_norm_bwd_workspace(R, H, torch.float32),), float("nan"), device=DEV)
     for which in ("dy", "x"):
         a, c = dy.clone(), x.clone()
         got = ops.layer_norm_bwd(a, c, mean, rstd, w, dx=a if which == "dy" else c, workspace=ws)
@@ -795,7 +795,7 @@ def test_captured_step_replays(ops):
     """layer_norm, its backward and the optimizer in one ops.Graph with workspaces of their own, the program's own eager work
     between the replays: every replay gives what the eager calls give on the same data."""
     R, H = 70, 200
-    ws = [torch.empty(ops.layer_norm_bwd_workspace(R, H), device=DEV), torch.empty(ops.adamw_multi_workspace(2), device=DEV)]
+    ws = [torch.empty(ops.layer_norm_bwd_workspace(R, H, torch.float32), device=DEV), torch.empty(ops.adamw_multi_workspace(2), device=DEV)]
     x, dy = torch.empty(R, H, device=DEV), torch.empty(R, H, device=DEV)
     y, dx = torch.empty_like(x), torch.empty_like(x)
     mean, rstd, dw, db, norm = (torch.empty(n, device=DEV) for n in (R, R, H, H, 1))
