@@ -470,7 +470,8 @@ inline bool one_launch(int R, int H, int x_size, int dy_size) {
 // (16384 x 2048 bf16: eight waves 48, sixteen 60 us; 32768 x 4096: 177 and 163).
 inline int bwd_parts(int R, int H, int size) {
     if (!in_registers(H)) return (int)std::min<long long>(R, 64);
-    const int wide = std::max(1, 1024 / threads_of(H)), narrow = std::max(1, 512 / threads_of(H));
+    const int waves = threads_of(H) / 64, places = waves > 4 ? (waves + 3) / 4 * 4 : waves;     // the same number on all four SIMDs
+    const int wide = std::max(1, 16 / places), narrow = std::max(1, 8 / places);
     const bool many = size == 2 && (H <= 1024 || R >= 16ll * wide * cu_count());
     return norm_blocks(R, std::max(rows_of_block(H) * 2, 6), many ? wide : narrow);
 }
