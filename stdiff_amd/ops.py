@@ -1,13 +1,16 @@
 """Tensor-level wrappers over the C ABI (one function per entry point of include/stdiff_hip.h).
 Tensors must live on the GPU; outputs are allocated with torch when not supplied."""
 import ctypes as C
-import operator
 
-import numpy as np
 import torch
 
 from . import _lib as L
 from ._lib import F32, check, dt_of, lib, lib_for, ptr, require_gpu, stream
+
+try:
+    from . import _bind
+except ImportError as e:
+    raise RuntimeError("stdiff_amd/_bind.so was not built (make -C stdiff_amd/csrc) or does not fit this torch") from e
 
 
 def round_up(a, b):
@@ -382,221 +385,63 @@ def clip_adamw(p, g, m, v, sumsq, step_dev, scal, lr, max_norm=1.0, grad_scale=1
 
 
 # ---------------------------------------------------------------- norm, optimizer and 8-bit product beside the DiT
-def _one_device(first, *rest):
-    """Index of the device that all of these tensors are on (None entries are skipped)."""
-    dev = first.get_device()
-    for t in rest:
-        if t is not None and t.get_device() != dev:
-            require_gpu(first, t)
-            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
-    if dev < 0:
-        require_gpu(first)
-    return dev
+# (checked and called by the extension module stdiff_amd/_bind.so, csrc/bind.cpp: small calls cost less than through ctypes)
+def _entries(fp16):
+    """Addresses of the C ABI's entry points that _bind calls."""
+    names = ("layer_norm", "layer_norm_bwd_workspace", "layer_norm_bwd", "adamw_multi_workspace", "adamw_multi", "quantize_rows",
+             "gemm_i8", "error_string")
+    return tuple(C.cast(getattr(lib(bool(fp16)), "stdiff_" + n), C.c_void_p).value for n in names)
 
 
-_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-
-
-def _enqueue(dev, fn, *args):
-    """check(fn(*args, stream)) with the stream that is current on device `dev`, `dev` being the current device meanwhile."""
-    if dev == _current_device():
-        rc = fn(*args, _current_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _current_stream(dev))
-    if rc:
-        check(rc)
-
-
-def _lib_of(*dtypes):
-    """lib_for by dtype."""
-    if torch.float16 in dtypes:
-        if torch.bfloat16 in dtypes:
-            raise TypeError("float16 and bfloat16 tensors in one stdiff_hip call")
-        return lib(True)
-    return lib()
-
-
-def _read_ld(t, name, shape=None):
-    """Leading dimension of a matrix that is only read: rows may overlap or be one row broadcast."""
-    size = t.shape
-    if len(size) != 2 or (shape is not None and size != shape):
-        raise ValueError(f"{name}: a matrix{'' if shape is None else f' of {tuple(shape)}'} is needed, got {tuple(size)}")
-    ld, one = t.stride()
-    if one != 1 and size[1] > 1:
-        raise ValueError(f"{name}: the elements of a row have to be neighbours, got strides {t.stride()}")
-    return ld if size[0] > 1 else size[1]
-
-
-def _write_ld(t, name, shape):
-    ld = _read_ld(t, name, shape)
-    if ld < t.shape[1]:
-        raise ValueError(f"{name}: rows of an output may not overlap, got strides {t.stride()}")
-    return ld
-
-
-def _vector(t, name, n, dtype=torch.float32):
-    """None, or the address of a contiguous vector of n elements of this type (or of one of these)."""
-    if t is None:
-        return None
-    kind = t.dtype
-    if t.numel() != n or (t.stride() != (1,) and not (t.dim() == 1 and n <= 1)) or \
-            not (kind is dtype or (dtype is _FLOATS and kind in _FLOATS)):
-        raise ValueError(f"{name}: a contiguous vector of {n} elements of {dtype} is needed, got {tuple(t.shape)} {kind}")
-    return t.data_ptr()
-
-
-_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
-
-
-def _affine(weight, bias, H):
-    """(address, address, dtype) of a norm's weight and bias, which share one dtype."""
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: one dtype is needed")
-    one = weight if weight is not None else bias
-    return _vector(weight, "weight", H, _FLOATS), _vector(bias, "bias", H, _FLOATS), torch.float32 if one is None else one.dtype
-
-
-def _code(dtype):
-    """The C ABI's code of a torch dtype (dt_of by dtype)."""
-    if dtype is torch.float32:
-        return F32
-    if dtype is torch.bfloat16 or dtype is torch.float16:
-        return L.BF16
-    raise TypeError(f"unsupported dtype {dtype}")
+_bind.setup(_entries, L.StdiffError)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, mean=None, rstd=None):
     """LayerNorm of the rows of x [R, H] with a weight and a bias per column (None: 1 and 0; one dtype for both).
     x and out: fp32 or a 16-bit type, any row stride, any H.  mean / rstd (fp32 [R], optional): receive the statistics
     that layer_norm_bwd takes.  out may be x."""
-    dev = _one_device(x, weight, bias, out, mean, rstd)
-    ldx = _read_ld(x, "x")
-    R, H = x.shape
-    if out is None:
-        out, ldy = x.new_empty((R, H), dtype=out_dtype), H
-    else:
-        ldy = _write_ld(out, "out", x.shape)
-    w, b, wdt = _affine(weight, bias, H)
-    mp = rp = None
-    if mean is not None or rstd is not None:
-        mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
-    xdt, ydt = x.dtype, out.dtype
-    _enqueue(dev, _lib_of(xdt, ydt, wdt).stdiff_layer_norm, x.data_ptr(), ldx, _code(xdt), w, b, _code(wdt), eps, out.data_ptr(), ldy,
-             _code(ydt), mp, rp, R, H)
-    return out
+    return _bind.layer_norm(x, weight, bias, eps, out, out_dtype, mean, rstd)
 
 
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None, accumulate=False, workspace=None):
     """Backward of layer_norm from its mean / rstd: (dx, dweight, dbias).  dx has x's dtype (allocated unless given; it may be
     dy or x).  dweight / dbias are fp32 [H]: with a weight both are allocated unless given, without one those that are
     given are formed (else None); accumulate=True adds to what the given ones hold.  They are sums over the rows in a
-    fixed order: the same bits every run.
+    fixed order: the same bits every run.  dy may be one row for all rows (an expanded tensor).
     workspace (fp32, at least layer_norm_bwd_workspace(R, H, ..) floats, none for few rows; allocated unless given):
     give one of its own to a call that is captured into an ops.Graph."""
-    dev = _one_device(x, dy, mean, rstd, weight, dx, dweight, dbias, workspace)
-    ldx = _read_ld(x, "x")
-    R, H = x.shape
-    lddy = _read_ld(dy, "dy", x.shape)
-    if accumulate and (dweight is None and dbias is None):
-        raise ValueError("accumulate: there is no dweight or dbias to add to")
-    if dx is None:
-        dx, lddx = x.new_empty((R, H)), H
-    elif dx.dtype != x.dtype:
-        raise TypeError(f"dx is {dx.dtype}, x {x.dtype}")
-    else:
-        lddx = _write_ld(dx, "dx", x.shape)
-    dw, db = _vector(dweight, "dweight", H), _vector(dbias, "dbias", H)
-    w, wdt = None, torch.float32
-    if weight is not None:
-        w, wdt = _vector(weight, "weight", H, _FLOATS), weight.dtype
-        if not accumulate:
-            if dweight is None:
-                dweight = x.new_empty((H,), dtype=torch.float32)
-                dw = dweight.data_ptr()
-            if dbias is None:
-                dbias = x.new_empty((H,), dtype=torch.float32)
-                db = dbias.data_ptr()
-    if mean is None or rstd is None:
-        raise ValueError("mean and rstd of the forward are needed")
-    mp, rp = _vector(mean, "mean", R), _vector(rstd, "rstd", R)
-    xdt, ddt = _code(x.dtype), _code(dy.dtype)
-    lb = _lib_of(x.dtype, dy.dtype, wdt)
-    if workspace is None and (dweight is not None or dbias is not None):
-        need = lb.stdiff_layer_norm_bwd_workspace(R, H, xdt, ddt)
-        if need > 0:
-            workspace = x.new_empty((need // 4,), dtype=torch.float32)
-    ws, nb = _workspace(workspace)
-    _enqueue(dev, lb.stdiff_layer_norm_bwd, dy.data_ptr(), lddy, ddt, x.data_ptr(), ldx, xdt, mp, rp, w, _code(wdt),
-             dx.data_ptr(), lddx, dw, db, int(accumulate), ws, nb, R, H)
-    return dx, dweight, dbias
+    return _bind.layer_norm_bwd(dy, x, mean, rstd, weight, dx, dweight, dbias, accumulate, workspace)
 
 
 def layer_norm_bwd_workspace(R, H, x_dtype, dy_dtype=None):
     """Floats that layer_norm_bwd needs as workspace for x [R, H] and dy of these types (dy's is x's unless given)."""
-    x_code = _code(x_dtype)
-    n = lib().stdiff_layer_norm_bwd_workspace(R, H, x_code, x_code if dy_dtype is None else _code(dy_dtype))
+    codes = []
+    for t in (x_dtype, dy_dtype or x_dtype):
+        if t not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError(f"unsupported dtype {t}")
+        codes.append(F32 if t == torch.float32 else L.BF16)
+    n = lib().stdiff_layer_norm_bwd_workspace(R, H, *codes)
     if n < 0:
         raise ValueError(f"layer_norm_bwd_workspace: bad size {R} x {H}")
     return n // 4
-
-
-def _workspace(t):
-    """(address, bytes) of a workspace tensor (None: none)."""
-    if t is None:
-        return None, 0
-    if not t.is_contiguous():
-        raise ValueError("workspace: a contiguous tensor is needed")
-    return t.data_ptr(), t.numel() * t.element_size()
 
 
 class AdamWTensors:
     """Parameters and their states as adamw_multi takes them (made by adamw_multi_args; holds the tensors and their memory)."""
 
     def __init__(self, params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, weight_decay):
-        n = len(params)
-        none = [None] * n
-        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
-        lists = [list(params), list(exp_avg), list(exp_avg_sq), list(exp_avg_scale or none), list(exp_avg_sq_scale or none)]
-        if any(len(t) != n for t in lists) or len(decay) != n:
-            raise ValueError("adamw_multi_args: lists of different lengths")
-        self.params = lists[0]
-        self.state_bits = 8 if n and exp_avg[0].dtype == torch.float8_e4m3fn else 32
-        kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
-        self.table = (L.AdamWTensor * max(n, 1))()
-        self.rows = np.frombuffer(self.table, dtype=np.dtype(L.AdamWTensor))[:n]
-        every = [t for k in lists for t in k if t is not None]
-        self.device = _one_device(*every) if n else None
-        self.sizes, self.addresses = [p.numel() for p in params], [p.data_ptr() for p in params]
-        for i, (p, m, v, ms, vs, size) in enumerate(zip(*lists, self.sizes)):
-            if m.dtype != kind or v.dtype != kind:
-                raise TypeError(f"tensor {i}: states are {m.dtype} and {v.dtype}, {kind} is needed like in the first")
-            if m.numel() != size or v.numel() != size:
-                raise ValueError(f"tensor {i}: states of {m.numel()} and {v.numel()} elements for {size} parameters")
-            if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-                raise ValueError(f"tensor {i}: the parameter or a state of it is not contiguous")
-            if self.state_bits == 32 and (ms is not None or vs is not None):
-                raise ValueError("32-bit states have no scales")
-            if self.state_bits == 8 and (ms is None or vs is None):
-                raise ValueError("8-bit states need exp_avg_scale and exp_avg_sq_scale")
-            blocks = -(-size // 256)
-            self.table[i] = (self.addresses[i], 0, m.data_ptr(), v.data_ptr(), _vector(ms, "exp_avg_scale", blocks),
-                             _vector(vs, "exp_avg_sq_scale", blocks), size, _code(p.dtype), 0, decay[i], 0)
-        ranges = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in every if t.numel())
-        if any(at + size > after for (at, size), (after, _) in zip(ranges, ranges[1:])):
-            raise ValueError("adamw_multi_args: two of the parameters and states share memory")
-        self.memory = [t.untyped_storage() for t in every]         # alive even where a tensor is given other memory
-        self.partial = False                  # the last step left tensors out
-        self.half = {p.dtype for p in params} - {torch.float32}
-        if len(self.half) > 1:
-            raise TypeError("float16 and bfloat16 parameters in one adamw_multi")
+        self.params = list(params)
+        none = [None] * len(self.params)
+        decay = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(self.params)
+        self.table = _bind.adamw_table(self.params, exp_avg, exp_avg_sq, exp_avg_scale or none, exp_avg_sq_scale or none, decay)
 
 
 def adamw_multi_args(params, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq_scale=None, weight_decay=0.0):
     """What adamw_multi updates: lists of contiguous tensors, one entry per parameter (fp32 or one 16-bit type; views into
-    larger buffers are fine).  exp_avg / exp_avg_sq: fp32, or torch.float8_e4m3fn with a vector of
-    ceil(numel / 256) fp32 scales per tensor in exp_avg_scale / exp_avg_sq_scale (adamw8_state makes all four).
-    weight_decay: one number, or one per tensor.  The states are read and written in place by every step."""
+    larger buffers are fine, no two may share memory).  exp_avg / exp_avg_sq: fp32, or torch.float8_e4m3fn with a vector
+    of ceil(numel / 256) fp32 scales per tensor in exp_avg_scale / exp_avg_sq_scale (adamw8_state makes all four).
+    weight_decay: one number, or one per tensor.  The states are read and written in place by every step.  A model whose
+    parameters move to other memory (.to(), a DiT_stDiff at its first forward under autograd) needs new args."""
     return AdamWTensors(params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, weight_decay)
 
 
@@ -627,116 +472,21 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     workspace (fp32, at least adamw_multi_workspace(len(grads)) floats; allocated unless given): give one of its own to a
     call that is captured into an ops.Graph.  A captured step keeps lr and the other numbers it was captured with, and its
     replays do not raise the parameters' version counters: torch.autograd.graph.increment_version does."""
-    sizes, rows, n = args.sizes, args.rows, len(args.sizes)
-    if len(grads) != n:
-        raise ValueError(f"adamw_multi: {len(grads)} gradients for {n} parameters")
-    if list(map(_data_ptr, args.params)) != args.addresses:
-        raise ValueError("adamw_multi: a parameter was given other memory since adamw_multi_args")
-    dev = args.device if n else step_dev.get_device()
-    if _one_device(step_dev, norm, workspace) != dev:
-        raise ValueError(f"step_dev on {step_dev.device}, the parameters on device {dev}")
-    try:
-        kinds = set(map(_dtype, grads))
-    except AttributeError:
-        kinds = None                           # some are missing
-    if kinds is not None and len(kinds) == 1:
-        if args.partial:
-            args.partial, rows["n"] = False, sizes
-        _gradients(grads, sizes, dev, kinds, rows)
-    else:
-        args.partial, rows["n"] = True, 0
-        kinds = set()
-        for i, g in enumerate(grads):
-            if g is not None:
-                _gradients([g], [sizes[i]], dev, {g.dtype}, rows[i:i + 1])
-                rows["n"][i] = sizes[i]
-                kinds.add(g.dtype)
-    kinds = (kinds | args.half) - {torch.float32}
-    if len(kinds) > 1:
-        raise TypeError("float16 and bfloat16 tensors in one adamw_multi")
-    if max_norm is not None and not max_norm > 0:
-        raise ValueError(f"max_norm has to be positive (or None), got {max_norm}")
-    if workspace is None:
-        workspace = step_dev.new_empty((adamw_multi_workspace(n),), dtype=torch.float32)
-    ws, nb = _workspace(workspace)
-    a = L.AdamWMultiArgs(args.table, n, args.state_bits, _vector(step_dev, "step_dev", 1, torch.int32),
-                         _vector(norm, "norm", 1), ws, nb, lr, betas[0], betas[1], eps, max_norm or 0.0, grad_scale)
-    _enqueue(dev, lib(torch.float16 in kinds).stdiff_adamw_multi, C.byref(a))
-    if n:
-        torch.autograd.graph.increment_version(args.params)        # who keeps copies of them (DiT_stDiff) sees the change
-
-
-_dtype, _numel, _get_device = operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.get_device
-_is_contiguous, _data_ptr = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
-
-
-def _gradients(grads, sizes, dev, kind, rows):
-    """Checks gradients of one dtype and enters them into their rows of the table."""
-    if list(map(_numel, grads)) != sizes or set(map(_get_device, grads)) != {dev} or not all(map(_is_contiguous, grads)):
-        raise ValueError(f"adamw_multi: contiguous gradients of the parameters' {sizes if len(sizes) < 9 else 'sizes'} elements on device "
-                         f"{dev} are needed")
-    rows["grad"] = list(map(_data_ptr, grads))
-    for dtype in kind:
-        rows["grad_dtype"] = _code(dtype)
+    _bind.adamw_multi(args.table, args.params, grads, step_dev, lr, max_norm, grad_scale, betas[0], betas[1], eps, norm, workspace)
 
 
 def quantize_rows(x, out=None, scale=None):
     """(q, scale): the rows of x [R, K] (fp32 or a 16-bit type) as int8 with one fp32 scale each, scale = max |x| / 127 and
     q = rint(x * (127 / max |x|)).  q is a [R, K] view of rows that begin on 16-byte borders, zeros behind K, as gemm_i8
-    takes them (a given `out` has to be such a view).  A row that holds an infinity or a NaN gets a scale that is not
-    finite."""
-    dev = _one_device(x, out, scale)
-    ldx = _read_ld(x, "x")
-    R, K = x.shape
-    if out is None:
-        ldq = round_up(K, 16)
-        out = x.new_empty((R, ldq), dtype=torch.int8)
-        if ldq != K:
-            out = out[:, :K]
-    else:
-        ldq = _rows16(out, "out", (R, K))
-    if scale is None:
-        scale = x.new_empty((R,), dtype=torch.float32)
-    sp = _vector(scale, "scale", R)
-    _enqueue(dev, _lib_of(x.dtype).stdiff_quantize_rows, x.data_ptr(), ldx, _code(x.dtype), out.data_ptr(), ldq, sp, R, K)
-    return out, scale
-
-
-def _rows16(t, name, shape=None):
-    """Leading dimension of an int8 matrix whose rows begin on 16-byte borders and may be touched up to the next border."""
-    if t.dtype is not torch.int8:
-        raise TypeError(f"{name}: int8 is needed, got {t.dtype}")
-    ld = _read_ld(t, name, shape)
-    rows, k = t.shape
-    kp = (k + 15) & ~15
-    if rows == 1:
-        ld = kp
-    if (ld & 15 or ld < kp or t.data_ptr() & 15 or
-            (kp > k and t.storage_offset() + (rows - 1) * ld + kp > t.untyped_storage().nbytes())) and rows:
-        raise ValueError(f"{name}: rows have to begin on 16-byte borders and to reach the next border behind their end in memory, "
-                         f"as quantize_rows lays them out; got shape {tuple(t.shape)}, strides {t.stride()}")
-    return ld
+    takes them (a given `out` has to be such a view, and its rows are written up to the next border).  A row that holds an
+    infinity or a NaN gets a scale that is not finite."""
+    return _bind.quantize_rows(x, out, scale)
 
 
 def gemm_i8(A, a_scale, W, w_scale, bias=None, out=None, out_dtype=torch.float32):
-    """out[M, N] = (A[M, K] @ W[N, K]^T) * a_scale[M, None] * w_scale[N] + bias: int8 operands as quantize_rows makes them,
+    """out[M, N] = (A[M, K] @ W[N, K]^T) * w_scale[N] * a_scale[M, None] + bias: int8 operands as quantize_rows makes them,
     the sum over K exact in int32 (K <= 131071), scales and bias fp32, out fp32 or a 16-bit type."""
-    dev = _one_device(A, a_scale, W, w_scale, bias, out)
-    lda, ldw = _rows16(A, "A"), _rows16(W, "W")
-    (M, K), N = A.shape, W.shape[0]
-    if W.shape[1] != K:
-        raise ValueError(f"A has {K} columns, W {W.shape[1]}")
-    if a_scale is None or w_scale is None:
-        raise ValueError("a_scale and w_scale are needed")
-    if out is None:
-        out, ldc = a_scale.new_empty((M, N), dtype=out_dtype), N
-    else:
-        ldc = _write_ld(out, "out", (M, N))
-    a = L.GemmI8Args(M, N, K, A.data_ptr(), lda, W.data_ptr(), ldw, _vector(a_scale, "a_scale", M),
-                     _vector(w_scale, "w_scale", N), _vector(bias, "bias", N), out.data_ptr(), ldc,
-                     _code(out.dtype))
-    _enqueue(dev, _lib_of(out.dtype).stdiff_gemm_i8, C.byref(a))
-    return out
+    return _bind.gemm_i8(A, a_scale, W, w_scale, bias, out, out_dtype)
 
 
 class Graph:

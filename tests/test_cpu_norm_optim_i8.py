@@ -130,32 +130,59 @@ def test_structs_match_the_header(tmp_path):
     assert got == want
 
 
-def test_python_checks():
+def test_tensors_are_checked_first():
+    """what is wrong with the tensors themselves is refused without a GPU too, with the argument's name"""
     from stdiff_amd import ops
-    t = torch.zeros(4, 6)
-    assert ops._read_ld(t, "t") == 6 and ops._read_ld(t[:, 1:4], "t") == 6 and ops._read_ld(t[:1].expand(3, 6), "t") == 0
-    assert ops._read_ld(torch.zeros(1, 6).expand(1, 6), "t") == 6
-    for bad in (t.t(), t[:, ::2], t[0], t[None]):
-        with pytest.raises(ValueError):
-            ops._read_ld(bad, "t")
-    with pytest.raises(ValueError, match="overlap"):
-        ops._write_ld(t[:1].expand(3, 6), "t", (3, 6))
-    with pytest.raises(ValueError):
-        ops._write_ld(t, "t", (4, 5))
-    assert ops._vector(None, "v", 3, torch.float32) is None
-    for bad in (torch.zeros(2), torch.zeros(6)[::2], torch.zeros(3, 1), torch.zeros(3).double()):
-        with pytest.raises(ValueError):
-            ops._vector(bad, "v", 3, torch.float32)
+    x, w, s4 = torch.zeros(4, 32), torch.ones(32), torch.zeros(4)
+
+    def refused(kind, match, call):
+        with pytest.raises(kind, match=match):
+            call()
+    for bad in (x.t(), x[:, ::2], x[0], x[None]):
+        refused(ValueError, "x:", lambda: ops.layer_norm(bad))
+    for bad in (torch.ones(31), torch.ones(64)[::2], torch.ones(32, 1), torch.ones(32).double(), torch.ones(32).int()):
+        refused(ValueError, "weight:", lambda: ops.layer_norm(x, bad))
+    refused(TypeError, "one dtype", lambda: ops.layer_norm(x, w, w.bfloat16()))
+    refused(TypeError, "float16 and bfloat16", lambda: ops.layer_norm(x.half(), w.bfloat16()))
+    refused(TypeError, "dtype", lambda: ops.layer_norm(x.double()))
+    refused(TypeError, "dtype", lambda: ops.layer_norm(x, out_dtype=torch.int32))
+    refused(TypeError, "tensor", lambda: ops.layer_norm([1.0]))
+    refused(TypeError, "torch.dtype", lambda: ops.layer_norm(x, out_dtype="fp32"))
+    refused(TypeError, "real number", lambda: ops.layer_norm(x, eps="small"))
+    refused(ValueError, "overlap", lambda: ops.layer_norm(x, out=torch.zeros(32).expand(4, 32)))
+    refused(ValueError, "out:", lambda: ops.layer_norm(x, out=torch.zeros(4, 31)))
+    refused(ValueError, "mean", lambda: ops.layer_norm(x, mean=torch.zeros(5)))
+    refused(ValueError, "mean and rstd", lambda: ops.layer_norm_bwd(x, x, s4, None))
+    refused(ValueError, "dy:", lambda: ops.layer_norm_bwd(x[:3], x, s4, s4))
+    refused(ValueError, "accumulate", lambda: ops.layer_norm_bwd(x, x, s4, s4, w, accumulate=True))
+    refused(ValueError, "dweight", lambda: ops.layer_norm_bwd(x, x, s4, s4, w, dweight=w.bfloat16()))
+    refused(TypeError, "dx is", lambda: ops.layer_norm_bwd(x, x, s4, s4, w, dx=x.bfloat16()))
+    refused(ValueError, "workspace", lambda: ops.layer_norm_bwd(x, x, s4, s4, w, workspace=torch.zeros(8, 8).t()))
     q = torch.zeros(5, 48, dtype=torch.int8)
-    base = q.data_ptr() % 16
-    if base == 0:
-        assert ops._rows16(q, "q") == 48 and ops._rows16(q[:, :40], "q") == 48 and ops._rows16(q[:1, :3], "q") == 16
-        assert ops._rows16(q[4:, 32:40], "q") == 16
+    assert q.data_ptr() % 16 == 0
+    ones = torch.ones(5)
     for bad in (q[:, 1:20], torch.zeros(5, 40, dtype=torch.int8), torch.zeros(4 * 48 + 40, dtype=torch.int8).as_strided((5, 40), (48, 1))):
-        with pytest.raises(ValueError, match="borders"):
-            ops._rows16(bad, "q")
-    with pytest.raises(TypeError):
-        ops._rows16(q.float(), "q")
+        refused(ValueError, "A: rows", lambda: ops.gemm_i8(bad, ones, q, ones))
+        refused(ValueError, "out: rows", lambda: ops.quantize_rows(torch.zeros(bad.shape), out=bad))
+    for good in (q, q[:, :40], q[:1, :3], q[4:, 32:40]):
+        n = torch.ones(good.shape[0])
+        refused(RuntimeError, "MI355X", lambda: ops.gemm_i8(good, n, good, n))
+    refused(TypeError, "W: int8", lambda: ops.gemm_i8(q, ones, q.float(), ones))
+    refused(ValueError, "columns", lambda: ops.gemm_i8(q, ones, q[:, :16], ones))
+    refused(ValueError, "w_scale", lambda: ops.gemm_i8(q, ones, q, torch.ones(4)))
+    refused(ValueError, "are needed", lambda: ops.gemm_i8(q, None, q, ones))
+    refused(ValueError, "out:", lambda: ops.gemm_i8(q, ones, q, ones, out=torch.zeros(5, 6)))
+    p, m, v = (torch.zeros(300) for _ in range(3))
+    refused(ValueError, "lengths", lambda: ops.adamw_multi_args([p], [m], []))
+    refused(ValueError, "lengths", lambda: ops.adamw_multi_args([p], [m], [v], weight_decay=[0.0, 1.0]))
+    refused(TypeError, "states are", lambda: ops.adamw_multi_args([p], [m.half()], [v]))
+    refused(ValueError, "states of", lambda: ops.adamw_multi_args([p], [m[:7]], [v]))
+    refused(ValueError, "contiguous", lambda: ops.adamw_multi_args([torch.zeros(600)[::2]], [m], [v]))
+    refused(ValueError, "scales", lambda: ops.adamw_multi_args([p], [m], [v], [ones], [ones]))
+    refused(TypeError, "float16 and bfloat16", lambda: ops.adamw_multi_args([p.half(), p.bfloat16()], [m, m.clone()], [v, v.clone()]))
+    c = [torch.zeros(300).to(torch.float8_e4m3fn) for _ in range(2)]
+    refused(ValueError, "8-bit", lambda: ops.adamw_multi_args([p], c[:1], c[1:]))
+    refused(ValueError, "exp_avg_scale", lambda: ops.adamw_multi_args([p], c[:1], c[1:], [torch.zeros(1)], [torch.zeros(2)]))
 
 
 def test_no_cpu_path():
