@@ -502,7 +502,7 @@ int stdiff_dit_backward(const stdiff_train_weights* w, const stdiff_train_acts* 
  * LayerNorm over rows of H with a weight and a bias per column (either may be NULL: 1 and 0; both have w_dtype):
  *   mean = mean x, rstd = 1 / sqrt(mean (x - mean)^2 + eps), y = (x - mean) * rstd * weight + bias
  * statistics in fp32 from the centred row; mean / rstd (fp32 [R], either may be NULL) are kept for the backward.
- * y may be x (same dtype and leading dimension). */
+ * y may be x (same dtype and leading dimension); else they share no element.  H > 2^30: STDIFF_ERR_SHAPE. */
 int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, const void* weight, const void* bias, int w_dtype, float eps,
                       void* y, long long ldy, int y_dtype, float* mean, float* rstd, int R, int H, void* stream);
 /* Its backward from the forward's statistics:  xhat = (x - mean) * rstd, g = dy * weight,
@@ -525,7 +525,7 @@ int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const vo
  * code; all zeros is the state before the first step.  A block that holds an infinity or a NaN is NaN from the next step on.
  * step_dev: int32 [1], the steps done before this call; incremented by it.  max_norm <= 0: no clipping.  norm (may be
  * NULL): receives the norm.  A norm that is NaN makes every parameter NaN.  The `tensors` array is read during the call
- * only; the tensors must not overlap.  workspace: stdiff_adamw_multi_workspace(n_tensors) bytes, 4-byte aligned. */
+ * only; the tensors must not overlap; weight_decay >= 0.  workspace: stdiff_adamw_multi_workspace(n_tensors) bytes, 4-byte aligned. */
 typedef struct {
     void* param; const void* grad; void* exp_avg; void* exp_avg_sq; float* exp_avg_scale; float* exp_avg_sq_scale;
     long long n; int param_dtype; int grad_dtype; float weight_decay; int reserved;

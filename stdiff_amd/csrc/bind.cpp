@@ -127,6 +127,27 @@ int64_t rows16(const Tensor& t, const char* name) {
     return ld;
 }
 
+// Outputs share no memory with what a call reads, but where an operator may work in place: then they are the same elements.
+// (Side by side in the rows of one buffer they are apart.)
+void keep_apart(const Tensor& out, const char* name, int64_t ldo, const Tensor& in, const char* other, int64_t ldi, bool in_place) {
+    if (!out.numel() || !in.numel()) return;
+    const int64_t rows = out.size(0), so = out.element_size(), si = in.element_size();
+    const uintptr_t p = (uintptr_t)out.data_ptr(), q = (uintptr_t)in.data_ptr();
+    const int64_t lp = ldo * so, lq = ldi * si, wp = out.size(1) * so, wq = in.size(1) * si;
+    if (p + (rows - 1) * lp + wp <= q || q + (in.size(0) - 1) * lq + wq <= p) return;
+    if (in_place && p == q && lp == lq && out.scalar_type() == in.scalar_type()) return;
+    if (lp == lq) {
+        const int64_t off = (int64_t)(q - p) % lp, d = off < 0 ? off + lp : off;
+        if (d >= wp && d + wq <= lp) return;
+    }
+    refuse(PyExc_ValueError, name, " and ", other, " share memory", in_place ? " and are not the same elements" : "");
+}
+void keep_apart(const Tensor* a, const char* name, const Tensor* b, const char* other) {
+    if (!a || !b || !a->numel() || !b->numel()) return;
+    const uintptr_t p = (uintptr_t)a->data_ptr(), q = (uintptr_t)b->data_ptr();
+    if (p < q + b->nbytes() && q < p + a->nbytes()) refuse(PyExc_ValueError, name, " and ", other, " share memory");
+}
+
 // The device that all tensors of a call are on is current while this lives; its current stream.
 struct Place {
     int device, was;
@@ -143,7 +164,11 @@ struct Place {
     explicit Place(int dev) { enter(dev); }
     Place(const Place&) = delete;
     ~Place() {
-        if (was != device) c10::hip::set_device((c10::DeviceIndex)was);
+        if (was == device) return;
+        try {
+            c10::hip::set_device((c10::DeviceIndex)was);
+        } catch (...) {                    // a destructor's exception would end the process
+        }
     }
     [[noreturn]] static void not_here() { refuse(PyExc_RuntimeError, "stdiff_amd runs on MI355X only: got a CPU tensor (no CPU fallback exists)"); }
 
@@ -176,6 +201,8 @@ PyObject* layer_norm(PyObject* const* a) {
     if (w && b && w->scalar_type() != b->scalar_type())
         refuse(PyExc_TypeError, "weight is ", w->scalar_type(), ", bias ", b->scalar_type(), ": one dtype is needed");
     void *wp = vector(w, "weight", H, true), *bp = vector(b, "bias", H, true), *mp = vector(mean, "mean", R), *rp = vector(rstd, "rstd", R);
+    if (given) keep_apart(*given, "out", ldy, x, "x", ldx, true);
+    keep_apart(mean, "mean", rstd, "rstd");
     Half half;
     const ScalarType yt = given ? given->scalar_type() : dtype(a[5], x.scalar_type());
     const int xc = half.code(x.scalar_type()), yc = half.code(yt), wc = w ? half.code(w->scalar_type()) : b ? half.code(b->scalar_type()) : STDIFF_F32;
@@ -202,6 +229,11 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
     vector(dw_, "dweight", H);
     vector(db_, "dbias", H);
     if (ws_ && !ws_->is_contiguous()) refuse(PyExc_ValueError, "workspace: a contiguous tensor is needed");
+    if (dx_) {
+        keep_apart(*dx_, "dx", lddx, x, "x", ldx, true);
+        keep_apart(*dx_, "dx", lddx, dy, "dy", lddy, true);
+    }
+    keep_apart(dw_, "dweight", db_, "dbias");
     Half half;
     const int xc = half.code(x.scalar_type()), dc = half.code(dy.scalar_type()), wc = w ? half.code(w->scalar_type()) : STDIFF_F32;
     Place here(x, {&dy, mean, rstd, w, dx_, dw_, db_, ws_});
@@ -231,6 +263,7 @@ PyObject* quantize_rows(PyObject* const* a) {
     if (out_) read_ld(*out_, "out", &x);
     const int64_t ldq = out_ ? rows16(*out_, "out") : kp;
     vector(scale_, "scale", R);
+    if (out_) keep_apart(*out_, "out", ldq, x, "x", ldx, false);
     Half half;
     const int xc = half.code(x.scalar_type());
     Place here(x, {out_, scale_});
@@ -259,6 +292,10 @@ PyObject* gemm_i8(PyObject* const* a) {
     if (out_ && (out_->dim() != 2 || out_->size(0) != M || out_->size(1) != N))
         refuse(PyExc_ValueError, "out: a matrix of [", M, ", ", N, "] is needed, got ", out_->sizes());
     g.ldc = out_ ? write_ld(*out_, "out") : N;
+    if (out_) {
+        keep_apart(*out_, "out", g.ldc, A, "A", lda, false);
+        keep_apart(*out_, "out", g.ldc, W, "W", ldw, false);
+    }
     Half half;
     const ScalarType ct = out_ ? out_->scalar_type() : dtype(a[6], ScalarType::Float);
     g.c_dtype = half.code(ct);

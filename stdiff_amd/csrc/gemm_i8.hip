@@ -117,7 +117,7 @@ int launch_quantize(const void* x, long long ldx, void* q, long long ldq, float*
                        dim3(256), 0, st, (const TX*)x, ldx, (signed char*)q, ldq, scale, R, K)
     if (K <= 512) QR(1, 64);
     else if (K <= 1024) QR(2, 64);
-    else if (K <= 2048) QR(4, 64);
+    else if (K <= 2048) QR(1, 256);
     else if (K <= 4096) QR(2, 256);
     else if (K <= 8192) QR(4, 256);
     else
@@ -547,7 +547,7 @@ template <typename TC> int launch_gemm_i8(const Params8& p, hipStream_t st) {
     // through LDS, 1.5 times as fast a byte)
     const auto busiest = [&](int mt) { return ((p.N + 15ll) / 16 * ((p.M + 16ll * mt - 1) / (16 * mt)) + cus - 1) / cus * (16 + 16 * mt) * 3 / 2; };
     const long long r1 = busiest(1), r2 = busiest(2), r4 = busiest(4), least = std::min(r1, std::min(r2, r4));
-    const int kind = p.M <= 65536 && least <= (t64 + cus - 1) / cus * 128 ? 1 : t256 >= cus * 3 / 8 ? 4 : t64 > 2 * cus ? 3 : 2;
+    const int kind = p.M <= 65536 && p.N <= 1 << 26 && least <= (t64 + cus - 1) / cus * 128 ? 1 : t256 >= cus * 3 / 8 ? 4 : t64 > 2 * cus ? 3 : 2;
     if (kind == 1) {
         const int mt = least == r1 ? 1 : least == r2 ? 2 : 4;
         const dim3 grid(cdiv(p.N, 16), cdiv(p.M, 16 * mt));

@@ -289,6 +289,10 @@ __global__ __launch_bounds__((most_threads<T, V>())) void layer_norm_bwd_kernel(
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const span<V> col((i * (int)blockDim.x + t) * V, H);
+                if (!col.skip) {
+                    stv<V>(out + k * ldp + col.at, a[i]);
+                    continue;
+                }
 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     if (j >= col.skip) out[k * ldp + col.at + j] = a[i][j];
@@ -445,6 +449,7 @@ __global__ __launch_bounds__(256) void fill_zero_kernel(float* a, float* b, int 
     if (b) b[i] = 0.f;
 }
 
+constexpr int LONGEST = 1 << 30;          // columns are counted in 32 bits, a workgroup's stride behind the end included
 constexpr int IN_REGISTERS = 16384;       // longest row that the register kernels take; the shortest is a vector
 inline bool in_registers(int H) { return H >= 8 && H <= IN_REGISTERS; }
 
@@ -473,7 +478,8 @@ inline int bwd_parts(int R, int H, int size) {
     const int waves = threads_of(H) / 64, places = waves > 4 ? (waves + 3) / 4 * 4 : waves;     // the same number on all four SIMDs
     const int wide = std::max(1, 16 / places), narrow = std::max(1, 8 / places);
     const bool many = size == 2 && (H <= 1024 || R >= 16ll * wide * cu_count());
-    return norm_blocks(R, std::max(rows_of_block(H) * 2, 6), many ? wide : narrow);
+    const int least = std::max(1, std::min(6, R / cu_count()));
+    return norm_blocks(R, std::max(rows_of_block(H) * 2, least), many ? wide : narrow);
 }
 inline int ld_parts(int H) { return (H + 3) / 4 * 4; }
 
@@ -587,6 +593,7 @@ extern "C" int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, cons
     STDIFF_CHECK_ARG(R >= 0 && H > 0 && (R == 0 || (x && y)) && ldx >= 0 && ldy >= H && eps >= 0.f);
     STDIFF_CHECK_ARG(dtype_ok(x_dtype) && dtype_ok(y_dtype) && dtype_ok(w_dtype));
     if (R == 0) return STDIFF_OK;
+    if (H > LONGEST) return STDIFF_ERR_SHAPE;
     if (!at_element(x, x_dtype) || !at_element(y, y_dtype) || !at_element(weight, w_dtype) || !at_element(bias, w_dtype) ||
         !at_element(mean, STDIFF_F32) || !at_element(rstd, STDIFF_F32))
         return STDIFF_ERR_ALIGN;
@@ -606,6 +613,7 @@ extern "C" int stdiff_layer_norm(const void* x, long long ldx, int x_dtype, cons
 
 extern "C" long long stdiff_layer_norm_bwd_workspace(int R, int H, int x_dtype, int dy_dtype) {
     if (R < 0 || H <= 0 || !dtype_ok(x_dtype) || !dtype_ok(dy_dtype)) return STDIFF_ERR_ARG;
+    if (H > LONGEST) return STDIFF_ERR_SHAPE;
     const int size = (int)dtype_size(x_dtype);
     return one_launch(R, H, size, (int)dtype_size(dy_dtype)) ? 0 : (long long)bwd_parts(R, H, size) * 2 * ld_parts(H) * 4;
 }
@@ -616,6 +624,7 @@ extern "C" int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtyp
                                      long long workspace_bytes, int R, int H, void* stream) {
     STDIFF_CHECK_ARG(R >= 0 && H > 0 && (R == 0 || (dy && x && mean && rstd && dx)) && lddy >= 0 && ldx >= 0 && lddx >= H);
     STDIFF_CHECK_ARG(dtype_ok(dy_dtype) && dtype_ok(x_dtype) && dtype_ok(w_dtype));
+    if (H > LONGEST) return STDIFF_ERR_SHAPE;
     if (!at_element(dy, dy_dtype) || !at_element(x, x_dtype) || !at_element(dx, x_dtype) || !at_element(weight, w_dtype) ||
         !at_element(mean, STDIFF_F32) || !at_element(rstd, STDIFF_F32) || !at_element(dweight, STDIFF_F32) ||
         !at_element(dbias, STDIFF_F32) || ((uintptr_t)workspace & 15))

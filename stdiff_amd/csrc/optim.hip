@@ -397,7 +397,7 @@ int check_multi(const stdiff_adamw_multi_args* a) {
     for (int i = 0; i < a->n_tensors; ++i) {
         const stdiff_adamw_tensor& s = a->tensors[i];
         STDIFF_CHECK_ARG(s.n >= 0 && (s.param_dtype == STDIFF_F32 || s.param_dtype == STDIFF_BF16) &&
-                         (s.grad_dtype == STDIFF_F32 || s.grad_dtype == STDIFF_BF16));
+                         (s.grad_dtype == STDIFF_F32 || s.grad_dtype == STDIFF_BF16) && s.weight_decay >= 0.f);
         if (s.n == 0) continue;
         STDIFF_CHECK_ARG(s.param && s.grad && s.exp_avg && s.exp_avg_sq);
         STDIFF_CHECK_ARG(a->state_bits == 32 || (s.exp_avg_scale && s.exp_avg_sq_scale));

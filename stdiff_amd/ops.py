@@ -10,7 +10,18 @@ from ._lib import F32, check, dt_of, lib, lib_for, ptr, require_gpu, stream
 try:
     from . import _bind
 except ImportError as e:
-    raise RuntimeError("stdiff_amd/_bind.so was not built (make -C stdiff_amd/csrc) or does not fit this torch") from e
+    class _NoBind:
+        """In the place of an extension module that was not built or does not fit this torch: what needs it raises."""
+
+        def __init__(self, why):
+            self.why = why
+
+        def setup(self, *a):
+            pass
+
+        def __getattr__(self, name):
+            raise RuntimeError(f"stdiff_amd/_bind.so cannot be used (make -C stdiff_amd/csrc builds it): {self.why}")
+    _bind = _NoBind(str(e))
 
 
 def round_up(a, b):
@@ -399,7 +410,7 @@ _bind.setup(_entries, L.StdiffError)
 def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, mean=None, rstd=None):
     """LayerNorm of the rows of x [R, H] with a weight and a bias per column (None: 1 and 0; one dtype for both).
     x and out: fp32 or a 16-bit type, any row stride, any H.  mean / rstd (fp32 [R], optional): receive the statistics
-    that layer_norm_bwd takes.  out may be x."""
+    that layer_norm_bwd takes.  out may be x; else it shares no memory with it."""
     return _bind.layer_norm(x, weight, bias, eps, out, out_dtype, mean, rstd)
 
 
@@ -440,7 +451,7 @@ def adamw_multi_args(params, exp_avg, exp_avg_sq, exp_avg_scale=None, exp_avg_sq
     """What adamw_multi updates: lists of contiguous tensors, one entry per parameter (fp32 or one 16-bit type; views into
     larger buffers are fine, no two may share memory).  exp_avg / exp_avg_sq: fp32, or torch.float8_e4m3fn with a vector
     of ceil(numel / 256) fp32 scales per tensor in exp_avg_scale / exp_avg_sq_scale (adamw8_state makes all four).
-    weight_decay: one number, or one per tensor.  The states are read and written in place by every step.  A model whose
+    weight_decay: one number, or one per tensor (not negative).  The states are read and written in place by every step.  A model whose
     parameters move to other memory (.to(), a DiT_stDiff at its first forward under autograd) needs new args."""
     return AdamWTensors(params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, weight_decay)
 

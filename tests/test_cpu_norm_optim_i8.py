@@ -193,3 +193,66 @@ def test_no_cpu_path():
                  lambda: ops.adamw_multi_args([p], [p], [p]), lambda: ops.adamw8_state(p)):
         with pytest.raises(RuntimeError, match="MI355X"):
             call()
+
+
+def test_longest_rows_and_decay(lib):
+    """columns are counted in 32 bits with a workgroup's stride behind them; a weight decay is not negative"""
+    from stdiff_amd import _lib as L
+    H = (1 << 30) + 1
+    assert lib.stdiff_layer_norm(AT, H, 0, AT, AT, 0, 1e-6, AT, H, 0, None, None, 1, H, None) == SHAPE
+    assert lib.stdiff_layer_norm(AT, 2**31 - 1, 1, None, None, 0, 1e-6, AT, 2**31 - 1, 1, None, None, 3, 2**31 - 1, None) == SHAPE
+    assert lib.stdiff_layer_norm_bwd_workspace(4, H, 0, 0) == SHAPE
+    assert lib.stdiff_layer_norm_bwd(AT, H, 0, AT, H, 0, AT, AT, AT, 0, AT, H, AT, AT, 0, AT, 1 << 50, 4, H, None) == SHAPE
+    for wd in (-0.1, float("nan")):
+        t = (L.AdamWTensor * 1)()
+        t[0].param = t[0].grad = t[0].exp_avg = t[0].exp_avg_sq = AT
+        t[0].n, t[0].weight_decay = 5, wd
+        a = L.AdamWMultiArgs()
+        a.tensors, a.n_tensors, a.state_bits = t, 1, 32
+        a.step_dev, a.workspace, a.workspace_bytes = AT, AT, 1 << 20
+        a.lr, a.beta1, a.beta2, a.eps, a.grad_scale = 1e-3, 0.9, 0.999, 1e-8, 1.0
+        assert lib.stdiff_adamw_multi(C.byref(a), None) == ARG, wd
+
+
+def test_shared_memory_is_refused():
+    """an output may be the input where that is said, and may lie beside it in one buffer; everything else that overlaps is refused"""
+    from stdiff_amd import ops
+    buf, s4, w = torch.zeros(4, 96), torch.zeros(4), torch.ones(32)
+    x = buf[:, 32:64]
+
+    def refused(match, call, kind=ValueError):
+        with pytest.raises(kind, match=match):
+            call()
+    for out in (buf[:, 31:63], buf[:, 33:65], buf.view(-1)[32:160].view(4, 32)):
+        refused("share memory", lambda: ops.layer_norm(x, out=out))
+        refused("share memory", lambda: ops.layer_norm_bwd(torch.zeros(4, 32), x, s4, s4, dx=out))
+        refused("share memory", lambda: ops.layer_norm_bwd(x, torch.zeros(4, 32), s4, s4, dx=out))
+    refused("share memory", lambda: ops.layer_norm(x, out=buf.view(torch.bfloat16)[:, 64:96]))
+    refused("share memory", lambda: ops.layer_norm(buf[:1, :32].expand(4, 32), out=buf[:, :32]))
+    # the same elements, columns beside them, the other rows: these are fine as far as a machine without a GPU can tell
+    for out in (x, buf[:, :32], buf[:, 64:], torch.zeros(4, 32)):
+        refused("MI355X", lambda: ops.layer_norm(x, out=out), RuntimeError)
+        refused("MI355X", lambda: ops.layer_norm_bwd(x, x, s4, s4, dx=out), RuntimeError)
+    rows = torch.zeros(8, 32)
+    refused("MI355X", lambda: ops.layer_norm(rows[:4], out=rows[4:]), RuntimeError)
+    refused("share memory", lambda: ops.layer_norm(rows[:4], out=rows[3:7]))
+    refused("MI355X", lambda: ops.layer_norm(rows[::2], out=rows[1::2]), RuntimeError)
+    refused("mean and rstd", lambda: ops.layer_norm(x, mean=s4, rstd=s4))
+    refused("dweight and dbias", lambda: ops.layer_norm_bwd(x, x, s4, s4, w, dweight=w, dbias=w))
+    refused("share memory", lambda: ops.quantize_rows(buf, out=buf.view(torch.int8)[:, :96]))
+    q = torch.zeros(4, 32, dtype=torch.int8)
+    refused("out and A", lambda: ops.gemm_i8(q, s4, q.clone(), s4, out=q.view(torch.float32)[:, :4]))
+    refused("out and W", lambda: ops.gemm_i8(q.clone(), s4, q, s4, out=q.view(torch.float32)[:, :4]))
+
+
+def test_without_the_extension_module(tmp_path):
+    """what does not need _bind works without it, what needs it says what is missing"""
+    import subprocess
+    import sys
+    code = ("import sys; sys.modules['stdiff_amd._bind'] = None\n"
+            "import torch; from stdiff_amd import ops\n"
+            "assert ops.round_up(5, 4) == 8 and ops.adamw_multi_workspace(1) > 0\n"
+            "try: ops.layer_norm(torch.zeros(2, 8))\n"
+            "except RuntimeError as e: print('refused', e)\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0 and "refused stdiff_amd/_bind.so cannot be used" in r.stdout, r.stderr

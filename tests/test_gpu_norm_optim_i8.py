@@ -852,3 +852,128 @@ def test_side_stream(ops):
         z = ops.gemm_i8(q, sc, q, sc)
     s.synchronize()
     assert torch.equal(y, ops.layer_norm(x)) and torch.equal(q, ops.quantize_rows(x)[0]) and torch.equal(z, ops.gemm_i8(q, sc, q, sc))
+
+
+@pytest.mark.parametrize("H", [3, 48, 100, 320, 1000, 1024, 2051, 9001, 17000])
+@pytest.mark.parametrize("xt", ["fp32", "bf16"])
+def test_layer_norm_in_place_and_beside(ops, H, xt):
+    """out in x's place, and out and x as columns of one buffer: the bits of a call with memory of its own"""
+    R = 70
+    x, w, b = rnd(R, H, seed=400).to(DT[xt]).to(DEV), rnd(H, seed=401).to(DEV), rnd(H, seed=402).to(DEV)
+    want = ops.layer_norm(x, w, b)
+    buf = torch.full((R, 3 * H + 5), 7.0, device=DEV, dtype=DT[xt])
+    a, out = buf[:, 1:H + 1], buf[:, H + 1:2 * H + 1]
+    a.copy_(x)
+    assert ops.layer_norm(a, w, b, out=out) is out and torch.equal(out, want) and torch.equal(a, x)
+    ops.layer_norm(a, w, b, out=a)
+    assert torch.equal(a, want) and torch.equal(out, want)
+    assert bool((buf[:, :1] == 7).all()) and bool((buf[:, 2 * H + 1:] == 7).all())
+
+
+def test_gemm_i8_very_many_columns(ops):
+    """more columns than a launch of 16 each can have; the first and the last ones are right, the gap behind them stays"""
+    N, K = (1 << 27) + 40, 16
+    W = torch.zeros(N, K, device=DEV, dtype=torch.int8)
+    at = torch.tensor([0, 1, 77, 1 << 26, (1 << 26) + 13, (1 << 27) - 1, 1 << 27, N - 17, N - 1], device=DEV)
+    rows = torch.randint(-127, 128, (len(at), K), generator=torch.Generator().manual_seed(5)).to(torch.int8)
+    W[at] = rows.to(DEV)
+    A = torch.randint(-127, 128, (1, K), generator=torch.Generator().manual_seed(6)).to(torch.int8)
+    sa, sw = torch.full((1,), 0.5, device=DEV), torch.full((N,), 0.25, device=DEV)
+    C = torch.full((1, N + 8), 9.0, device=DEV)
+    ops.gemm_i8(A.to(DEV), sa, W, sw, out=C[:, :N])
+    want = (A.long() @ rows.long().t()).double()[0] * 0.125
+    assert torch.equal(C[0, at].cpu().double(), want)
+    assert bool((C[0, N:] == 9).all())
+    C[0, at] = 0
+    assert not bool(C[0, :N].any())
+
+
+def test_two_threads(ops):
+    """calls of two threads on streams of their own, with other sizes and types: each gets what it gets alone"""
+    import threading
+    jobs = [(300, 1000, torch.float32, 1e-2), (257, 520, torch.bfloat16, 3e-2)]
+
+    def work(k, n):
+        R, H, t, lr = jobs[k]
+        x, dy = rnd(R, H, seed=410 + k).to(t).to(DEV), rnd(R, H, seed=420 + k).to(t).to(DEV)
+        p = torch.ones(H, device=DEV)
+        m, v = torch.zeros_like(p), torch.zeros_like(p)
+        args, step = ops.adamw_multi_args([p], [m], [v]), torch.zeros(1, device=DEV, dtype=torch.int32)
+        mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+        for _ in range(n):
+            y = ops.layer_norm(x, p, mean=mean, rstd=rstd)
+            dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, p)
+            ops.adamw_multi(args, [dw], step, lr, max_norm=1.0)
+            q, s = ops.quantize_rows(y)
+            z = ops.gemm_i8(q, s, q, s)
+        torch.cuda.current_stream().synchronize()
+        return p, dx, z
+    alone = [work(k, 30) for k in range(2)]
+    together, failed = [None, None], []
+
+    def thread(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                together[k] = work(k, 30)
+        except BaseException as e:
+            failed.append(e)
+    torch.cuda.synchronize()
+    ts = [threading.Thread(target=thread, args=(k,)) for k in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not failed
+    for k in range(2):
+        for a, b in zip(alone[k], together[k]):
+            assert torch.equal(a, b), k
+
+
+def test_torch_graph(ops):
+    """the same calls with outputs and workspaces of their own allocation, captured by torch.cuda.graph"""
+    R, H = 2200, 260
+    x, dy, w = torch.empty(R, H, device=DEV), torch.empty(R, H, device=DEV), rnd(H, seed=430).to(DEV)
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+
+    def body(mean, rstd):
+        y = ops.layer_norm(x, w, mean=mean, rstd=rstd)
+        q, s = ops.quantize_rows(y)
+        return (y, s, ops.gemm_i8(q, s, q[:100], s[:100])) + ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    x.zero_(), dy.zero_()
+    body(mean, rstd)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = body(mean, rstd)
+    for k in range(4):
+        x.copy_(rnd(R, H, seed=440 + k).to(DEV))
+        dy.copy_(rnd(R, H, seed=450 + k).to(DEV))
+        g.replay()
+        want = body(torch.empty_like(mean), torch.empty_like(rstd))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_multi_edges(ops, bits):
+    """no tensors, no gradients, empty tensors, a norm that nothing is clipped by, the largest and smallest clips"""
+    step, norm = torch.zeros(1, device=DEV, dtype=torch.int32), torch.full((1,), 5.0, device=DEV)
+    none = ops.adamw_multi_args([], [], [])
+    ops.adamw_multi(none, [], step, 1e-2, max_norm=1.0, norm=norm)
+    assert int(step) == 1 and float(norm) == 0
+    ps, dp, st, args = make(ops, [(300,), (0,), (5,)], bits, "fp32", 0.1)
+    before = [p.clone() for p in dp]
+    norm.fill_(5)
+    ops.adamw_multi(args, [None, None, None], step, 1e-2, max_norm=1.0, norm=norm)
+    assert int(step) == 2 and float(norm) == 0 and all(torch.equal(a, b) for a, b in zip(dp, before))
+    gs = [torch.full((300,), 2.0, device=DEV), torch.empty(0, device=DEV), None]
+    step.zero_()
+    ops.adamw_multi(args, gs, step, 0.0, norm=norm)                  # lr 0: the states move, the parameters stay
+    assert abs(float(norm) - 1200 ** 0.5) < 1e-3 and all(torch.equal(a, b) for a, b in zip(dp, before))
+    m = st[0][0].float() * (st[0][2].repeat_interleave(256)[:300] if bits == 8 else 1)
+    assert bool((abs(m - 0.2) < 1e-6).all())
+    step.zero_()
+    for max_norm, grad_scale in ((1e-45, 1.0), (1e300, 1.0), (1.0, 1e-30)):
+        ops.adamw_multi(args, gs, step, 1e-3, max_norm=max_norm, grad_scale=grad_scale)
+    assert all(bool(torch.isfinite(p).all()) for p in dp) and torch.equal(dp[2], before[2])
