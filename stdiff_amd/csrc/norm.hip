@@ -81,10 +81,9 @@ template <int V> struct span {
     __device__ __forceinline__ bool in() const { return skip < V; }
 };
 
-// T lanes share a row; BLOCK and BIG_BLOCK: the whole workgroup does.  For fp32 rows BLOCK has up to 512 threads (held to the 128
-// registers of 1024 threads the backward keeps 25 of its 148 in memory: 199 against 138 us for 32768 x 2048) and BIG_BLOCK
-// up to 1024; for 16-bit rows BLOCK has up to 1024 (6 of 133 in memory, but a fourth wave per SIMD: 96 against 106 us for
-// 16000 x 4096).
+// T lanes share a row; BLOCK and BIG_BLOCK: the whole workgroup does.  The backward needs 118 to 124 registers for 16-bit rows, so
+// BLOCK has up to 1024 threads there; for fp32 rows it needs 138, and BLOCK has up to 512 threads (held to the 128 registers of
+// 1024 threads 30000 x 2050 takes 146 us instead of 130), BIG_BLOCK, which keeps 11 of them in memory, up to 1024.
 enum { BLOCK = 0, BIG_BLOCK = 1 };
 constexpr int E = 16;                     // elements per lane
 template <int T> __device__ __forceinline__ int row_lanes() { return T > BIG_BLOCK ? T : (int)blockDim.x; }
@@ -481,17 +480,17 @@ inline int rows_of_block(int H) { return H <= 1024 ? 256 / lanes_of(H) : 1; }
 inline bool one_launch(int R, int H, int x_size, int dy_size) {
     return (long long)R * 32 * (x_size + dy_size) <= 320 << 10 && H >= 8 && H <= 8192;
 }
-// Workgroups of the backward, each of which leaves partial sums as large as two fp32 rows: at least six rows for each (4096 x 2048
-// bf16: two 40, six 26 us).  Eight waves per CU; sixteen for rows of 16 bits, which have half the bytes in flight (65536 x
-// 1024 bf16: 106 against 75 us), but where a workgroup has one row at a time only if that leaves sixteen rows for each
-// (16384 x 2048 bf16: eight waves 48, sixteen 60 us; 32768 x 4096: 177 and 163).
+// Workgroups of the backward, each of which leaves partial sums as large as two fp32 rows: at least six rows for each where that
+// leaves one per CU (4096 x 2048 bf16: two 40, six 26 us; 16 x 16384 fp32: one 14, six 44).  fp32 rows: eight waves per CU
+// (32768 x 2048: 142 us, sixteen 157).  Rows of 16 bits have half the bytes in flight: sixteen waves where a wave has a row
+// (65536 x 1024 bf16: 74 us, eight 78), else four workgroups of two or three waves (30000 x 2050: 78, three 90), two of four to
+// eight (32768 x 4096: 144, four 152; 16000 x 8192: 138, one 158).
 inline int bwd_parts(int R, int H, int size) {
     if (!in_registers(H)) return (int)std::min<long long>(R, 64);
     const int waves = threads_of(H) / 64, places = waves > 4 ? (waves + 3) / 4 * 4 : waves;     // the same number on all four SIMDs
-    const int wide = std::max(1, 16 / places), narrow = std::max(1, 8 / places);
-    const bool many = size == 2 && (H <= 1024 || R >= 16ll * wide * cu_count());
+    const int per_cu = size == 4 ? std::max(1, 8 / places) : H <= 1024 || waves <= 3 ? 4 : waves <= 8 ? 2 : 1;
     const int least = std::max(1, std::min(6, R / cu_count()));
-    return norm_blocks(R, std::max(rows_of_block(H) * 2, least), many ? wide : narrow);
+    return norm_blocks(R, std::max(rows_of_block(H) * 2, least), per_cu);
 }
 inline int ld_parts(int H) { return (H + 3) / 4 * 4; }
 
