@@ -10,7 +10,7 @@
 // still under the slow decay of v.  The step itself uses m and v before they are rounded.
 // Bound by memory: 120 M parameters in 32 bits 81 us for the norm (5.9 TB/s) and 565 for the step (5.9 TB/s), 30 M with 8-bit states
 // 14 and 88 us (5.0 TB/s; 230 vector instructions per 256 elements are 60 % of it), 479 M 1447 us together.  Small models are two launches
-// of 5.6 and 6.9 us, of which the host needs most.
+// of 4.6 and 6.1 us: the table, the data, for the step also the partial sums, one trip to memory each.
 // A block that holds an infinity or a NaN gets a scale that is not finite: all its elements are NaN from the next step on.
 #include <float.h>
 
@@ -139,9 +139,18 @@ __device__ __forceinline__ float of_lane(float v, int k) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), k));
 }
 
-template <typename B> __device__ __forceinline__ int tensor_of(const B& b, int chunk, int t) {
-    while (chunk < b.first[t]) --t;
-    return t;
+// The tensor of a workgroup's first chunk: all borders are compared at once (one trip to the table, which no cache holds yet; a
+// walk makes one per 16 borders, one after the other).
+template <typename T, int N> __device__ __forceinline__ int tensor_of(const batch<T, N>& b, int chunk) {
+    const int lane = threadIdx.x & 63;
+    int below = 0;
+#pragma unroll
+    for (int i = 0; i < (N + 63) / 64; ++i) {
+        const int k = i * 64 + lane;
+        const int border = b.first[min(k + 1, N)];
+        below += __popcll(__builtin_amdgcn_ballot_w64(k < b.count && border <= chunk));
+    }
+    return below;
 }
 
 // step count and the two bias corrections of this step, by one thread
@@ -163,9 +172,9 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(batchg b, float* parts,
                                                          double b1, double b2) {
     if (step_dev && blockIdx.x == 0 && threadIdx.x == 0) next_step(step_dev, scalars, lr, b1, b2);
     f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    int t = b.count - 1;
-    for (int chunk = b.first[b.count] - 1 - (int)blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
-        t = tensor_of(b, chunk, t);
+    int chunk = b.first[b.count] - 1 - (int)blockIdx.x;
+    for (int t = tensor_of(b, chunk); chunk >= 0; chunk -= gridDim.x) {
+        while (chunk < b.first[t]) --t;
         const bool half = b.t[t].n < 0;
         const long long n = half ? ~b.t[t].n : b.t[t].n, start = (long long)(chunk - b.first[t]) * NORM_CHUNK;
         const float* g32 = (const float*)b.t[t].g + start + threadIdx.x * 4;
@@ -327,8 +336,8 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(B b, update_arg a) {
     __shared__ float part[4];
     factors f;
     f.known = false;
-    int t = 0;
-    for (int chunk = blockIdx.x; chunk < b.first[b.count]; chunk += gridDim.x) {
+    int chunk = blockIdx.x;
+    for (int t = tensor_of(b, chunk); chunk < b.first[b.count]; chunk += gridDim.x) {
         while (chunk >= b.first[t + 1]) ++t;
         const auto& q = b.t[t];
         const long long start = (long long)(chunk - b.first[t]) * (U * 1024);
