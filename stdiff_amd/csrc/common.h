@@ -108,7 +108,7 @@ __device__ __forceinline__ void st4(bf16_t* p, f32x4 v) {
 __device__ __forceinline__ float silu_f(float v) { return v / (1.0f + expf(-v)); }
 __device__ __forceinline__ float gelu_erf_f(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f)); }
 
-// GELU(erf) for bf16 OUTPUTS, 4 lanes at a time, no transcendentals (packs into v_pk_fma_f32): Phi(x) = 0.5 + xc*Q(u),
+// GELU(erf) for bf16 OUTPUTS, 4 lanes at a time, no transcendentals: Phi(x) = 0.5 + xc*Q(u),
 // xc = clamp(x, -5, 5), u = 2*xc^2/25 - 1, Q = degree-12 minimax fit (tools/fit_gelu.py).  |Phi - exact| <= 2.6e-7,
 // |gelu - exact| <= 1.3e-6 on [-5, 5] and <= 1.5e-6*|x|/5 beyond: 3 orders below a bf16 ulp of the result scale.
 __device__ __forceinline__ f32x4 gelu_phi4(f32x4 x) {
