@@ -181,6 +181,10 @@ private:
     }
 };
 
+// autograd refuses a backward through what it had saved of a tensor that was written since
+void written(const Tensor* t) {
+    if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 PyObject* same(PyObject* given, const Tensor& made) {
     if (given != Py_None) {
         Py_INCREF(given);
@@ -210,6 +214,7 @@ PyObject* layer_norm(PyObject* const* a) {
     const Tensor out = given ? *given : at::empty({R, H}, x.options().dtype(yt));
     const Library& l = library(half.fp16);
     check(l, l.layer_norm(x.data_ptr(), ldx, xc, wp, bp, wc, (float)eps, out.data_ptr(), ldy, yc, (float*)mp, (float*)rp, (int)R, (int)H, here.stream));
+    for (const Tensor* t : {given, mean, rstd}) written(t);
     return same(a[4], out);
 }
 
@@ -249,6 +254,7 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
     check(l, l.layer_norm_bwd(dy.data_ptr(), lddy, dc, x.data_ptr(), ldx, xc, (float*)mp, (float*)rp, wp, wc, dx.data_ptr(), lddx,
                               dw.defined() ? (float*)dw.data_ptr() : nullptr, db.defined() ? (float*)db.data_ptr() : nullptr, accumulate,
                               ws.defined() ? (float*)ws.data_ptr() : nullptr, ws.defined() ? (long long)ws.nbytes() : 0, (int)R, (int)H, here.stream));
+    for (const Tensor* t : {dx_, dw_, db_}) written(t);
     PyObject* r = PyTuple_New(3);
     if (!r) throw Refusal{nullptr, ""};
     PyTuple_SET_ITEM(r, 0, same(a[5], dx));
@@ -272,6 +278,7 @@ PyObject* quantize_rows(PyObject* const* a) {
     const Tensor scale = scale_ ? *scale_ : floats(x, R);
     const Library& l = library(half.fp16);
     check(l, l.quantize_rows(x.data_ptr(), ldx, xc, out.data_ptr(), ldq, (float*)scale.data_ptr(), (int)R, (int)K, here.stream));
+    for (const Tensor* t : {out_, scale_}) written(t);
     PyObject* r = PyTuple_New(2);
     if (!r) throw Refusal{nullptr, ""};
     PyTuple_SET_ITEM(r, 0, same(a[1], out));
@@ -304,6 +311,7 @@ PyObject* gemm_i8(PyObject* const* a) {
     g.C = out.data_ptr();
     const Library& l = library(half.fp16);
     check(l, l.gemm_i8(&g, here.stream));
+    written(out_);
     return same(a[5], out);
 }
 
@@ -312,6 +320,7 @@ struct Table {
     std::vector<stdiff_adamw_tensor> rows;
     std::vector<int64_t> sizes;
     std::vector<c10::Storage> memory;      // alive even where a tensor is given other memory
+    std::vector<std::pair<Tensor, void*>> states;
     Half half;
     int bits = 32, device = -1;
 };
@@ -371,6 +380,7 @@ PyObject* adamw_table(PyObject* const* a) {
         for (j = 0; j < 5; ++j)
             if (k[j]) {
                 t->memory.push_back(k[j]->storage());
+                if (j) t->states.push_back({*k[j], k[j]->data_ptr()});
                 if (k[j]->numel()) ranges.push_back({(uintptr_t)k[j]->data_ptr(), k[j]->nbytes()});
             }
     }
@@ -403,6 +413,8 @@ PyObject* adamw_multi(PyObject* const* a) {
     if (step.scalar_type() != ScalarType::Int || step.numel() != 1) refuse(PyExc_ValueError, "step_dev: one int32 element is needed, got ", step.sizes(), " ", step.scalar_type());
     g.norm = (float*)vector(norm, "norm", 1);
     if (ws_ && !ws_->is_contiguous()) refuse(PyExc_ValueError, "workspace: a contiguous tensor is needed");
+    for (const auto& s : t->states)
+        if (s.first.data_ptr() != s.second) refuse(PyExc_ValueError, "adamw_multi: a state was given other memory since adamw_multi_args");
     Half half = t->half;
     std::vector<stdiff_adamw_tensor> rows = t->rows;       // of this call: two calls do not see each other's gradients
     for (Py_ssize_t i = 0; i < n; ++i) {
@@ -428,10 +440,7 @@ PyObject* adamw_multi(PyObject* const* a) {
     check(l, l.adamw_multi(&g, here.stream));
     // who keeps copies of the parameters (DiT_stDiff's packed operands) sees by their version counters that they changed
     for (Py_ssize_t i = 0; i < n; ++i)
-        if (rows[i].n) {
-            const Tensor& p = THPVariable_Unpack(params[i]);
-            if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
-        }
+        if (rows[i].n) written(&THPVariable_Unpack(params[i]));
     return Py_NewRef(Py_None);
 }
 

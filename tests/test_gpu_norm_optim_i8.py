@@ -977,3 +977,33 @@ def test_adamw_multi_edges(ops, bits):
     for max_norm, grad_scale in ((1e-45, 1.0), (1e300, 1.0), (1.0, 1e-30)):
         ops.adamw_multi(args, gs, step, 1e-3, max_norm=max_norm, grad_scale=grad_scale)
     assert all(bool(torch.isfinite(p).all()) for p in dp) and torch.equal(dp[2], before[2])
+
+
+def test_written_tensors_and_moved_states(ops):
+    """what a call wrote counts as changed for autograd; states that were given other memory are refused"""
+    x = rnd(9, 32, seed=460).to(DEV)
+    w = torch.ones(32, device=DEV)
+    mean, rstd, sc = (torch.ones(9, device=DEV) for _ in range(3))
+    q, out = torch.empty(9, 32, device=DEV, dtype=torch.int8), torch.empty(9, 9, device=DEV)
+    dw, db, dx = torch.zeros(32, device=DEV), torch.zeros(32, device=DEV), torch.empty_like(x)
+    a = torch.ones(9, 32, device=DEV, requires_grad=True)
+    b = a * x                                                        # saves x
+    for call, changed in ((lambda: ops.layer_norm_bwd(x, x, mean, rstd, w, dx=dx, dweight=dw, dbias=db), (dx, dw, db)),
+                          (lambda: ops.quantize_rows(x, out=q, scale=sc), (q, sc)), (lambda: ops.gemm_i8(q, sc, q, sc, out=out), (out,)),
+                          (lambda: ops.layer_norm(x, out=x, mean=mean, rstd=rstd), (x, mean, rstd))):
+        before = [t._version for t in changed]
+        call()
+        assert all(t._version > v for t, v in zip(changed, before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        b.sum().backward()
+    with torch.inference_mode():
+        y = torch.ones(3, 32, device=DEV)
+        ops.layer_norm(y, out=y)
+    assert not bool(y.any())
+    p, m, v = (torch.zeros(300, device=DEV) for _ in range(3))
+    args, step = ops.adamw_multi_args([p], [m], [v]), torch.zeros(1, device=DEV, dtype=torch.int32)
+    ops.adamw_multi(args, [torch.ones(300, device=DEV)], step, 1e-3)
+    v.data = torch.zeros(300, device=DEV)
+    with pytest.raises(ValueError, match="memory"):
+        ops.adamw_multi(args, [torch.ones(300, device=DEV)], step, 1e-3)
+    assert int(step) == 1
