@@ -372,8 +372,9 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_tile_kernel(Params8 p, int ti
 template <typename TC, bool TAIL>
 __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tiles_m, int tiles_n, int whole, int units) {
     constexpr int HALF = 128 * SLAB;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[9 * HALF];
-    __shared__ __attribute__((aligned(16))) float scales[3][256];       // a_scale, w_scale and bias of the tile
+    constexpr int SCALES = 9 * HALF;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[SCALES + 6 * 1024];
+    float* scales = (float*)(smem + SCALES);                            // a_scale, w_scale and bias of the tile, 256 of each; the next tile's
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wid >> 2, wc = wid & 3, fr = lane & 15, fq = lane >> 4, nk = (p.K + SLAB - 1) / SLAB;
     const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
@@ -398,10 +399,12 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
     auto dma = [&](int buf, int slot, int t) {                          // half tile `slot` of slab t into buffer buf
         unsigned char* dst = smem + (buf * 4 + slot) * HALF + 2 * wid * 1024;
         const bool in = t * SLAB + piece < p.K;
+        unsigned at = slot < 2 ? va : vw;
+        asm volatile("" : "+v"(at));       // the offsets are added up here, not kept (and spilled) across the K loop
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (slot < 2) load_lds(ra, dst + i * 1024, in ? va + (unsigned)(((slot & 1) * 128 + i * 8) * (int)p.lda + t * SLAB) : OUTSIDE);
-            else load_lds(rw, dst + i * 1024, in ? vw + (unsigned)(((slot & 1) * 128 + i * 8) * (int)p.ldw + t * SLAB) : OUTSIDE);
+            if (slot < 2) load_lds(ra, dst + i * 1024, in ? at + (unsigned)(((slot & 1) * 128 + i * 8) * (int)p.lda + t * SLAB) : OUTSIDE);
+            else load_lds(rw, dst + i * 1024, in ? at + (unsigned)(((slot & 1) * 128 + i * 8) * (int)p.ldw + t * SLAB) : OUTSIDE);
         }
     };
     auto prologue = [&]() {                                             // slab 0, and A0 of slab 1
@@ -446,9 +449,13 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
         __builtin_amdgcn_s_setprio(0);                                                                       \
     } while (0)
 
-    int unit = blockIdx.x;
+    constexpr int STORES = sizeof(TC) == 2 ? 16 : 32;                   // of C, per wave and whole tile
+    int unit = blockIdx.x, side = 0;
+    bool behind = false;                                                // so many are under way when a tile begins
     set_tile(unit);
     prologue();
+    scales[tid] = s0;
+    if (tid >= 256) scales[256 + tid] = s1;
     while (true) {
 #pragma unroll
         for (int mh = 0; mh < 2; ++mh)
@@ -458,10 +465,15 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) acc[mh][nh][i][j] = i32x4{0, 0, 0, 0};
-        BARRIER();                                                      // every wave is done with the C image and the scales
-        scales[tid >> 8][tid & 255] = s0;
-        if (tid >= 256) scales[2][tid & 255] = s1;
-        if (nk > 1) { dma(1, 2, 1); dma(1, 3, 1); VMCNT(4); } else { VMCNT(0); }
+        BARRIER();                                                      // every wave is done with the C image
+        if (nk > 1) {
+            dma(1, 2, 1);
+            dma(1, 3, 1);
+            if (behind) { if (STORES == 16) VMCNT(20); else VMCNT(36); }
+            else VMCNT(4);
+        } else {
+            VMCNT(0);
+        }
         LGKMCNT0();
         BARRIER();
         if (wr == 1) BARRIER();
@@ -472,7 +484,12 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
             load_w(b, 1);
             __builtin_amdgcn_sched_barrier(0);
             load_a(b, 0, t);
-            if (n1) { dma(nb, 1, t + 1); VMCNT(8); } else { VMCNT(0); }                          // A1(t) is here
+            if (n1) {
+                dma(nb, 1, t + 1);
+                if (t || !behind) VMCNT(8);                             // A1(t) is here
+            } else {
+                VMCNT(0);
+            }
             LGKMCNT0();                                                 // what was read may be overwritten behind the barrier
             BARRIER();
             MMA(0, 0);
@@ -492,6 +509,8 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
         if (wr == 0) BARRIER();                                         // all waves are past their last read of the buffers
         const int em = m0, en = n0, next = unit + (int)gridDim.x;
         const bool was_full = full;
+        behind = was_full && em + 256 <= p.M && en + 256 <= p.N;
+        const float* now = scales + side * 768;
         if (next < units) {
             set_tile(next);
             prologue();
@@ -505,8 +524,8 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int n = nh * 128 + wc * 32 + j * 16 + fq * 4;
-                ws[nh][j] = *(const f32x4*)&scales[1][n];
-                bs[nh][j] = *(const f32x4*)&scales[2][n];
+                ws[nh][j] = *(const f32x4*)&now[256 + n];
+                bs[nh][j] = *(const f32x4*)&now[512 + n];
             }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -516,7 +535,7 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int r = wr * 32 + j * 16 + fr, m = (q >> 1) * 128 + wr * 64 + ((q & 1) * 2 + j) * 16 + fr;
-                const float as = scales[0][m];
+                const float as = now[m];
 #pragma unroll
                 for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
@@ -529,20 +548,32 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
             }
             LGKMCNT0();
             BARRIER();
-            constexpr int PIECES = ROW / 16;
+            constexpr int PIECES = ROW / 16, EACH = 64 * PIECES / 512;
+            u32x4 v[EACH];
 #pragma unroll
-            for (int i = 0; i < 64 * PIECES / 512; ++i) {
+            for (int i = 0; i < EACH; ++i) {
                 const int r = (tid + 512 * i) / PIECES, c = (tid + 512 * i) % PIECES;
-                const int m = em + (q >> 1) * 128 + (r >> 5) * 64 + (q & 1) * 32 + (r & 31);
-                u32x4 v;
-                if constexpr (sizeof(TC) == 2) v = *(const u32x4*)(img + r * ROW + (((2 * c) ^ ((r & 15) << 1)) << 3));
-                else v = *(const u32x4*)(img + r * ROW + ((c ^ (r & 15)) << 4));
-                if (m < p.M) store16<true>((TC*)p.C + m * p.ldc, en + c * (16 / (int)sizeof(TC)), p.N, v);
+                if constexpr (sizeof(TC) == 2) v[i] = *(const u32x4*)(img + r * ROW + (((2 * c) ^ ((r & 15) << 1)) << 3));
+                else v[i] = *(const u32x4*)(img + r * ROW + ((c ^ (r & 15)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int r = (tid + 512 * i) / PIECES, c = (tid + 512 * i) % PIECES;
+                const int m = em + (q >> 1) * 128 + (r >> 5) * 64 + (q & 1) * 32 + (r & 31), n = en + c * (16 / (int)sizeof(TC));
+                TC* row = (TC*)p.C + m * p.ldc;
+                if (behind) __builtin_nontemporal_store(v[i], (u32x4_u*)(row + n));
+                else if (m < p.M) store16<true>(row, n, p.N, v[i]);
+            }
+            if (q == 1) {                                               // the next tile's scales are here
+                float* then = scales + (side ^ 1) * 768;
+                then[tid] = s0;
+                if (tid >= 256) then[256 + tid] = s1;
             }
             LGKMCNT0();
         }
         if (next >= units) break;
         unit = next;
+        side ^= 1;
     }
 #undef MMA
 }
