@@ -5,8 +5,8 @@
 // scales are applied to the finished sum in fp32, the weight's first: sum * a_scale would overflow for activations above
 // 1e31 whose product with a weight is still a number.
 // Measured: quantisation of 65536 x 2048 bf16 76 us (5.3 TB/s of the 5.9 that a copy of this file's kind reaches), of 4 rows 2.1 us; product
-// of 4 x 4096 x 1024 3.8 us (a launch, one trip to memory and one barrier), of 65536 x 8192 x 2048 930 us (2.36 POP/s; 8192 x
-// 8192 x 8192 2.8 to 2.9): the matrix units are busy 61 % of the cycles, and the clock falls to 1.94 GHz.
+// of 4 x 4096 x 1024 3.8 us (a launch, one trip to memory and one barrier), of 65536 x 8192 x 2048 892 us (2.47 POP/s; 8192 x
+// 8192 x 8192 2.85): the matrix units are busy 61 % of the cycles, and the clock falls to 1.94 GHz.
 #include "common.h"
 
 namespace {
@@ -212,7 +212,7 @@ template <bool NT, typename TC> __device__ __forceinline__ void store16(TC* row,
     }
 }
 // Tile of workgroup i.  Workgroups i and i + 8 share an XCD's L2: each XCD gets a contiguous range of tiles, in groups of four rows
-// of tiles (16384 x 6144 x 2048: four 173, eight 184 us; 8192 x 8192 x 8192: 382 and 386; 131072 x 4096 x 1024: 557 and 545).
+// of tiles (16384 x 6144 x 2048: two 170, four 168, eight 176 us; 8192 x 8192 x 8192: 390, 380 and 380; 131072 x 4096 x 1024: 530, 530 and 523).
 __device__ __forceinline__ void tile_at(int i, int tiles_m, int tiles_n, int* tm, int* tn) {
     constexpr int HIGH = 4;
     const int n = tiles_m * tiles_n, q = n >> 3, r = n & 7, x = i & 7;
@@ -366,8 +366,9 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_tile_kernel(Params8 p, int ti
 // instructions per wave) while the halves that were read last are refilled two slabs ahead; the waits are counted, and
 // waves 4-7 run one barrier behind waves 0-3, so that on every SIMD one wave multiplies while the other reads.  The
 // first loads of the next tile are issued before C leaves through the buffers that they do not use.
-// The compiler lets reads of LDS wait for all DMA under way, the scales being an array of their own; that the slabs arrive is not the
-// bound: in one array, without these waits, 65536 x 8192 x 2048 takes 950 us instead of 920 (36 bytes of registers spilled).
+// All of LDS is one array: with another for the scales the compiler lets every read wait for all DMA under way.
+// Measured per tile: 1.43 us for a slab (the instructions alone 1.06 at the clock that they leave), 5 us for C, half of it conversions and
+// scales.  The stores of C are under way during the next tile's first slab: the counted waits know how many they are.
 // TAIL: K is no multiple of 16.  (A form of its own: the kernel uses all 256 registers, and the masks cost some.)
 template <typename TC, bool TAIL>
 __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tiles_m, int tiles_n, int whole, int units) {
@@ -407,9 +408,9 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
             else load_lds(rw, dst + i * 1024, in ? at + (unsigned)(((slot & 1) * 128 + i * 8) * (int)p.ldw + t * SLAB) : OUTSIDE);
         }
     };
-    auto prologue = [&]() {                                             // slab 0, and A0 of slab 1
+    auto prologue = [&]() {                                             // slab 0, and all of slab 1 but A1
         dma(0, 0, 0); dma(0, 2, 0); dma(0, 3, 0); dma(0, 1, 0);
-        if (nk > 1) dma(1, 0, 1);
+        if (nk > 1) { dma(1, 0, 1); dma(1, 2, 1); dma(1, 3, 1); }
     };
     int oa[2], ow[2];
 #pragma unroll
@@ -465,17 +466,12 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) acc[mh][nh][i][j] = i32x4{0, 0, 0, 0};
-        BARRIER();                                                      // every wave is done with the C image
-        if (nk > 1) {
-            dma(1, 2, 1);
-            dma(1, 3, 1);
-            if (behind) { if (STORES == 16) VMCNT(20); else VMCNT(36); }
-            else VMCNT(4);
-        } else {
-            VMCNT(0);
-        }
+        if (nk == 1) VMCNT(0);                                          // slab 0 is here
+        else if (!behind) VMCNT(6);
+        else if (STORES == 16) VMCNT(22);
+        else VMCNT(38);
         LGKMCNT0();
-        BARRIER();
+        BARRIER();                                                      // every wave's share too; the C image has been read
         if (wr == 1) BARRIER();
         for (int t = 0; t < nk; ++t) {
             const int b = t & 1, nb = b ^ 1;
@@ -496,8 +492,14 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
             MMA(0, 1);
             BARRIER();
             if (full) load_a(b, 1, t);
-            if (n2) { dma(b, 0, t + 2); dma(b, 2, t + 2); dma(b, 3, t + 2); VMCNT(8); }          // A0 W0 W1 (t + 1) are here
-            else if (n1) { VMCNT(2); }
+            if (n2) {
+                dma(b, 0, t + 2); dma(b, 2, t + 2); dma(b, 3, t + 2);
+                if (t || !behind) VMCNT(8);                             // A0 W0 W1 (t + 1) are here
+                else if (STORES == 16) VMCNT(24);
+                else VMCNT(40);
+            } else if (n1) {
+                VMCNT(2);
+            }
             LGKMCNT0();
             BARRIER();
             if (full) {
@@ -515,9 +517,10 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
             set_tile(next);
             prologue();
         }
-        // C by quarters of 64 rows (32 of each wave group) through an image in the last four half tiles; 16-bit quarters
-        // alternate between two images, so one barrier per quarter is enough
-        constexpr int ROW = 256 * (int)sizeof(TC), IMAGES = sizeof(TC) == 2 ? 2 : 1;
+        // C by eighths of 32 rows (16 of each wave group) through images in the half tiles 5 (A1 of slab 1) and 8, which the
+        // loads under way do not use: 16-bit eighths alternate, so one barrier each is enough, fp32 ones take both
+        constexpr int ROW = 256 * (int)sizeof(TC);
+        const auto image = [&](int e, int group) { return smem + ((sizeof(TC) == 2 ? e & 1 : group) ? 8 : 5) * HALF + (sizeof(TC) == 2 ? group * 16 * ROW : 0); };
         f32x4 ws[2][2], bs[2][2];
 #pragma unroll
         for (int nh = 0; nh < 2; ++nh)
@@ -528,43 +531,40 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
                 bs[nh][j] = *(const f32x4*)&now[512 + n];
             }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if (q == 2 && !was_full) break;
-            unsigned char* img = smem + 5 * HALF + (q % IMAGES) * 64 * ROW;
-            if (q && IMAGES == 1) BARRIER();                            // the previous quarter's image has been read
+        for (int e = 0; e < 8; ++e) {
+            if (e == 4 && !was_full) break;
+            if (e && sizeof(TC) == 4) BARRIER();                        // the previous eighth's image has been read
+            unsigned char* put = image(e, wr) + fr * ROW;
+            const float as = now[(e >> 2) * 128 + wr * 64 + (e & 3) * 16 + fr];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int r = wr * 32 + j * 16 + fr, m = (q >> 1) * 128 + wr * 64 + ((q & 1) * 2 + j) * 16 + fr;
-                const float as = now[m];
+            for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
-                for (int nh = 0; nh < 2; ++nh)
-#pragma unroll
-                    for (int jn = 0; jn < 2; ++jn) {
-                        const int c = nh * 32 + wc * 8 + jn * 4 + fq;   // group of four columns
-                        const f32x4 v = scaled(acc[q >> 1][nh][(q & 1) * 2 + j][jn], as, ws[nh][jn], bs[nh][jn]);
-                        if constexpr (sizeof(TC) == 2) put4((TC*)(img + r * ROW + ((c ^ (fr << 1)) << 3)), v);
-                        else put4((TC*)(img + r * ROW + ((c ^ fr) << 4)), v);
-                    }
-            }
+                for (int jn = 0; jn < 2; ++jn) {
+                    const int c = nh * 32 + wc * 8 + jn * 4 + fq;       // group of four columns
+                    const f32x4 v = scaled(acc[e >> 2][nh][e & 3][jn], as, ws[nh][jn], bs[nh][jn]);
+                    if constexpr (sizeof(TC) == 2) put4((TC*)(put + ((c ^ (fr << 1)) << 3)), v);
+                    else put4((TC*)(put + ((c ^ fr) << 4)), v);
+                }
             LGKMCNT0();
             BARRIER();
-            constexpr int PIECES = ROW / 16, EACH = 64 * PIECES / 512;
+            constexpr int PIECES = ROW / 16, EACH = 32 * PIECES / 512;
             u32x4 v[EACH];
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int r = (tid + 512 * i) / PIECES, c = (tid + 512 * i) % PIECES;
-                if constexpr (sizeof(TC) == 2) v[i] = *(const u32x4*)(img + r * ROW + (((2 * c) ^ ((r & 15) << 1)) << 3));
-                else v[i] = *(const u32x4*)(img + r * ROW + ((c ^ (r & 15)) << 4));
+                const unsigned char* get = image(e, r >> 4) + (r & 15) * ROW;
+                if constexpr (sizeof(TC) == 2) v[i] = *(const u32x4*)(get + (((2 * c) ^ ((r & 15) << 1)) << 3));
+                else v[i] = *(const u32x4*)(get + ((c ^ (r & 15)) << 4));
             }
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 const int r = (tid + 512 * i) / PIECES, c = (tid + 512 * i) % PIECES;
-                const int m = em + (q >> 1) * 128 + (r >> 5) * 64 + (q & 1) * 32 + (r & 31), n = en + c * (16 / (int)sizeof(TC));
+                const int m = em + (e >> 2) * 128 + (r >> 4) * 64 + (e & 3) * 16 + (r & 15), n = en + c * (16 / (int)sizeof(TC));
                 TC* row = (TC*)p.C + m * p.ldc;
                 if (behind) __builtin_nontemporal_store(v[i], (u32x4_u*)(row + n));
                 else if (m < p.M) store16<true>(row, n, p.N, v[i]);
             }
-            if (q == 1) {                                               // the next tile's scales are here
+            if (e == 3) {                                               // the next tile's scales are here
                 float* then = scales + (side ^ 1) * 768;
                 then[tid] = s0;
                 if (tid >= 256) then[256 + tid] = s1;
@@ -586,12 +586,12 @@ template <typename TC> int launch_gemm_i8(const Params8& p, hipStream_t st) {
     // Small outputs: bytes of K that the busiest CU reads, a workgroup of 16 x 16 MT against a tile of 64 x 64 (the latter through
     // LDS, 1.5 times as fast a byte).  M x N x K, rows kernel and 64 tiles: 4 x 4096 x 1024 3.2 and 5.0 us, 64 x 1024 x 4096 6.1
     // and 11.9, 64 x 8192 x 4096 22.4 and 12.6.
-    // Tiles of 256 where they occupy 3/8 of the CUs, 128 and 256: 2048 x 4096 x 1024 17.6 and 15.6 us, 3000 x 2500 x 1000 19.1
-    // and 18.4, 2048 x 2048 x 2048 (a quarter) 15.8 and 20.0.  Between 64 and 128 two tiles of 64 per CU, 64 and 128: 512 x
-    // 4096 x 1024 6.9 and 8.6 us, 1024 x 4096 x 1024 12.2 and 9.5.
+    // Otherwise the smallest tiles that are done at once, with two of 64 or one of 128 per CU.  Tiles of 64 and 128: 512 x 4096 x 1024
+    // 6.9 and 8.6 us, 1024 x 4096 x 1024 12.2 and 9.5; of 128 and 256: 2048 x 2048 x 2048 16.5 and 20.2, 2000 x 1500 x 4096 23.9
+    // and 33.4, but where the CUs have a second one of 128, 1500 x 3000 x 1000 17.3 and 14.5, 2048 x 2560 x 2048 24.9 and 19.4.
     const auto busiest = [&](int mt) { return ((p.N + 15ll) / 16 * ((p.M + 16ll * mt - 1) / (16 * mt)) + cus - 1) / cus * (16 + 16 * mt) * 3 / 2; };
     const long long r1 = busiest(1), r2 = busiest(2), r4 = busiest(4), least = std::min(r1, std::min(r2, r4));
-    const int kind = p.M <= 65536 && p.N <= 1 << 26 && least <= (t64 + cus - 1) / cus * 128 ? 1 : t256 >= cus * 3 / 8 ? 4 : t64 > 2 * cus ? 3 : 2;
+    const int kind = p.M <= 65536 && p.N <= 1 << 26 && least <= (t64 + cus - 1) / cus * 128 ? 1 : t128 > cus ? 4 : t64 > 2 * cus ? 3 : 2;
     if (kind == 1) {
         const int mt = least == r1 ? 1 : least == r2 ? 2 : 4;
         const dim3 grid(cdiv(p.N, 16), cdiv(p.M, 16 * mt));
@@ -603,8 +603,8 @@ template <typename TC> int launch_gemm_i8(const Params8& p, hipStream_t st) {
     } else if (kind == 3) {
         hipLaunchKernelGGL((gemm_i8_tile_kernel<128, 128, 8, TC>), dim3((unsigned)t128), dim3(512), 0, st, p, cdiv(p.M, 128), cdiv(p.N, 128));
     } else {
-        // a last round of at most half the CUs' tiles is cut into half tiles (4096 x 5120 x 2048: 51.6 us, whole ones 53.3; 8192 x
-        // 4352 x 1024: 48.5 and 50.1)
+        // a last round of at most half the CUs' tiles is cut into half tiles (4096 x 5120 x 2048: 49.6 us, whole ones 50.6; 8192 x
+        // 4352 x 1024: 47.2 and 49.8)
         const int tail = (int)(t256 % cus);
         const int whole = tail && tail <= cus / 2 ? (int)t256 - tail : (int)t256, units = whole + 2 * ((int)t256 - whole);
         if (p.K % 16)
