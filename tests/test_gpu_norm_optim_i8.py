@@ -1007,3 +1007,22 @@ def test_written_tensors_and_moved_states(ops):
     with pytest.raises(ValueError, match="memory"):
         ops.adamw_multi(args, [torch.ones(300, device=DEV)], step, 1e-3)
     assert int(step) == 1
+
+
+@pytest.mark.parametrize("M,N", [(8192, 6400), (8000, 6500)])
+@pytest.mark.parametrize("K", [128, 256, 300, 640, 1024])
+def test_gemm_i8_many_tiles_per_workgroup(ops, M, N, K):
+    """a workgroup's tiles follow one another with loads and stores of the last one under way: whole tiles behind whole and cut ones, one to
+    eight slabs, both types of C, the same bits every time"""
+    A, W, sa, sw, b = [t.to(DEV) for t in operands(M, N, K, seed=M + K)]
+    prod = A[:, :K].double() @ W[:, :K].double().t().contiguous()
+    prod *= sa.double().view(-1, 1)
+    prod *= sw.double()
+    for ct in (torch.float32, torch.bfloat16):
+        for bias in (b, None):
+            want = prod + bias.double() if bias is not None else prod
+            y = ops.gemm_i8(A[:, :K], sa, W[:, :K], sw, bias, out_dtype=ct)
+            off = (y.double() - want).abs() - 4 * U * (prod.abs() + want.abs()) - half_step(y) * want.abs() * 1.001
+            assert float(off.max()) <= 0, (ct, float(off.max()))
+            for _ in range(8):
+                assert torch.equal(ops.gemm_i8(A[:, :K], sa, W[:, :K], sw, bias, out_dtype=ct), y)
