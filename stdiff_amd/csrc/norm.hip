@@ -331,10 +331,13 @@ __global__ __launch_bounds__(512) void layer_norm_bwd_few_kernel(const TD* dy, l
                                                       (long long)(gridDim.x - cols) * ROWS, aw, ab);
         return;
     }
+    // workgroups b and b + 8 share an XCD's L2: they own neighbouring columns, which share lines (1200 x 4096
+    // bf16 12.9 -> 10.7 us, 2077 x 1001 11.4 -> 10.9)
+    const int b = blockIdx.x, group = b < (cols & ~15) ? (b & ~15) | (b & 7) << 1 | (b >> 3 & 1) : b;
     constexpr int LANES = 32 / V, SLOTS = 512 / LANES;
     __shared__ float sums[2][SLOTS][32 + 1];
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
-    const span<V> at(blockIdx.x * 32 + lane * V, H);
+    const span<V> at(group * 32 + lane * V, H);
     float aw[V], ab[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) aw[j] = ab[j] = 0.f;
@@ -358,7 +361,7 @@ __global__ __launch_bounds__(512) void layer_norm_bwd_few_kernel(const TD* dy, l
     __syncthreads();
     // 64 sums (two of 32 columns) of SLOTS terms each: eight threads per sum, then their eight in order
     const int col = threadIdx.x & 31, which = (threadIdx.x >> 5) & 1, share = threadIdx.x >> 6;
-    const int from = min(col + (blockIdx.x * 32 + col >= H / V * V ? (V - H % V) % V : 0), 31);
+    const int from = min(col + (group * 32 + col >= H / V * V ? (V - H % V) % V : 0), 31);
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < SLOTS / 8; ++i) s += sums[which][share * (SLOTS / 8) + i][from];
@@ -366,10 +369,10 @@ __global__ __launch_bounds__(512) void layer_norm_bwd_few_kernel(const TD* dy, l
     sums[which][share][col] = s;
     __syncthreads();
     float* dst = which ? dbias : dweight;
-    if (share || !dst || blockIdx.x * 32 + col >= H) return;
+    if (share || !dst || group * 32 + col >= H) return;
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += sums[which][i][col];
-    dst += blockIdx.x * 32 + col;
+    dst += group * 32 + col;
     *dst = accumulate ? *dst + s : s;
 }
 
