@@ -479,10 +479,10 @@ inline bool past_caches(long long bytes) { return bytes > (256ll << 20); }
 inline int lanes_of(int H) { return H <= 128 ? 8 : H <= 512 ? 32 : H <= 1024 ? 64 : BLOCK; }
 inline int threads_of(int H) { return H <= 1024 ? 256 : cdiv(H, 1024) * 64; }
 inline int rows_of_block(int H) { return H <= 1024 ? 256 / lanes_of(H) : 1; }
-// Few rows: the column sums walk down the rows in the launch that gives dx.  A workgroup reads 32 columns of all rows, and a CU draws
-// about 45 GB/s from the L2: up to 320 KB cost 7 us, which is what the second launch, the workspace and the partial sums
-// cost (512 x 1024 bf16: 4.0 us against 8.3; 1024 x 1024 fp32: 7.0 against 8.7; 2077 x 1001 fp16: 11.3 against 9.4, but 13.4
-// against 17.5 where the host launches; 2048 x 1024 fp32: 16 against 10).
+// Few rows: the column sums walk down the rows in the launch that gives dx.  A workgroup reads 32 columns of all rows: up to 320 KB that is
+// better than the second launch, the workspace and the partial sums (us per call, one and two launches: 512 x 1024 bf16 5.6
+// and 9.5, 1024 x 1024 fp32 5.7 and 10.0, 1200 x 4096 bf16 10.7 and 16.2, 2500 x 1024 bf16 7.4 and 10.3; rows that begin anywhere,
+// 2077 x 1001 bf16, 10.6 and 9.8; behind the limit, 4096 x 1024 bf16, 21 and 11).
 inline bool one_launch(int R, int H, int x_size, int dy_size) {
     return (long long)R * 32 * (x_size + dy_size) <= 320 << 10 && H >= 8 && H <= 8192;
 }
