@@ -358,9 +358,14 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(B b, update_arg a) {
 
 inline bool at_bytes(const void* p, int size) { return ((uintptr_t)p & (size - 1)) == 0; }
 inline int max_blocks() { return 4 * cu_count(); }
-// Workgroups per CU of the update: four, for what is larger than the caches by far two, whose fewer streams suit the memory
-// better (8-bit states, 30 M elements: four 99, two 113 us; 479 M: 1515 and 1436 us; 32-bit, 120 M: 649 and 645 us)
-inline int update_blocks(long long elements) { return (elements > (1ll << 26) ? 2 : 4) * cu_count(); }
+// Workgroups per CU of the update: four, but where the data are much, as few as keep the memory busy: fewer streams suit it better.
+// 32-bit states, four and one: 5 M elements 26.6 and 27.1 us, 10 M 53.3 and 52.1, 30 M 157 and 146, two and one: 120 M 633 and 601.
+// 8-bit states, whose codes cost instructions: 60 M four 183, two with half the elements each 181; 470 M two 1442, two with half
+// 1339, one 1675.
+inline bool much8(long long elements) { return elements > (1ll << 26); }
+inline int update_blocks(int bits, long long elements) {
+    return (bits == 32 ? elements > (1ll << 23) ? 1 : 4 : much8(elements) ? 2 : 4) * cu_count();
+}
 
 void set_tensor(tensor32& t, const stdiff_adamw_tensor& s) {
     t.p = s.param; t.g = s.grad; t.m = (float*)s.exp_avg; t.v = (float*)s.exp_avg_sq; t.n = s.n; t.wd = s.weight_decay;
@@ -395,7 +400,7 @@ template <int BITS, int U, typename B> int update(const stdiff_adamw_multi_args*
     for (int at = 0; at < a->n_tensors;) {
         const int chunks = fill(a, &at, U * 1024, &b);
         if (!chunks) continue;
-        hipLaunchKernelGGL((adamw_update_kernel<BITS, U, B>), dim3(std::min(chunks, update_blocks(total))), dim3(256), 0, st, b, u);
+        hipLaunchKernelGGL((adamw_update_kernel<BITS, U, B>), dim3(std::min(chunks, update_blocks(BITS, total))), dim3(256), 0, st, b, u);
         STDIFF_LAUNCH_STATUS();
     }
     return STDIFF_OK;
@@ -469,6 +474,7 @@ extern "C" int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream
     // turns of 1024 elements instead of 4096 spread little work over all CUs (32 tensors of 1000: 8.7 against 11.5 us, of 20000: 9.4
     // and 10.7; 8 of 200000: 13.1 and 12.5, with 8-bit states 12.3 and 13.0)
     const bool few = total < 4096ll * 2 * cu_count();
+    if (a->state_bits == 8 && much8(total)) return update<8, 2, batch8>(a, u, total, st);
     if (a->state_bits == 8) return few ? update<8, 1, batch8>(a, u, total, st) : update<8, 4, batch8>(a, u, total, st);
     return few ? update<32, 1, batch32>(a, u, total, st) : update<32, 4, batch32>(a, u, total, st);
 }
