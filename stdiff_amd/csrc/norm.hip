@@ -517,7 +517,12 @@ int launch_ln(const void* x, long long ldx, const void* w, const void* b, float 
               float* rstd, int R, int H, hipStream_t st) {
     constexpr int V = sizeof(TX) == 2 ? 8 : 4;
     const bool streams = past_caches((long long)R * H * (sizeof(TX) + sizeof(TY)));
-    const dim3 grid(norm_blocks(R, rows_of_block(H), 2048 / threads_of(std::min(H, IN_REGISTERS)))), block(threads_of(H));
+    // all the threads that a CU holds; past the caches fewer streams suit the memory better: sixteen waves (262144 x 300 bf16 76 -> 69
+    // us, 131072 x 1024 bf16 102 -> 99), for fp32 rows eight or two workgroups (131072 x 1024 -> bf16 140 -> 131, 65536 x 2048 197 -> 180,
+    // 16384 x 8192 -> bf16 142 -> 127, one workgroup 166)
+    const int threads = threads_of(std::min(H, IN_REGISTERS));
+    const int per_cu = !streams ? 2048 / threads : V == 8 ? 1024 / threads : std::max(2, 512 / threads);
+    const dim3 grid(norm_blocks(R, rows_of_block(H), per_cu)), block(threads_of(H));
 #define LN_AT(T, NT)                                                                                                           \
     hipLaunchKernelGGL((layer_norm_kernel<TX, TY, TW, V, T, NT>), grid, block, 0, st, (const TX*)x, ldx, (const TW*)w, (const TW*)b, eps, \
                        (TY*)y, ldy, mean, rstd, R, H)
