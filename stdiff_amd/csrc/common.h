@@ -181,17 +181,21 @@ __device__ __forceinline__ float wave_max(float v) {
 // between rows.  The same result in all lanes.  (Another order of additions than wave_sum's.)
 #define STDIFF_DPP(v, ctrl) __builtin_amdgcn_update_dpp(0, (int)(v), ctrl, 0xf, 0xf, true)
 typedef unsigned u32x2_swap __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) {
+// over groups of T lanes
+template <int T> __device__ __forceinline__ unsigned lanes_umax_dpp(unsigned v) {
+    static_assert(T == 8 || T == 32 || T == 64, "");
     v = max(v, (unsigned)STDIFF_DPP(v, 0xb1));        // lanes 1 apart
     v = max(v, (unsigned)STDIFF_DPP(v, 0x4e));        // 2
     v = max(v, (unsigned)STDIFF_DPP(v, 0x141));       // mirror of eight
+    if (T == 8) return v;
     v = max(v, (unsigned)STDIFF_DPP(v, 0x140));       // mirror of sixteen
     u32x2_swap s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = max(s[0], s[1]);
+    if (T == 32) return v;
     s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return max(s[0], s[1]);
 }
-// over groups of T lanes
+__device__ __forceinline__ unsigned wave_umax_dpp(unsigned v) { return lanes_umax_dpp<64>(v); }
 template <int T> __device__ __forceinline__ float lanes_sum_dpp(float v) {
     static_assert(T == 8 || T == 32, "");
 #define STDIFF_DPP_ADD(ctrl) v += __builtin_bit_cast(float, STDIFF_DPP(__builtin_bit_cast(int, v), ctrl))

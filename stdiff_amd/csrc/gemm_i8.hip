@@ -4,7 +4,7 @@
 // The sum over k is exact: int32 holds K * 127 * 127 up to K = 133143 (and K * 128 * 128 up to 131071, the limit here).  The
 // scales are applied to the finished sum in fp32, the weight's first: sum * a_scale would overflow for activations above
 // 1e31 whose product with a weight is still a number.
-// Measured: quantisation of 65536 x 2048 bf16 76 us (5.3 TB/s of the 5.9 that a copy of this file's kind reaches), of 4 rows 2.1 us; product
+// Measured: quantisation of 65536 x 2048 bf16 71 us (5.6 TB/s), of 4 rows 2.1 us; product
 // of 4 x 4096 x 1024 3.8 us (a launch, one trip to memory and one barrier), of 65536 x 8192 x 2048 892 us (2.47 POP/s; 8192 x
 // 8192 x 8192 2.85): the matrix units are busy 61 % of the cycles, and the clock falls to 1.94 GHz.
 #include "common.h"
@@ -19,9 +19,11 @@ typedef u32x2 u32x2_u __attribute__((aligned(2)));
 // ---------------------------------------------------------------- row quantisation
 __device__ __forceinline__ unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
-__device__ __forceinline__ void ld8(const float* p, int k, float* o) {
+// NT: past the caches
+template <bool NT = false> __device__ __forceinline__ void ld8(const float* p, int k, float* o) {
     if (k >= 8) {
-        const f32x4 a = *(const f32x4_u*)p, b = *(const f32x4_u*)(p + 4);
+        const f32x4 a = NT ? __builtin_nontemporal_load((const f32x4_u*)p) : *(const f32x4_u*)p;
+        const f32x4 b = NT ? __builtin_nontemporal_load((const f32x4_u*)(p + 4)) : *(const f32x4_u*)(p + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { o[j] = a[j]; o[4 + j] = b[j]; }
     } else {
@@ -29,9 +31,9 @@ __device__ __forceinline__ void ld8(const float* p, int k, float* o) {
         for (int j = 0; j < 8; ++j) o[j] = j < k ? p[j] : 0.f;
     }
 }
-__device__ __forceinline__ void ld8(const bf16_t* p, int k, float* o) {
+template <bool NT = false> __device__ __forceinline__ void ld8(const bf16_t* p, int k, float* o) {
     if (k >= 8) {
-        const u32x4 v = *(const u32x4_u*)p;
+        const u32x4 v = NT ? __builtin_nontemporal_load((const u32x4_u*)p) : *(const u32x4_u*)p;
 #pragma unroll
         for (int j = 0; j < 4; ++j) { o[2 * j] = bf_lo(v[j]); o[2 * j + 1] = bf_hi(v[j]); }
     } else {
@@ -56,7 +58,7 @@ __device__ __forceinline__ u32x2 to_i8(const float* v, float f) {
     return u32x2{o[0], o[1]};
 }
 template <int T> __device__ __forceinline__ unsigned row_max(unsigned top, unsigned* part) {
-    top = wave_umax_dpp(top);
+    top = lanes_umax_dpp<T < 64 ? T : 64>(top);
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
         __syncthreads();
@@ -67,7 +69,7 @@ template <int T> __device__ __forceinline__ unsigned row_max(unsigned top, unsig
 }
 
 // a row stays in the registers of T lanes, eight elements per lane and vector
-template <typename TX, int NV, int T>
+template <typename TX, int NV, int T, bool NT>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const TX* x, long long ldx, signed char* q, long long ldq, float* scale,
                                                             int R, int K) {
     __shared__ unsigned part[2][4];
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const TX* x, long lo
         float v[NV][8], s;
         unsigned top = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) ld8(x + row * ldx + (i * T + t) * 8, K - (i * T + t) * 8, v[i]);
+        for (int i = 0; i < NV; ++i) ld8<NT>(x + row * ldx + (i * T + t) * 8, K - (i * T + t) * 8, v[i]);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -115,12 +117,22 @@ __global__ __launch_bounds__(256) void quantize_rows_long_kernel(const TX* x, lo
 
 template <typename TX>
 int launch_quantize(const void* x, long long ldx, void* q, long long ldq, float* scale, int R, int K, hipStream_t st) {
-#define QR(NV, T)                                                                                                              \
-    hipLaunchKernelGGL((quantize_rows_kernel<TX, NV, T>), dim3((unsigned)std::min<long long>((R + 256 / T - 1ll) / (256 / T), 8ll * cu_count())), \
+    // 16-bit rows that are larger than the memory-side cache (256 MB) go past the caches (65536 x 4096 bf16: 126 us, through them 148;
+    // 200000 x 300, which it holds: 72 and 50; fp32 rows are read in two pieces per lane, 65536 x 1024: 64 and 59)
+    const bool streams = sizeof(TX) == 2 && (long long)R * K * 3 > (256ll << 20);
+#define QR_AT(NV, T, NT)                                                                                                       \
+    hipLaunchKernelGGL((quantize_rows_kernel<TX, NV, T, NT>), dim3((unsigned)std::min<long long>((R + 256 / T - 1ll) / (256 / T), 8ll * cu_count())), \
                        dim3(256), 0, st, (const TX*)x, ldx, (signed char*)q, ldq, scale, R, K)
-    // a wave per row up to 1024 columns, then the workgroup (65536 x 1024 bf16: a wave 31.7 us, the workgroup the same, but 4 rows 2.4
-    // and 2.9; 65536 x 2048: 80 and 76, 4 rows 3.0 and 2.4)
-    if (K <= 512) QR(1, 64);
+#define QR(NV, T)                                                              \
+    do {                                                                       \
+        if (streams) QR_AT(NV, T, sizeof(TX) == 2);                            \
+        else QR_AT(NV, T, false);                                              \
+    } while (0)
+    // 8, 32 or 64 lanes per row up to 1024 columns (400000 x 128 bf16: 8 lanes 25 us, a wave 74; 200000 x 300: 32 lanes 36, a wave
+    // 50), then the workgroup (65536 x 1024 bf16: a wave 31.7 us, the workgroup the same, but 4
+    // rows 2.4 and 2.9; 65536 x 2048: 80 and 76, 4 rows 3.0 and 2.4)
+    if (K <= 128) QR(2, 8);
+    else if (K <= 512) QR(2, 32);
     else if (K <= 1024) QR(2, 64);
     else if (K <= 2048) QR(1, 256);
     else if (K <= 4096) QR(2, 256);
@@ -129,6 +141,7 @@ int launch_quantize(const void* x, long long ldx, void* q, long long ldq, float*
         hipLaunchKernelGGL(quantize_rows_long_kernel<TX>, dim3((unsigned)std::min<long long>(R, 8ll * cu_count())), dim3(256), 0, st,
                            (const TX*)x, ldx, (signed char*)q, ldq, scale, R, K);
 #undef QR
+#undef QR_AT
     STDIFF_LAUNCH_STATUS();
     return STDIFF_OK;
 }

@@ -1026,3 +1026,17 @@ def test_gemm_i8_many_tiles_per_workgroup(ops, M, N, K):
             assert float(off.max()) <= 0, (ct, float(off.max()))
             for _ in range(8):
                 assert torch.equal(ops.gemm_i8(A[:, :K], sa, W[:, :K], sw, bias, out_dtype=ct), y)
+
+
+@pytest.mark.parametrize("xt", ["fp32", "bf16"])
+@pytest.mark.parametrize("R,K", [(1000, 3), (999, 64), (1001, 100), (517, 128), (515, 129), (1003, 300), (301, 512), (300, 513), (90000, 1000), (3, 1025), (70, 2048), (45000, 2100)])
+def test_quantize_rows_groups_of_lanes(ops, R, K, xt):
+    """rows that share a wave, rows of a workgroup, and more than a cache holds: q and scale as the formula has them, padding zero"""
+    x = torch.randn(R, K, device=DEV, generator=torch.Generator(DEV).manual_seed(R + K)).to(DT[xt])
+    x[R // 2] = 0
+    q, s = ops.quantize_rows(x)
+    top = x.float().abs().amax(1, keepdim=True)
+    want = torch.round(x.float() * torch.where(top > 0, torch.full_like(top, 127.0) / top, torch.zeros_like(top)))
+    assert torch.equal(s, (top / torch.full_like(top, 127.0)).view(-1)) and torch.equal(q.float(), want)
+    kp = -(-K // 16) * 16
+    assert not bool(torch.as_strided(q, (R, kp), (kp, 1))[:, K:].any())
