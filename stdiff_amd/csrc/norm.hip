@@ -11,8 +11,8 @@
 // them out of the sums and stores them a second time with the same bits.  (Element by element, the 7 elements at the end
 // of rows of 999 cost 0.8 of the time of all others.)
 // Bound by memory where there are many rows, by launch and one trip to memory where there are few: forward of one row of
-// 1024 1.8 us, of 131072 x 1024 fp32 -> bf16 139 us (5.8 TB/s), backward of 32768 x 2048 fp32 138 + 5 us for the partial sums (5.7
-// TB/s), of 512 x 1024 bf16 3.7 us in one launch.
+// 1024 1.8 us, of 131072 x 1024 fp32 -> bf16 130 us (6.2 TB/s), backward of 32768 x 2048 fp32 135 + 5 us for the partial sums (5.8
+// TB/s), of 512 x 1024 bf16 3.5 us in one launch.
 // The variance is formed from the centred values (a second walk over the registers), so a row whose mean is far larger
 // than its spread keeps its digits.  All statistics and sums are fp32.
 #include "common.h"
@@ -473,8 +473,9 @@ inline bool in_registers(int H) { return H >= 8 && H <= IN_REGISTERS; }
 inline int norm_blocks(long long R, int rows_per_block, int per_cu) {
     return (int)std::min<long long>((R + rows_per_block - 1) / rows_per_block, (long long)per_cu * cu_count());
 }
-// A call that moves more than the memory-side cache holds (256 MB) goes past the caches: 131072 x 1024 fp32 -> bf16 146 against
-// 155 us, backward of 32768 x 2048 fp32 139 against 150 us.  Below that the next kernel finds the result in a cache.
+// A call that moves more than the memory-side cache holds (256 MB) goes past the caches: 131072 x 1024 fp32 -> bf16 131 against
+// 152 us, backward of 32768 x 2048 fp32 141 against 154, 262144 x 300 bf16 70 against 66.  Below that the next kernel finds the result in a
+// cache.
 inline bool past_caches(long long bytes) { return bytes > (256ll << 20); }
 inline int lanes_of(int H) { return H <= 128 ? 8 : H <= 512 ? 32 : H <= 1024 ? 64 : BLOCK; }
 inline int threads_of(int H) { return H <= 1024 ? 256 : cdiv(H, 1024) * 64; }

@@ -8,8 +8,8 @@
 // code (2^-9): it never becomes zero beside a first moment that is not, which would divide by eps alone.  The largest of a
 // block keeps fp32 precision through its scale, so a block whose elements grow evenly keeps its codes and none stands
 // still under the slow decay of v.  The step itself uses m and v before they are rounded.
-// Bound by memory: 120 M parameters in 32 bits 81 us for the norm (5.9 TB/s) and 565 for the step (5.9 TB/s), 30 M with 8-bit states
-// 14 and 88 us (5.0 TB/s; 230 vector instructions per 256 elements keep the vector units busy 56 % of it), 479 M 1447 us together.  Small models are two launches
+// Bound by memory: 120 M parameters in 32 bits 82 us for the norm (5.8 TB/s) and 547 for the step (6.1 TB/s), 30 M with 8-bit states
+// 14 and 86 us (5.0 TB/s; 230 vector instructions per 256 elements keep the vector units busy 56 % of it), 479 M 1386 us together.  Small models are two launches
 // of 4.6 and 6.1 us: the table, the data, for the step also the partial sums, one trip to memory each.
 // A block that holds an infinity or a NaN gets a scale that is not finite: all its elements are NaN from the next step on.
 #include <float.h>
