@@ -203,15 +203,11 @@ __device__ __forceinline__ f32x4 scaled(i32x4 sum, float as, f32x4 ws, f32x4 b) 
 __device__ __forceinline__ void put4(float* p, f32x4 v) { *(f32x4*)p = v; }
 __device__ __forceinline__ void put4(bf16_t* p, f32x4 v) { *(u32x2*)p = u32x2{pack2bf(v[0], v[1]), pack2bf(v[2], v[3])}; }
 // 16 bytes of a row of C, which may begin at any element and end inside the piece
-template <bool NT, typename TC> __device__ __forceinline__ void store16(TC* row, int n, int N, u32x4 v) {
+template <typename TC> __device__ __forceinline__ void store16(TC* row, int n, int N, u32x4 v) {
     constexpr int E = 16 / sizeof(TC);
     if (n + E <= N) {
         if constexpr (sizeof(TC) == 4) {
-            const f32x4 o = __builtin_bit_cast(f32x4, v);
-            if (NT) __builtin_nontemporal_store(o, (f32x4_u*)(row + n));
-            else *(f32x4_u*)(row + n) = o;
-        } else if (NT) {
-            __builtin_nontemporal_store(v, (u32x4_u*)(row + n));
+            *(f32x4_u*)(row + n) = __builtin_bit_cast(f32x4, v);
         } else {
             *(u32x4_u*)(row + n) = v;
         }
@@ -370,7 +366,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_tile_kernel(Params8 p, int ti
 #pragma unroll 4
     for (int i = tid; i < BM * PIECES; i += NW * 64) {
         const int m = i / PIECES, c = i % PIECES;
-        if (m0 + m < p.M) store16<false>((TC*)p.C + (m0 + m) * p.ldc, n0 + c * (16 / (int)sizeof(TC)), p.N, *(const u32x4*)(smem + m * ROW + c * 16));
+        if (m0 + m < p.M) store16((TC*)p.C + (m0 + m) * p.ldc, n0 + c * (16 / (int)sizeof(TC)), p.N, *(const u32x4*)(smem + m * ROW + c * 16));
     }
 }
 
@@ -382,8 +378,8 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_tile_kernel(Params8 p, int ti
 // All of LDS is one array: with another for the scales the compiler lets every read wait for all DMA under way.
 // Measured per tile: 1.43 us for a slab (the instructions alone 1.06 at the clock that they leave), 5 us for C, half of it conversions and
 // scales.  The stores of C are under way during the next tile's first slab: the counted waits know how many they are.
-// TAIL: K is no multiple of 16.  (A form of its own: the kernel uses all 256 registers, and the masks cost some.)
-template <typename TC, bool TAIL>
+// PAST: C goes past the caches.  TAIL: K is no multiple of 16.  (A form of its own: the kernel uses all 256 registers, and the masks cost some.)
+template <typename TC, bool TAIL, bool PAST>
 __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tiles_m, int tiles_n, int whole, int units) {
     constexpr int HALF = 128 * SLAB;
     constexpr int SCALES = 9 * HALF;
@@ -574,8 +570,12 @@ __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tile
                 const int r = (tid + 512 * i) / PIECES, c = (tid + 512 * i) % PIECES;
                 const int m = em + (e >> 2) * 128 + (r >> 4) * 64 + (e & 3) * 16 + (r & 15), n = en + c * (16 / (int)sizeof(TC));
                 TC* row = (TC*)p.C + m * p.ldc;
-                if (behind) __builtin_nontemporal_store(v[i], (u32x4_u*)(row + n));
-                else if (m < p.M) store16<true>(row, n, p.N, v[i]);
+                if (behind) {
+                    if (PAST) __builtin_nontemporal_store(v[i], (u32x4_u*)(row + n));
+                    else *(u32x4_u*)(row + n) = v[i];
+                } else if (m < p.M) {
+                    store16(row, n, p.N, v[i]);
+                }
             }
             if (e == 3) {                                               // the next tile's scales are here
                 float* then = scales + (side ^ 1) * 768;
@@ -620,12 +620,21 @@ template <typename TC> int launch_gemm_i8(const Params8& p, hipStream_t st) {
         // 4352 x 1024: 47.2 and 49.8)
         const int tail = (int)(t256 % cus);
         const int whole = tail && tail <= cus / 2 ? (int)t256 - tail : (int)t256, units = whole + 2 * ((int)t256 - whole);
-        if (p.K % 16)
-            hipLaunchKernelGGL((gemm_i8_256_kernel<TC, true>), dim3(std::min(units, cus)), dim3(512), 0, st, p, cdiv(p.M, 256),
-                               cdiv(p.N, 256), whole, units);
-        else
-            hipLaunchKernelGGL((gemm_i8_256_kernel<TC, false>), dim3(std::min(units, cus)), dim3(512), 0, st, p, cdiv(p.M, 256),
-                               cdiv(p.N, 256), whole, units);
+        // Past the caches, but where rows begin inside cache lines and the caches hold most of C: its lines are whole before they leave
+        // (26628 x 3464 x 64 -> fp32, 369 MB: 101 us past the caches, 85 through them, -> bf16 63 and 43; 25055 x 5127 x 449 -> fp32,
+        // 514 MB: 171 and 176; whole lines, 131072 x 4096 x 128 -> bf16: 209 and 252).
+        const bool past = (((uintptr_t)p.C | (uintptr_t)(p.ldc * sizeof(TC))) & 127) == 0 || (long long)p.M * p.N * (long long)sizeof(TC) > (400ll << 20);
+#define TILES(TAIL, PAST)                                                                                                      \
+    hipLaunchKernelGGL((gemm_i8_256_kernel<TC, TAIL, PAST>), dim3(std::min(units, cus)), dim3(512), 0, st, p, cdiv(p.M, 256),  \
+                       cdiv(p.N, 256), whole, units)
+        if (p.K % 16) {
+            if (past) TILES(true, true);
+            else TILES(true, false);
+        } else {
+            if (past) TILES(false, true);
+            else TILES(false, false);
+        }
+#undef TILES
     }
     STDIFF_LAUNCH_STATUS();
     return STDIFF_OK;
