@@ -5,8 +5,8 @@
 // scales are applied to the finished sum in fp32, the weight's first: sum * a_scale would overflow for activations above
 // 1e31 whose product with a weight is still a number.
 // Measured: quantisation of 65536 x 2048 bf16 71 us (5.6 TB/s), of 4 rows 2.1 us; product
-// of 4 x 4096 x 1024 3.8 us (a launch, one trip to memory and one barrier), of 65536 x 8192 x 2048 892 us (2.47 POP/s; 8192 x
-// 8192 x 8192 2.85): the matrix units are busy 61 % of the cycles, and the clock falls to 1.94 GHz.
+// of 4 x 4096 x 1024 3.8 us (a launch, one trip to memory and one barrier), of 65536 x 8192 x 2048 865 us (2.54 POP/s; 8192 x
+// 8192 x 8192 2.97): the matrix units are busy 69 % of the cycles, and the clock falls to 1.9 GHz.
 #include "common.h"
 
 namespace {
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_tile_kernel(Params8 p, int ti
 // waves 4-7 run one barrier behind waves 0-3, so that on every SIMD one wave multiplies while the other reads.  The
 // first loads of the next tile are issued before C leaves through the buffers that they do not use.
 // All of LDS is one array: with another for the scales the compiler lets every read wait for all DMA under way.
-// Measured per tile: 1.43 us for a slab (the instructions alone 1.06 at the clock that they leave), 5 us for C, half of it conversions and
+// Measured per tile: 1.36 us for a slab (the instructions alone 1.1 at the clock that they leave), 5 us for C, half of it conversions and
 // scales.  The stores of C are under way during the next tile's first slab: the counted waits know how many they are.
 // PAST: C goes past the caches.  TAIL: K is no multiple of 16.  (A form of its own: the kernel uses all 256 registers, and the masks cost some.)
 template <typename TC, bool TAIL, bool PAST>
