@@ -466,7 +466,7 @@ def concurrent_streams(device, n, candidates=12, spin_us=500):
 # Why they are not drawn afresh from torch's pool of 32 per object: a HIP stream that has carried a deep queue of graph
 # replays keeps its pool of completion signals (KFD interrupt events) for the life of the process, and once about 21
 # DIFFERENT streams of a process had done so, no new GPU process could start on that GPU: its hsa_init failed to create
-# its first event and ROCr's async-events thread dereferenced the null HsaEvent (SIGSEGV; scripts/diag/, DESIGN.md 6a').
+# its first event and ROCr's async-events thread dereferenced the null HsaEvent (SIGSEGV).
 # A 5-fold run through both 16-bit formats made 30 such streams.  With the cache a process uses 2 (lanes) + 1 (side).
 _STREAMS = {}
 
