@@ -543,7 +543,7 @@ int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream);
  * zeros.  A row that holds an infinity or a NaN gets a scale that is not finite. */
 int stdiff_quantize_rows(const void* x, long long ldx, int x_dtype, void* q, long long ldq, float* scale, int R, int K, void* stream);
 /* C[M,N] = (sum_k A[m,k] W[n,k]) * w_scale[n] * a_scale[m] + bias[n]   (A, W int8; the sum exact in int32, K <= 131071;
- * bias may be NULL; C fp32 or 16-bit).  A and W 16-byte aligned, lda / ldw % 16 == 0 and >= round_up(K, 16): a row is read
+ * bias may be NULL; C fp32 or 16-bit; M and N <= 2^30).  A and W 16-byte aligned, lda / ldw % 16 == 0 and >= round_up(K, 16): a row is read
  * up to round_up(K, 16), what stands behind K does not matter. */
 typedef struct {
     int M, N, K;

@@ -657,7 +657,7 @@ extern "C" int stdiff_gemm_i8(const stdiff_gemm_i8_args* a, void* stream) {
     STDIFF_CHECK_ARG(a && a->M >= 0 && a->N >= 0 && a->K > 0 && (a->c_dtype == STDIFF_F32 || a->c_dtype == STDIFF_BF16));
     if (a->M == 0 || a->N == 0) return STDIFF_OK;
     STDIFF_CHECK_ARG(a->A && a->W && a->a_scale && a->w_scale && a->C && a->ldc >= a->N);
-    if (a->K > 131071) return STDIFF_ERR_SHAPE;
+    if (a->K > 131071 || a->M > (1 << 30) || a->N > (1 << 30)) return STDIFF_ERR_SHAPE;      // a tile behind the last row or column: still 32 bits
     const long long kp = (a->K + 15) / 16 * 16;
     STDIFF_CHECK_ARG(a->lda >= kp && a->ldw >= kp);
     if (a->lda > (1 << 23) || a->ldw > (1 << 23)) return STDIFF_ERR_SHAPE;

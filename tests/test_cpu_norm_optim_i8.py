@@ -256,3 +256,17 @@ def test_without_the_extension_module(tmp_path):
             "except RuntimeError as e: print('refused', e)\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0 and "refused stdiff_amd/_bind.so cannot be used" in r.stdout, r.stderr
+
+
+def test_largest_products(lib):
+    """rows and columns of C are counted in 32 bits with a tile behind them: more than 2^30 of either are refused"""
+    from stdiff_amd import _lib as L
+    for M, N in (((1 << 30) + 1, 8), (8, (1 << 30) + 1), (2**31 - 1, 1), (1, 2**31 - 1)):
+        a = L.GemmI8Args()
+        a.M, a.N, a.K = M, N, 16
+        a.A = a.W = a.a_scale = a.w_scale = a.C = AT
+        a.lda = a.ldw = 16
+        a.ldc = N
+        for c_dtype in (0, 1):
+            a.c_dtype = c_dtype
+            assert lib.stdiff_gemm_i8(C.byref(a), None) == SHAPE, (M, N, c_dtype)
