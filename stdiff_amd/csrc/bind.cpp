@@ -128,12 +128,12 @@ int64_t rows16(const Tensor& t, const char* name) {
 }
 
 // Outputs share no memory with what a call reads, but where an operator may work in place: then they are the same elements.
-// (Side by side in the rows of one buffer they are apart.)
-void keep_apart(const Tensor& out, const char* name, int64_t ldo, const Tensor& in, const char* other, int64_t ldi, bool in_place) {
+// (Side by side in the rows of one buffer they are apart.)  columns: how many of a row of `out` are written, its padding included.
+void keep_apart(const Tensor& out, const char* name, int64_t ldo, int64_t columns, const Tensor& in, const char* other, int64_t ldi, bool in_place) {
     if (!out.numel() || !in.numel()) return;
     const int64_t rows = out.size(0), so = out.element_size(), si = in.element_size();
     const uintptr_t p = (uintptr_t)out.data_ptr(), q = (uintptr_t)in.data_ptr();
-    const int64_t lp = ldo * so, lq = ldi * si, wp = out.size(1) * so, wq = in.size(1) * si;
+    const int64_t lp = ldo * so, lq = ldi * si, wp = columns * so, wq = in.size(1) * si;
     if (p + (rows - 1) * lp + wp <= q || q + (in.size(0) - 1) * lq + wq <= p) return;
     if (in_place && p == q && lp == lq && out.scalar_type() == in.scalar_type()) return;
     if (lp == lq) {
@@ -205,7 +205,7 @@ PyObject* layer_norm(PyObject* const* a) {
     if (w && b && w->scalar_type() != b->scalar_type())
         refuse(PyExc_TypeError, "weight is ", w->scalar_type(), ", bias ", b->scalar_type(), ": one dtype is needed");
     void *wp = vector(w, "weight", H, true), *bp = vector(b, "bias", H, true), *mp = vector(mean, "mean", R), *rp = vector(rstd, "rstd", R);
-    if (given) keep_apart(*given, "out", ldy, x, "x", ldx, true);
+    if (given) keep_apart(*given, "out", ldy, H, x, "x", ldx, true);
     keep_apart(mean, "mean", rstd, "rstd");
     Half half;
     const ScalarType yt = given ? given->scalar_type() : dtype(a[5], x.scalar_type());
@@ -235,8 +235,8 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
     vector(db_, "dbias", H);
     if (ws_ && !ws_->is_contiguous()) refuse(PyExc_ValueError, "workspace: a contiguous tensor is needed");
     if (dx_) {
-        keep_apart(*dx_, "dx", lddx, x, "x", ldx, true);
-        keep_apart(*dx_, "dx", lddx, dy, "dy", lddy, true);
+        keep_apart(*dx_, "dx", lddx, H, x, "x", ldx, true);
+        keep_apart(*dx_, "dx", lddx, H, dy, "dy", lddy, true);
     }
     keep_apart(dw_, "dweight", db_, "dbias");
     Half half;
@@ -269,7 +269,7 @@ PyObject* quantize_rows(PyObject* const* a) {
     if (out_) read_ld(*out_, "out", &x);
     const int64_t ldq = out_ ? rows16(*out_, "out") : kp;
     vector(scale_, "scale", R);
-    if (out_) keep_apart(*out_, "out", ldq, x, "x", ldx, false);
+    if (out_) keep_apart(*out_, "out", ldq, kp, x, "x", ldx, false);
     Half half;
     const int xc = half.code(x.scalar_type());
     Place here(x, {out_, scale_});
@@ -300,8 +300,8 @@ PyObject* gemm_i8(PyObject* const* a) {
         refuse(PyExc_ValueError, "out: a matrix of [", M, ", ", N, "] is needed, got ", out_->sizes());
     g.ldc = out_ ? write_ld(*out_, "out") : N;
     if (out_) {
-        keep_apart(*out_, "out", g.ldc, A, "A", lda, false);
-        keep_apart(*out_, "out", g.ldc, W, "W", ldw, false);
+        keep_apart(*out_, "out", g.ldc, N, A, "A", lda, false);
+        keep_apart(*out_, "out", g.ldc, N, W, "W", ldw, false);
     }
     Half half;
     const ScalarType ct = out_ ? out_->scalar_type() : dtype(a[6], ScalarType::Float);

@@ -270,3 +270,21 @@ def test_largest_products(lib):
         for c_dtype in (0, 1):
             a.c_dtype = c_dtype
             assert lib.stdiff_gemm_i8(C.byref(a), None) == SHAPE, (M, N, c_dtype)
+
+
+def test_quantize_rows_padding_is_kept_apart():
+    """the rows of q are written up to the next 16-byte border, so x may lie behind that, not behind K"""
+    from stdiff_amd import ops
+    buf = torch.zeros(4, 64)
+    q = buf.view(torch.int8)
+    assert q.data_ptr() % 16 == 0
+    for rows in (4, 1):
+        for first in (10, 11):                                # bytes 40 and 44 of the row, q's end at 48
+            with pytest.raises(ValueError, match="out and x share memory"):
+                ops.quantize_rows(buf[:rows, first:first + 40], out=q[:rows, :40])
+        with pytest.raises(ValueError, match="out and x share memory"):
+            ops.quantize_rows(buf.view(torch.bfloat16)[:rows, 3:8], out=q[:rows, :5])      # in the padding alone
+        with pytest.raises(RuntimeError, match="MI355X"):
+            ops.quantize_rows(buf[:rows, 12:52], out=q[:rows, :40])
+        with pytest.raises(RuntimeError, match="MI355X"):
+            ops.quantize_rows(buf[:rows, :40], out=q[:rows, 160:200])
