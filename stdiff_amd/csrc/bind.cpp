@@ -127,25 +127,46 @@ int64_t rows16(const Tensor& t, const char* name) {
     return ld;
 }
 
-// Outputs share no memory with what a call reads, but where an operator may work in place: then they are the same elements.
-// (Side by side in the rows of one buffer they are apart.)  columns: how many of a row of `out` are written, its padding included.
-void keep_apart(const Tensor& out, const char* name, int64_t ldo, int64_t columns, const Tensor& in, const char* other, int64_t ldi, bool in_place) {
-    if (!out.numel() || !in.numel()) return;
-    const int64_t rows = out.size(0), so = out.element_size(), si = in.element_size();
-    const uintptr_t p = (uintptr_t)out.data_ptr(), q = (uintptr_t)in.data_ptr();
-    const int64_t lp = ldo * so, lq = ldi * si, wp = columns * so, wq = in.size(1) * si;
-    if (p + (rows - 1) * lp + wp <= q || q + (in.size(0) - 1) * lq + wq <= p) return;
-    if (in_place && p == q && lp == lq && out.scalar_type() == in.scalar_type()) return;
-    if (lp == lq) {
-        const int64_t off = (int64_t)(q - p) % lp, d = off < 0 ? off + lp : off;
-        if (d >= wp && d + wq <= lp) return;
-    }
-    refuse(PyExc_ValueError, name, " and ", other, " share memory", in_place ? " and are not the same elements" : "");
+// Memory that a call reads or writes: rows of `width` bytes, `ld` bytes apart (a vector is one row).
+struct Area {
+    const char* name;
+    uintptr_t at;
+    int64_t rows, ld, width;               // no rows: nothing
+    ScalarType type;
+    bool empty() const { return rows <= 0 || width <= 0; }
+    uintptr_t end() const { return at + (rows - 1) * ld + width; }
+};
+// columns: how many of a row are touched, where that is not the tensor's own number (padding included)
+Area matrix(const Tensor* t, const char* name, int64_t ld, int64_t columns = -1) {
+    if (!t || !t->numel()) return {name, 0, 0, 0, 0, ScalarType::Undefined};
+    const int64_t size = t->element_size();
+    return {name, (uintptr_t)t->data_ptr(), ld ? t->size(0) : 1, ld * size, (columns < 0 ? t->size(1) : columns) * size, t->scalar_type()};
 }
-void keep_apart(const Tensor* a, const char* name, const Tensor* b, const char* other) {
-    if (!a || !b || !a->numel() || !b->numel()) return;
-    const uintptr_t p = (uintptr_t)a->data_ptr(), q = (uintptr_t)b->data_ptr();
-    if (p < q + b->nbytes() && q < p + a->nbytes()) refuse(PyExc_ValueError, name, " and ", other, " share memory");
+Area flat(const Tensor* t, const char* name) {
+    if (!t || !t->numel()) return {name, 0, 0, 0, 0, ScalarType::Undefined};
+    const int64_t bytes = (int64_t)t->nbytes();
+    return {name, (uintptr_t)t->data_ptr(), 1, bytes, bytes, t->scalar_type()};
+}
+// Side by side in the rows of one buffer, or in the gaps between rows, two areas are apart.
+bool meet(const Area& a, const Area& b) {
+    if (a.empty() || b.empty() || a.end() <= b.at || b.end() <= a.at) return false;
+    if (a.rows == 1 && b.rows > 1) return meet(b, a);
+    if (b.rows == 1) {                     // the first row of a that ends behind b's beginning: does it begin before b's end?
+        const int64_t behind = (int64_t)(b.at - a.at) - a.width, row = behind < 0 ? 0 : behind / a.ld + 1;
+        return row < a.rows && a.at + row * a.ld < b.end();
+    }
+    if (a.ld == b.ld) {
+        const int64_t off = (int64_t)(b.at - a.at) % a.ld, d = off < 0 ? off + a.ld : off;
+        if (d >= a.width && d + b.width <= a.ld) return false;
+    }
+    return true;
+}
+// Outputs share no memory with what a call reads, nor with each other, but where an operator may work in place: then they are
+// the same elements.
+void keep_apart(const Area& out, const Area& in, bool in_place = false) {
+    if (!meet(out, in)) return;
+    if (in_place && out.at == in.at && out.ld == in.ld && out.type == in.type) return;
+    refuse(PyExc_ValueError, out.name, " and ", in.name, " share memory", in_place ? " and are not the same elements" : "");
 }
 
 // The device that all tensors of a call are on is current while this lives; its current stream.
@@ -205,8 +226,13 @@ PyObject* layer_norm(PyObject* const* a) {
     if (w && b && w->scalar_type() != b->scalar_type())
         refuse(PyExc_TypeError, "weight is ", w->scalar_type(), ", bias ", b->scalar_type(), ": one dtype is needed");
     void *wp = vector(w, "weight", H, true), *bp = vector(b, "bias", H, true), *mp = vector(mean, "mean", R), *rp = vector(rstd, "rstd", R);
-    if (given) keep_apart(*given, "out", ldy, H, x, "x", ldx, true);
-    keep_apart(mean, "mean", rstd, "rstd");
+    const Area ax = matrix(&x, "x", ldx), ao = matrix(given, "out", ldy), am = flat(mean, "mean"), ar = flat(rstd, "rstd");
+    const Area aw = flat(w, "weight"), ab = flat(b, "bias");
+    keep_apart(ao, ax, true);
+    keep_apart(am, ar);
+    for (const Area* in : {&aw, &ab, &am, &ar}) keep_apart(ao, *in);
+    for (const Area* stat : {&am, &ar})
+        for (const Area* in : {&ax, &aw, &ab}) keep_apart(*stat, *in);
     Half half;
     const ScalarType yt = given ? given->scalar_type() : dtype(a[5], x.scalar_type());
     const int xc = half.code(x.scalar_type()), yc = half.code(yt), wc = w ? half.code(w->scalar_type()) : b ? half.code(b->scalar_type()) : STDIFF_F32;
@@ -234,11 +260,10 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
     vector(dw_, "dweight", H);
     vector(db_, "dbias", H);
     if (ws_ && !ws_->is_contiguous()) refuse(PyExc_ValueError, "workspace: a contiguous tensor is needed");
-    if (dx_) {
-        keep_apart(*dx_, "dx", lddx, H, x, "x", ldx, true);
-        keep_apart(*dx_, "dx", lddx, H, dy, "dy", lddy, true);
-    }
-    keep_apart(dw_, "dweight", db_, "dbias");
+    const Area ax = matrix(&x, "x", ldx), ady = matrix(&dy, "dy", lddy), adx = matrix(dx_, "dx", lddx), adw = flat(dw_, "dweight"), adb = flat(db_, "dbias");
+    keep_apart(adx, ax, true);
+    keep_apart(adx, ady, true);
+    keep_apart(adw, adb);
     Half half;
     const int xc = half.code(x.scalar_type()), dc = half.code(dy.scalar_type()), wc = w ? half.code(w->scalar_type()) : STDIFF_F32;
     Place here(x, {&dy, mean, rstd, w, dx_, dw_, db_, ws_});
@@ -269,7 +294,8 @@ PyObject* quantize_rows(PyObject* const* a) {
     if (out_) read_ld(*out_, "out", &x);
     const int64_t ldq = out_ ? rows16(*out_, "out") : kp;
     vector(scale_, "scale", R);
-    if (out_) keep_apart(*out_, "out", ldq, kp, x, "x", ldx, false);
+    const Area ax = matrix(&x, "x", ldx), aq = matrix(out_, "out", ldq, kp);
+    keep_apart(aq, ax);
     Half half;
     const int xc = half.code(x.scalar_type());
     Place here(x, {out_, scale_});
@@ -299,10 +325,9 @@ PyObject* gemm_i8(PyObject* const* a) {
     if (out_ && (out_->dim() != 2 || out_->size(0) != M || out_->size(1) != N))
         refuse(PyExc_ValueError, "out: a matrix of [", M, ", ", N, "] is needed, got ", out_->sizes());
     g.ldc = out_ ? write_ld(*out_, "out") : N;
-    if (out_) {
-        keep_apart(*out_, "out", g.ldc, N, A, "A", lda, false);
-        keep_apart(*out_, "out", g.ldc, N, W, "W", ldw, false);
-    }
+    const Area ao = matrix(out_, "out", g.ldc);
+    keep_apart(ao, matrix(&A, "A", lda));
+    keep_apart(ao, matrix(&W, "W", ldw));
     Half half;
     const ScalarType ct = out_ ? out_->scalar_type() : dtype(a[6], ScalarType::Float);
     g.c_dtype = half.code(ct);

@@ -410,7 +410,7 @@ _bind.setup(_entries, L.StdiffError)
 def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, mean=None, rstd=None):
     """LayerNorm of the rows of x [R, H] with a weight and a bias per column (None: 1 and 0; one dtype for both).
     x and out: fp32 or a 16-bit type, any row stride, any H.  mean / rstd (fp32 [R], optional): receive the statistics
-    that layer_norm_bwd takes.  out may be x; else it shares no memory with it."""
+    that layer_norm_bwd takes.  out may be x; else outputs share no memory with inputs or each other."""
     return _bind.layer_norm(x, weight, bias, eps, out, out_dtype, mean, rstd)
 
 

@@ -288,3 +288,39 @@ def test_quantize_rows_padding_is_kept_apart():
             ops.quantize_rows(buf[:rows, 12:52], out=q[:rows, :40])
         with pytest.raises(RuntimeError, match="MI355X"):
             ops.quantize_rows(buf[:rows, :40], out=q[:rows, 160:200])
+
+
+def apart(call):
+    """as far as a machine without a GPU can tell, the call's tensors may lie where they do"""
+    with pytest.raises(RuntimeError, match="MI355X"):
+        call()
+
+
+def shared(names, call):
+    with pytest.raises(ValueError, match=f"{names} share memory"):
+        call()
+
+
+def test_layer_norm_outputs_are_kept_apart():
+    """out, mean and rstd against everything that is read, and against each other; in the gaps between rows they may lie"""
+    from stdiff_amd import ops
+    buf = torch.zeros(8, 64)
+    x, w, b, flat = buf[:4, :32], torch.ones(32), torch.zeros(32), buf.view(-1)
+    shared("out and weight", lambda: ops.layer_norm(x, buf[5, :32], out=buf[4:, :32]))
+    shared("out and bias", lambda: ops.layer_norm(x, w, buf[7, 31:63], out=buf[4:, :32]))
+    shared("out and weight", lambda: ops.layer_norm(x, x[2], out=x))
+    shared("out and mean", lambda: ops.layer_norm(x, mean=buf[6, 29:33], out=buf[4:, :32]))
+    shared("out and rstd", lambda: ops.layer_norm(x, rstd=flat[4 * 64 - 3:4 * 64 + 1], out=buf[4:, :32]))
+    shared("mean and x", lambda: ops.layer_norm(x, mean=buf[3, 28:32]))
+    shared("rstd and x", lambda: ops.layer_norm(x, rstd=buf[0, :4]))
+    shared("mean and weight", lambda: ops.layer_norm(x, w, mean=w[:4]))
+    shared("rstd and weight", lambda: ops.layer_norm(x, w, rstd=w[28:]))
+    shared("mean and bias", lambda: ops.layer_norm(x, w, b, mean=b[5:9]))
+    shared("rstd and bias", lambda: ops.layer_norm(x, w, b, rstd=b[:4]))
+    shared("mean and rstd", lambda: ops.layer_norm(x, mean=w[:4], rstd=w[3:7]))
+    for at in (buf[0, 32:], buf[3, 32:], buf[2, 32:], flat[4 * 64:4 * 64 + 32]):
+        apart(lambda: ops.layer_norm(x, at[:32], at[:32], mean=flat[6 * 64:6 * 64 + 4], rstd=flat[7 * 64:7 * 64 + 4], out=x))
+    apart(lambda: ops.layer_norm(x, w, w, mean=buf[1, 32:36], rstd=buf[1, 36:40], out=buf[4:, 32:]))
+    # a row of its own as weight: of another row nothing is written
+    apart(lambda: ops.layer_norm(buf[:1, :32], buf[1, :32], buf[2, :32], out=buf[:1, :32]))
+    apart(lambda: ops.layer_norm(torch.zeros(0, 32), w, w, out=torch.zeros(0, 32), mean=w[:0], rstd=w[:0]))
