@@ -261,9 +261,14 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
     vector(db_, "dbias", H);
     if (ws_ && !ws_->is_contiguous()) refuse(PyExc_ValueError, "workspace: a contiguous tensor is needed");
     const Area ax = matrix(&x, "x", ldx), ady = matrix(&dy, "dy", lddy), adx = matrix(dx_, "dx", lddx), adw = flat(dw_, "dweight"), adb = flat(db_, "dbias");
+    const Area aw = flat(w, "weight"), am = flat(mean, "mean"), ar = flat(rstd, "rstd"), aws = flat(ws_, "workspace");
     keep_apart(adx, ax, true);
     keep_apart(adx, ady, true);
     keep_apart(adw, adb);
+    for (const Area* o : {&aw, &am, &ar, &adw, &adb}) keep_apart(adx, *o);
+    for (const Area* o : {&adw, &adb})
+        for (const Area* in : {&ax, &ady, &aw, &am, &ar}) keep_apart(*o, *in);
+    for (const Area* o : {&ax, &ady, &adx, &aw, &am, &ar, &adw, &adb}) keep_apart(aws, *o);
     Half half;
     const int xc = half.code(x.scalar_type()), dc = half.code(dy.scalar_type()), wc = w ? half.code(w->scalar_type()) : STDIFF_F32;
     Place here(x, {&dy, mean, rstd, w, dx_, dw_, db_, ws_});

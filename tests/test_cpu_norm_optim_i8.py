@@ -324,3 +324,37 @@ def test_layer_norm_outputs_are_kept_apart():
     # a row of its own as weight: of another row nothing is written
     apart(lambda: ops.layer_norm(buf[:1, :32], buf[1, :32], buf[2, :32], out=buf[:1, :32]))
     apart(lambda: ops.layer_norm(torch.zeros(0, 32), w, w, out=torch.zeros(0, 32), mean=w[:0], rstd=w[:0]))
+
+
+def test_layer_norm_bwd_outputs_are_kept_apart():
+    """dx, dweight, dbias and a given workspace against everything that is read, and against each other"""
+    from stdiff_amd import ops
+    buf = torch.zeros(12, 64)
+    x, dy, flat = buf[:4, :32], buf[4:8, :32], buf.view(-1)
+    w, s1, s2, g1, g2 = torch.ones(32), torch.zeros(4), torch.zeros(4), torch.zeros(32), torch.zeros(32)
+    ws = torch.zeros(4096)
+
+    def bwd(dy=dy, x=x, mean=s1, rstd=s2, w=w, **kw):
+        return lambda: ops.layer_norm_bwd(dy, x, mean, rstd, w, **kw)
+    assert ops.layer_norm_bwd_workspace(4, 32, torch.float32) == 0
+    shared("dweight and weight", bwd(dweight=w))
+    shared("dbias and weight", bwd(dbias=w))
+    shared("dweight and x", bwd(dweight=buf[3, :32]))
+    shared("dbias and dy", bwd(dbias=buf[4, 20:52]))
+    shared("dweight and mean", bwd(mean=g1[3:7], dweight=g1))
+    shared("dbias and rstd", bwd(rstd=g2[28:], dbias=g2))
+    shared("dx and weight", bwd(w=buf[8, :32], dx=buf[8:, :32]))
+    shared("dx and mean", bwd(mean=buf[11, 28:32], dx=buf[8:, :32]))
+    shared("dx and rstd", bwd(rstd=buf[9, 31:35], dx=buf[8:, :32]))
+    shared("dx and dweight", bwd(dweight=buf[10, 16:48], dx=buf[8:, :32]))
+    shared("dx and dbias", bwd(dbias=x[0], dx=x))
+    shared("dweight and dbias", bwd(dweight=ws[:32], dbias=ws[31:63]))
+    for name, kw in (("x", {}), ("dy", {}), ("dx", dict(dx=buf[8:, :32])), ("weight", {}), ("mean", {}), ("rstd", {}), ("dweight", dict(dweight=g1)),
+                     ("dbias", dict(dbias=g2))):
+        over = {"x": flat[200:260], "dy": flat[4 * 64 + 31:4 * 64 + 33], "dx": flat[8 * 64:8 * 64 + 4], "weight": w, "mean": s1, "rstd": s2[1:],
+                "dweight": g1[:16], "dbias": g2[16:]}[name]
+        shared(f"workspace and {name}", bwd(workspace=over, **kw))
+    for dx in (x, dy, buf[8:, :32], buf[:4, 32:]):
+        apart(bwd(dx=dx, dweight=g1, dbias=g2, workspace=ws))
+    apart(bwd(w=buf[1, 32:], mean=buf[2, 32:36], rstd=buf[2, 36:40], dweight=buf[3, 32:], dbias=buf[5, 32:], dx=x, workspace=flat[8 * 64:]))
+    apart(bwd(dy=dy[:1].expand(4, 32), dweight=dy[1], dbias=dy[2], dx=x))
