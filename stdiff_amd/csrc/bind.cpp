@@ -299,8 +299,10 @@ PyObject* quantize_rows(PyObject* const* a) {
     if (out_) read_ld(*out_, "out", &x);
     const int64_t ldq = out_ ? rows16(*out_, "out") : kp;
     vector(scale_, "scale", R);
-    const Area ax = matrix(&x, "x", ldx), aq = matrix(out_, "out", ldq, kp);
+    const Area ax = matrix(&x, "x", ldx), aq = matrix(out_, "out", ldq, kp), as = flat(scale_, "scale");
     keep_apart(aq, ax);
+    keep_apart(aq, as);
+    keep_apart(as, ax);
     Half half;
     const int xc = half.code(x.scalar_type());
     Place here(x, {out_, scale_});

@@ -490,7 +490,8 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
 def quantize_rows(x, out=None, scale=None):
     """(q, scale): the rows of x [R, K] (fp32 or a 16-bit type) as int8 with one fp32 scale each, scale = max |x| / 127 and
     q = rint(x * (127 / max |x|)).  q is a [R, K] view of rows that begin on 16-byte borders, zeros behind K, as gemm_i8
-    takes them (a given `out` has to be such a view, and its rows are written up to the next border).  A row that holds an
+    takes them (a given `out` has to be such a view, and its rows are written up to the next border; x, out and scale share no
+    memory).  A row that holds an
     infinity or a NaN gets a scale that is not finite."""
     return _bind.quantize_rows(x, out, scale)
 

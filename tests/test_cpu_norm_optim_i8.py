@@ -358,3 +358,18 @@ def test_layer_norm_bwd_outputs_are_kept_apart():
         apart(bwd(dx=dx, dweight=g1, dbias=g2, workspace=ws))
     apart(bwd(w=buf[1, 32:], mean=buf[2, 32:36], rstd=buf[2, 36:40], dweight=buf[3, 32:], dbias=buf[5, 32:], dx=x, workspace=flat[8 * 64:]))
     apart(bwd(dy=dy[:1].expand(4, 32), dweight=dy[1], dbias=dy[2], dx=x))
+
+
+def test_quantize_rows_scale_is_kept_apart():
+    """scale against x and out, the padding of out's rows included"""
+    from stdiff_amd import ops
+    buf = torch.zeros(8, 64)
+    x, q = buf[:4, :32], buf.view(torch.int8)[4:, :40]
+    assert q.data_ptr() % 16 == 0
+    shared("scale and x", lambda: ops.quantize_rows(x, scale=buf[3, 28:32]))
+    shared("scale and x", lambda: ops.quantize_rows(x[:1].expand(4, 32), scale=buf[0, :4]))
+    shared("out and scale", lambda: ops.quantize_rows(buf[:4, :40], out=q, scale=buf[5, 9:13]))
+    shared("out and scale", lambda: ops.quantize_rows(buf[:4, :40], out=q, scale=buf[5, 11:15]))      # in the padding: bytes 44 to 47
+    shared("out and scale", lambda: ops.quantize_rows(buf[:4, :40], out=q, scale=buf.view(-1)[4 * 64 - 1:4 * 64 + 3]))
+    for scale in (buf[5, 12:16], buf[0, 40:44], torch.zeros(4)):
+        apart(lambda: ops.quantize_rows(buf[:4, :40], out=q, scale=scale))
