@@ -335,6 +335,9 @@ PyObject* gemm_i8(PyObject* const* a) {
     const Area ao = matrix(out_, "out", g.ldc);
     keep_apart(ao, matrix(&A, "A", lda));
     keep_apart(ao, matrix(&W, "W", ldw));
+    keep_apart(ao, flat(sa, "a_scale"));
+    keep_apart(ao, flat(sw, "w_scale"));
+    keep_apart(ao, flat(bias, "bias"));
     Half half;
     const ScalarType ct = out_ ? out_->scalar_type() : dtype(a[6], ScalarType::Float);
     g.c_dtype = half.code(ct);

@@ -498,7 +498,8 @@ def quantize_rows(x, out=None, scale=None):
 
 def gemm_i8(A, a_scale, W, w_scale, bias=None, out=None, out_dtype=torch.float32):
     """out[M, N] = (A[M, K] @ W[N, K]^T) * w_scale[N] * a_scale[M, None] + bias: int8 operands as quantize_rows makes them,
-    the sum over K exact in int32 (K <= 131071; M and N <= 2^30), scales and bias fp32, out fp32 or a 16-bit type."""
+    the sum over K exact in int32 (K <= 131071; M and N <= 2^30), scales and bias fp32, out fp32 or a
+    16-bit type.  out shares no memory with the other operands."""
     return _bind.gemm_i8(A, a_scale, W, w_scale, bias, out, out_dtype)
 
 

@@ -373,3 +373,18 @@ def test_quantize_rows_scale_is_kept_apart():
     shared("out and scale", lambda: ops.quantize_rows(buf[:4, :40], out=q, scale=buf.view(-1)[4 * 64 - 1:4 * 64 + 3]))
     for scale in (buf[5, 12:16], buf[0, 40:44], torch.zeros(4)):
         apart(lambda: ops.quantize_rows(buf[:4, :40], out=q, scale=scale))
+
+
+def test_gemm_i8_output_is_kept_apart():
+    """out against the scales and the bias; in the gaps between its rows they may lie"""
+    from stdiff_amd import ops
+    A, W = torch.zeros(4, 32, dtype=torch.int8), torch.zeros(6, 32, dtype=torch.int8)
+    sa, sw, b, buf = torch.ones(4), torch.ones(6), torch.zeros(6), torch.zeros(4, 16)
+    out = buf[:, :6]
+    shared("out and bias", lambda: ops.gemm_i8(A, sa, W, sw, buf[2, :6], out=out))
+    shared("out and bias", lambda: ops.gemm_i8(A, sa, W, sw, buf[2, 5:11], out=out))
+    shared("out and a_scale", lambda: ops.gemm_i8(A, buf[0, 4:8], W, sw, b, out=out))
+    shared("out and w_scale", lambda: ops.gemm_i8(A, sa, W, buf.view(-1)[11:17], b, out=out))
+    shared("out and w_scale", lambda: ops.gemm_i8(A, sa, W, buf[3, :6], b, out=buf.view(torch.bfloat16)[:, 10:16]))
+    apart(lambda: ops.gemm_i8(A, buf[0, 6:10], W, buf[1, 6:12], buf[2, 10:16], out=out))
+    apart(lambda: ops.gemm_i8(A, sa, W, sw, sw, out=out))
