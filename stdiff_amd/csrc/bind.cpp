@@ -356,8 +356,23 @@ struct Table {
     std::vector<int64_t> sizes;
     std::vector<c10::Storage> memory;      // alive even where a tensor is given other memory
     std::vector<std::pair<Tensor, void*>> states;
+    std::vector<std::pair<uintptr_t, uintptr_t>> taken;    // beginning and end of all of it, in order
     Half half;
     int bits = 32, device = -1;
+};
+// Whether memory lies apart from a table's.  What was asked about last lies in some gap between the parameters and states; the next
+// gradient is often in the same one, and no search is needed.
+struct Apart {
+    const Table& t;
+    uintptr_t from = 1, to = 0;
+    bool operator()(const Area& a) {
+        if (a.empty() || (a.at >= from && a.end() <= to)) return true;
+        const auto next = std::upper_bound(t.taken.begin(), t.taken.end(), a.at, [](uintptr_t v, const auto& r) { return v < r.first; });
+        const uintptr_t below = next == t.taken.begin() ? 0 : (next - 1)->second, above = next == t.taken.end() ? UINTPTR_MAX : next->first;
+        if (a.at < below || a.end() > above) return false;
+        from = below, to = above;
+        return true;
+    }
 };
 constexpr const char* TABLE = "stdiff_amd.adamw_table";
 
@@ -380,7 +395,6 @@ PyObject* adamw_table(PyObject* const* a) {
     for (const Items* k : {&m, &v, &ms, &vs, &decay})
         if (k->n != p.n) refuse(PyExc_ValueError, "adamw_multi_args: lists of different lengths");
     std::unique_ptr<Table> t(new Table);
-    std::vector<std::pair<uintptr_t, size_t>> ranges;
     const Tensor *first = nullptr, *away = nullptr;
     for (Py_ssize_t i = 0; i < p.n; ++i) {
         const Tensor* k[5];
@@ -416,7 +430,7 @@ PyObject* adamw_table(PyObject* const* a) {
             if (k[j]) {
                 t->memory.push_back(k[j]->storage());
                 if (j) t->states.push_back({*k[j], k[j]->data_ptr()});
-                if (k[j]->numel()) ranges.push_back({(uintptr_t)k[j]->data_ptr(), k[j]->nbytes()});
+                if (k[j]->numel()) t->taken.push_back({(uintptr_t)k[j]->data_ptr(), (uintptr_t)k[j]->data_ptr() + k[j]->nbytes()});
             }
     }
     if (first) {
@@ -424,9 +438,9 @@ PyObject* adamw_table(PyObject* const* a) {
         if (away || !first->is_cuda()) Place::not_here();
         t->device = first->get_device();
     }
-    std::sort(ranges.begin(), ranges.end());
-    for (size_t i = 1; i < ranges.size(); ++i)
-        if (ranges[i - 1].first + ranges[i - 1].second > ranges[i].first)
+    std::sort(t->taken.begin(), t->taken.end());
+    for (size_t i = 1; i < t->taken.size(); ++i)
+        if (t->taken[i - 1].second > t->taken[i].first)
             refuse(PyExc_ValueError, "adamw_multi_args: two of the parameters and states share memory");
     PyObject* c = PyCapsule_New(t.get(), TABLE, [](PyObject* o) { delete (Table*)PyCapsule_GetPointer(o, TABLE); });
     if (!c) throw Refusal{nullptr, ""};
@@ -450,6 +464,12 @@ PyObject* adamw_multi(PyObject* const* a) {
     if (ws_ && !ws_->is_contiguous()) refuse(PyExc_ValueError, "workspace: a contiguous tensor is needed");
     for (const auto& s : t->states)
         if (s.first.data_ptr() != s.second) refuse(PyExc_ValueError, "adamw_multi: a state was given other memory since adamw_multi_args");
+    const Area cells[] = {flat(ws_, "workspace"), flat(norm, "norm"), flat(&step, "step_dev")};
+    Apart apart{*t};
+    for (int i = 0; i < 3; ++i) {
+        if (!apart(cells[i])) refuse(PyExc_ValueError, "adamw_multi: ", cells[i].name, " shares memory with a parameter or state");
+        for (int j = i + 1; j < 3; ++j) keep_apart(cells[i], cells[j]);
+    }
     Half half = t->half;
     std::vector<stdiff_adamw_tensor> rows = t->rows;       // of this call: two calls do not see each other's gradients
     for (Py_ssize_t i = 0; i < n; ++i) {
@@ -463,6 +483,10 @@ PyObject* adamw_multi(PyObject* const* a) {
         if (d->numel() != t->sizes[i] || !d->is_contiguous())
             refuse(PyExc_ValueError, "adamw_multi: gradient ", i, ": ", t->sizes[i], " contiguous elements are needed, got ", d->sizes(), " with strides ", d->strides());
         if (!d->is_cuda() || d->get_device() != t->device) refuse(PyExc_ValueError, "adamw_multi: gradient ", i, " is on ", d->device(), ", its parameter on device ", t->device);
+        const Area grad = flat(d, "gradient");
+        if (!apart(grad)) refuse(PyExc_ValueError, "adamw_multi: gradient ", i, " shares memory with a parameter or state");
+        for (const Area& c : cells)
+            if (meet(c, grad)) refuse(PyExc_ValueError, "adamw_multi: ", c.name, " and gradient ", i, " share memory");
         rows[i].grad = d->data_ptr();
         rows[i].grad_dtype = half.code(d->scalar_type());
     }

@@ -481,6 +481,8 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     16-bit type, or None (that parameter and its state stay as they are).  step_dev: int32 [1] on the device, the steps
     done so far; incremented.  max_norm: clip by the norm over all gradients (None: no clipping); norm (fp32 [1],
     optional) receives that norm; grad_scale multiplies every gradient first (1 / world size, 1 / loss scale).
+    Gradients, step_dev, norm and workspace share no memory with the parameters and states, the latter three none with the
+    gradients or each other.
     workspace (fp32, at least adamw_multi_workspace(len(grads)) floats; allocated unless given): give one of its own to a
     call that is captured into an ops.Graph.  A captured step keeps lr and the other numbers it was captured with, and its
     replays do not raise the parameters' version counters: torch.autograd.graph.increment_version does."""

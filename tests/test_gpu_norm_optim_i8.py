@@ -1040,3 +1040,59 @@ def test_quantize_rows_groups_of_lanes(ops, R, K, xt):
     assert torch.equal(s, (top / torch.full_like(top, 127.0)).view(-1)) and torch.equal(q.float(), want)
     kp = -(-K // 16) * 16
     assert not bool(torch.as_strided(q, (R, kp), (kp, 1))[:, K:].any())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_multi_keeps_apart(ops, bits):
+    """gradients, step_dev, norm and a given workspace share no memory with parameters and states, norm, step_dev and workspace none
+    with the gradients or each other; nothing is changed by a call that is refused"""
+    buf = rnd(8192, seed=470).to(DEV)
+    p = [buf[:300], buf[1024:2024], buf[600:900]]
+    free = [buf[300:600], buf[2024:3024], buf[4096:4396]]
+    if bits == 8:
+        st = [ops.adamw8_state(t) for t in p]
+        scales = [[s[k] for s in st] for k in (2, 3)]
+    else:
+        st = [(buf[5000:5300], buf[5300:5600]), (torch.zeros_like(p[1]), torch.zeros_like(p[1])), (torch.zeros_like(p[2]), torch.zeros_like(p[2]))]
+        buf[5300:5600].zero_()
+        scales = [None, None]
+    args = ops.adamw_multi_args(p, [s[0] for s in st], [s[1] for s in st], *scales)
+    step, norm = torch.zeros(1, device=DEV, dtype=torch.int32), torch.zeros(1, device=DEV)
+    ws = torch.empty(ops.adamw_multi_workspace(3), device=DEV)
+    before, states = buf.clone(), [[t.clone() for t in s] for s in st]
+
+    def refused(match, grads=free, step=step, **kw):
+        with pytest.raises(ValueError, match=match):
+            ops.adamw_multi(args, grads, step, 1e-3, **kw)
+    last = buf.view(torch.bfloat16)[2 * 899 + 1:][:300]          # begins in the last two bytes of a parameter
+    for i, bad in ((0, buf[299:599]), (0, buf[301:601]), (0, p[0]), (1, buf[100:1100]), (1, buf[1500:2500]), (2, buf[700:1000]), (2, last)):
+        refused(f"gradient {i} shares memory", [bad if k == i else t for k, t in enumerate(free)])
+    if bits == 8:
+        for k in range(2):                                       # codes and scales
+            refused("gradient 2 shares memory", free[:2] + [st[1][k].view(torch.uint8).view(torch.bfloat16)[100:400]])
+            refused("norm shares memory", norm=st[1][2 + k][1:2])
+    else:
+        refused("gradient 0 shares memory", [buf[5299:5599], free[1], free[2]])
+        refused("norm shares memory", norm=buf[5599:5600])
+    as_int = buf.view(torch.int32)
+    refused("step_dev shares memory", step=as_int[1024:1025])
+    refused("norm shares memory", norm=buf[899:900])
+    refused("workspace shares memory", workspace=buf[:8192])
+    refused("norm and gradient 1 share memory", norm=buf[3023:3024])
+    refused("step_dev and gradient 0 share memory", step=as_int[300:301])
+    refused("workspace and gradient 2 share memory", workspace=buf[4395:4999])
+    refused("workspace and norm share memory", workspace=ws, norm=ws[-1:])
+    refused("workspace and step_dev share memory", workspace=ws, step=ws.view(torch.int32)[:1])
+    refused("norm and step_dev share memory", norm=norm, step=norm.view(torch.int32))
+    for kw in (dict(max_norm=0.0), dict(max_norm=float("nan")), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(workspace=torch.zeros(3, device=DEV))):
+        refused(".", **kw)
+    assert torch.equal(buf, before) and int(step) == 0
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for s, t in zip(st, states) for a, b in zip(s, t))
+    # beside each other they may lie, as long as they are apart: the step of tensors of their own
+    own = [t.clone() for t in p]
+    so = [ops.adamw8_state(t) if bits == 8 else (torch.zeros_like(t), torch.zeros_like(t)) for t in own]
+    if bits == 32:
+        st[0][0].zero_()
+    ops.adamw_multi(ops.adamw_multi_args(own, *[[s[k] for s in so] for k in range(len(so[0]))]), [t.clone() for t in free], step.clone(), 1e-3, max_norm=1.0)
+    ops.adamw_multi(args, free, as_int[900:901].zero_(), 1e-3, max_norm=1.0, norm=buf[901:902], workspace=buf[6000:])
+    assert all(torch.equal(a, b) for a, b in zip(p, own)) and int(as_int[900]) == 1 and float(buf[901]) > 0
