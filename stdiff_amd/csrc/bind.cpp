@@ -498,8 +498,14 @@ PyObject* adamw_multi(PyObject* const* a) {
     g.step_dev = (int32_t*)step.data_ptr(), g.workspace = (float*)ws.data_ptr(), g.workspace_bytes = (long long)ws.nbytes();
     check(l, l.adamw_multi(&g, here.stream));
     // who keeps copies of the parameters (DiT_stDiff's packed operands) sees by their version counters that they changed
+    const size_t per = t->bits == 8 ? 4 : 2;               // states of a tensor
     for (Py_ssize_t i = 0; i < n; ++i)
-        if (rows[i].n) written(&THPVariable_Unpack(params[i]));
+        if (rows[i].n) {
+            written(&THPVariable_Unpack(params[i]));
+            for (size_t j = 0; j < per; ++j) written(&t->states[i * per + j].first);
+        }
+    written(&step);
+    written(norm);
     return Py_NewRef(Py_None);
 }
 

@@ -485,7 +485,7 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
     gradients or each other.
     workspace (fp32, at least adamw_multi_workspace(len(grads)) floats; allocated unless given): give one of its own to a
     call that is captured into an ops.Graph.  A captured step keeps lr and the other numbers it was captured with, and its
-    replays do not raise the parameters' version counters: torch.autograd.graph.increment_version does."""
+    replays do not raise the version counters of what they write: torch.autograd.graph.increment_version does."""
     _bind.adamw_multi(args.table, args.params, grads, step_dev, lr, max_norm, grad_scale, betas[0], betas[1], eps, norm, workspace)
 
 

@@ -1096,3 +1096,31 @@ def test_adamw_multi_keeps_apart(ops, bits):
     ops.adamw_multi(ops.adamw_multi_args(own, *[[s[k] for s in so] for k in range(len(so[0]))]), [t.clone() for t in free], step.clone(), 1e-3, max_norm=1.0)
     ops.adamw_multi(args, free, as_int[900:901].zero_(), 1e-3, max_norm=1.0, norm=buf[901:902], workspace=buf[6000:])
     assert all(torch.equal(a, b) for a, b in zip(p, own)) and int(as_int[900]) == 1 and float(buf[901]) > 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_multi_raises_version_counters(ops, bits):
+    """everything that a step writes counts as changed for autograd, what it leaves alone does not"""
+    p = [torch.ones(300, device=DEV), torch.ones(40, device=DEV), torch.ones(0, device=DEV)]
+    st = [ops.adamw8_state(t) if bits == 8 else (torch.zeros_like(t), torch.zeros_like(t)) for t in p]
+    args = ops.adamw_multi_args(p, *[[s[k] for s in st] for k in range(len(st[0]))])
+    step, norm = torch.zeros(1, device=DEV, dtype=torch.int32), torch.zeros(1, device=DEV)
+    x = torch.ones(300, device=DEV, requires_grad=True)
+    saved = x * st[0][-1][:1].float()                             # saves a state
+    written, left = [p[0], *st[0], step, norm], [p[1], *st[1], p[2], *st[2]]
+    before = [[t._version for t in ts] for ts in (written, left)]
+    ops.adamw_multi(args, [torch.ones(300, device=DEV), None, torch.ones(0, device=DEV)], step, 1e-3, norm=norm)
+    assert all(t._version > v for t, v in zip(written, before[0]))
+    assert all(t._version == v for t, v in zip(left, before[1]))
+    if bits == 8:
+        assert st[0][3]._version > before[0][4]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.sum().backward()
+    ops.adamw_multi(args, [None] * 3, step, 1e-3)                 # the step count alone
+    assert step._version > before[0][-2] + 1
+    with torch.inference_mode():                                  # tensors without counters
+        q = torch.ones(8, device=DEV)
+        s = [ops.adamw8_state(q)] if bits == 8 else [(torch.zeros_like(q), torch.zeros_like(q))]
+        ops.adamw_multi(ops.adamw_multi_args([q], *[[t[k] for t in s] for k in range(len(s[0]))]), [torch.ones(8, device=DEV)],
+                        torch.zeros(1, device=DEV, dtype=torch.int32), 1e-3)
+        assert bool((q < 1).all())
