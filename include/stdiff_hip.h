@@ -538,7 +538,8 @@ typedef struct {
 long long stdiff_adamw_multi_workspace(int n_tensors);
 int stdiff_adamw_multi(const stdiff_adamw_multi_args* a, void* stream);
 
-/* Rows in 8 bits:  scale[r] = max |x[r]| / 127, q[r][k] = rint(x[r][k] * (127 / max |x[r]|));  a zero row: zeros and scale 0.
+/* Rows in 8 bits:  scale[r] = max |x[r]| / 127, q[r][k] = rint(x[r][k] * (127 / max |x[r]|));  a zero row: zeros and scale 0;
+ * a row whose largest is below 4e-37 is scaled as if it were 4e-37 (127 over less is no fp32 number).
  * q: int8 [R][ldq], 16-byte aligned, ldq % 16 == 0, ldq >= round_up(K, 16); columns K .. round_up(K, 16) - 1 become
  * zeros.  A row that holds an infinity or a NaN gets a scale that is not finite. */
 int stdiff_quantize_rows(const void* x, long long ldx, int x_dtype, void* q, long long ldq, float* scale, int R, int K, void* stream);

@@ -46,8 +46,8 @@ template <bool NT = false> __device__ __forceinline__ void ld8(const bf16_t* p, 
 // finite the whole row of the product is NaN.  Columns K .. round_up(K, 16) - 1 of q become zeros.
 __device__ __forceinline__ float row_factor(unsigned top_bits, float* scale) {
     const float t = __builtin_bit_cast(float, top_bits);
-    // below 1e-30 the factor 127 / t would leave the range of fp32: such rows are scaled as if their largest were 1e-30
-    const float m = t > 0.f && t < 1e-30f ? 1e-30f : t;
+    // below 3.8e-37 the factor 127 / t would leave the range of fp32: such rows are scaled as if their largest were 4e-37
+    const float m = t > 0.f && t < 4e-37f ? 4e-37f : t;
     *scale = m / 127.0f;
     return m == 0.f ? 0.f : 127.0f / m;
 }

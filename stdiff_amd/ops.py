@@ -491,17 +491,17 @@ def adamw_multi(args, grads, step_dev, lr, max_norm=None, grad_scale=1.0, betas=
 
 def quantize_rows(x, out=None, scale=None):
     """(q, scale): the rows of x [R, K] (fp32 or a 16-bit type) as int8 with one fp32 scale each, scale = max |x| / 127 and
-    q = rint(x * (127 / max |x|)).  q is a [R, K] view of rows that begin on 16-byte borders, zeros behind K, as gemm_i8
-    takes them (a given `out` has to be such a view, and its rows are written up to the next border; x, out and scale share no
-    memory).  A row that holds an
-    infinity or a NaN gets a scale that is not finite."""
+    q = rint(x * (127 / max |x|)); a largest magnitude below 4e-37 counts as 4e-37, that of a zero row as 0.  q is a [R, K]
+    view of rows that begin on 16-byte borders, zeros behind K, as gemm_i8 takes them (a given `out` has to be such a view, and
+    its rows are written up to the next border; x, out and scale share no memory).  A row that holds an infinity or a NaN gets a
+    scale that is not finite."""
     return _bind.quantize_rows(x, out, scale)
 
 
 def gemm_i8(A, a_scale, W, w_scale, bias=None, out=None, out_dtype=torch.float32):
     """out[M, N] = (A[M, K] @ W[N, K]^T) * w_scale[N] * a_scale[M, None] + bias: int8 operands as quantize_rows makes them,
-    the sum over K exact in int32 (K <= 131071; M and N <= 2^30), scales and bias fp32, out fp32 or a
-    16-bit type.  out shares no memory with the other operands."""
+    the sum over K exact in int32 (K <= 131071; M and N <= 2^30), scales and bias fp32, out fp32 or a 16-bit type.  out shares
+    no memory with the other operands."""
     return _bind.gemm_i8(A, a_scale, W, w_scale, bias, out, out_dtype)
 
 

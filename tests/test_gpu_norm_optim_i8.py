@@ -1124,3 +1124,21 @@ def test_adamw_multi_raises_version_counters(ops, bits):
         ops.adamw_multi(ops.adamw_multi_args([q], *[[t[k] for t in s] for k in range(len(s[0]))]), [torch.ones(8, device=DEV)],
                         torch.zeros(1, device=DEV, dtype=torch.int32), 1e-3)
         assert bool((q < 1).all())
+
+
+@pytest.mark.parametrize("xt", ["fp32", "bf16"])
+@pytest.mark.parametrize("K", [40, 300, 1000, 3000, 9000])
+def test_quantize_rows_of_tiny_values(ops, xt, K):
+    """rows whose largest magnitude is far below one: the formula down to 4e-37, below it the scale of 4e-37"""
+    tops = torch.tensor([2e-30, 9e-31, 1e-33, 3e-35, 5e-37, 4.1e-37, 3e-37, 2e-38, 1e-39, 5e-42])
+    x = rnd(len(tops), K, seed=480).clamp(-1, 1)
+    x[:, 3] = -1
+    x = (x * tops.view(-1, 1)).to(DT[xt])
+    q, s = ops.quantize_rows(x.to(DEV))
+    f = x.float()
+    top = f.abs().amax(1, keepdim=True)
+    top = torch.where(top > 0, top.clamp_min(4e-37), top)        # bf16 holds the last row as zeros
+    assert torch.equal(s.cpu(), (top / torch.full_like(top, 127.0)).view(-1))
+    assert torch.equal(q.cpu().float(), torch.round(f * torch.where(top > 0, torch.full_like(top, 127.0) / top, torch.zeros_like(top))))
+    # half a step of the scale, the roundings of the product, and half of fp32's smallest step in the scale, 127 times
+    within(q.cpu().double() * s.cpu().double().view(-1, 1), f, s.cpu().double().view(-1, 1) * (0.5 + 200 * U) + 2 * U * f.double().abs() + 127 * 2.0 ** -150, "value")
