@@ -432,7 +432,7 @@ def layer_norm_bwd_workspace(R, H, x_dtype, dy_dtype=None):
         if t not in (torch.float32, torch.bfloat16, torch.float16):
             raise TypeError(f"unsupported dtype {t}")
         codes.append(F32 if t == torch.float32 else L.BF16)
-    n = lib().stdiff_layer_norm_bwd_workspace(R, H, *codes)
+    n = lib().stdiff_layer_norm_bwd_workspace(R, H, *codes) if 0 <= R < 2**31 and 0 <= H < 2**31 else -1   # ctypes would cut them to 32 bits
     if n < 0:
         raise ValueError(f"layer_norm_bwd_workspace: bad size {R} x {H}")
     return n // 4
@@ -470,7 +470,7 @@ def adamw8_state(param):
 
 def adamw_multi_workspace(n_tensors):
     """Floats that adamw_multi needs as workspace for this many tensors."""
-    n = lib().stdiff_adamw_multi_workspace(n_tensors)
+    n = lib().stdiff_adamw_multi_workspace(n_tensors) if 0 <= n_tensors < 2**31 else -1
     if n < 0:
         raise ValueError(f"adamw_multi_workspace: {n_tensors} tensors")
     return n // 4

@@ -388,3 +388,16 @@ def test_gemm_i8_output_is_kept_apart():
     shared("out and w_scale", lambda: ops.gemm_i8(A, sa, W, buf[3, :6], b, out=buf.view(torch.bfloat16)[:, 10:16]))
     apart(lambda: ops.gemm_i8(A, buf[0, 6:10], W, buf[1, 6:12], buf[2, 10:16], out=out))
     apart(lambda: ops.gemm_i8(A, sa, W, sw, sw, out=out))
+
+
+def test_workspace_queries_refuse_what_an_int_cannot_hold():
+    """sizes reach the C ABI as they are given, or are refused; they do not wrap"""
+    from stdiff_amd import ops
+    for n in (-1, 5 - 2**32, 2**31, 2**32 + 1, 2**64 + 1):
+        with pytest.raises(ValueError):
+            ops.adamw_multi_workspace(n)
+        with pytest.raises(ValueError):
+            ops.layer_norm_bwd_workspace(n, 64, torch.float32)
+        with pytest.raises(ValueError):
+            ops.layer_norm_bwd_workspace(64, n, torch.float32)
+    assert ops.layer_norm_bwd_workspace(2**31 - 1, 64, torch.float32) > 0 and ops.adamw_multi_workspace(2**31 - 1) > 2**31
