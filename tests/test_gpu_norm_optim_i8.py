@@ -1142,3 +1142,93 @@ def test_quantize_rows_of_tiny_values(ops, xt, K):
     assert torch.equal(q.cpu().float(), torch.round(f * torch.where(top > 0, torch.full_like(top, 127.0) / top, torch.zeros_like(top))))
     # half a step of the scale, the roundings of the product, and half of fp32's smallest step in the scale, 127 times
     within(q.cpu().double() * s.cpu().double().view(-1, 1), f, s.cpu().double().view(-1, 1) * (0.5 + 200 * U) + 2 * U * f.double().abs() + 127 * 2.0 ** -150, "value")
+
+
+@pytest.mark.parametrize("R,H", [(37, 7), (37, 48), (37, 1024), (37, 3000), (37, 8200), (20, 17000), (5000, 48), (2500, 1024), (2077, 1001), (3000, 301), (2100, 4099)])
+@pytest.mark.parametrize("xt", ["fp32", "bf16"])
+def test_layer_norm_bwd_column_sums_of_strided_rows(ops, R, H, xt):
+    """x and dy begin at odd elements, with strides of their own: dx, dweight and dbias against float64"""
+    big, bigdy = rnd(R, H + 5, seed=490).to(DT[xt]).to(DEV), rnd(R, H + 3, seed=491).to(DT[xt]).to(DEV)
+    x, dy, w = big[:, 3:H + 3], bigdy[:, 1:H + 1], rnd(H, seed=492).to(DEV)
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    ops.layer_norm(x, w, mean=mean, rstd=rstd)
+    wx, ww, wb, hat, g = grad64(dy.cpu(), x.cpu(), mean.cpu(), rstd.cpu(), w.cpu())
+    tx, tw, tb = grad_tol(dy.cpu(), rstd.cpu(), hat, g)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    within(dx, wx, tx * 1.01 + half_step(dx) * wx.abs() * 1.01, "dx")
+    within(dw, ww, tw, "dweight")
+    within(db, wb, tb, "dbias")
+
+
+def near(got, want, tol, what):
+    """within() for tensors on the device"""
+    off = (got.double() - want).abs() - tol
+    assert bool((off <= 0).all()), f"{what}: off by up to {float(off.max()):.3e} more than the tolerance"
+
+
+def rows_on_device(R, H, t, seed):
+    gen = torch.Generator(DEV).manual_seed(seed)
+    x = torch.randn(R, H, device=DEV, generator=gen)
+    return (x + torch.randn(R, 1, device=DEV, generator=gen)).to(DT[t])
+
+
+# calls that move more than 256 MiB: every kernel that goes past the caches (8, 32 and 64 lanes per row, the workgroup, the large workgroup
+# of fp32 rows), rows that end in a cut vector among them
+@pytest.mark.parametrize("R,H,xt,yt", [(400000, 127, "fp32", "fp32"), (150000, 301, "fp32", "bf16"), (50000, 1001, "fp32", "bf16"), (44000, 1024, "fp32", "bf16"),
+                                       (22000, 2051, "fp32", "bf16"), (5100, 9001, "fp32", "bf16"), (1000000, 72, "bf16", "bf16"), (250000, 300, "bf16", "bf16"),
+                                       (70000, 1001, "bf16", "bf16"), (33000, 2048, "bf16", "bf16"), (17000, 4099, "bf16", "bf16"), (7500, 9001, "fp16", "fp16")])
+def test_layer_norm_past_the_caches(ops, R, H, xt, yt):
+    x, w, b = rows_on_device(R, H, xt, 500), (1 + rnd(H, seed=501, scale=0.2)).to(DEV), rnd(H, seed=502).to(DEV)
+    assert R * H * (x.element_size() + torch.finfo(DT[yt]).bits // 8) > 256 << 20
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    y = ops.layer_norm(x, w, b, out_dtype=DT[yt], mean=mean, rstd=rstd)
+    step = (1 << 24) // H + 1
+    for i in range(0, R, step):                                   # rows by rows: float64 of all of them is large
+        r = slice(i, min(R, i + step))
+        want, m, s = norm64(x[r], w, b, 1e-6)
+        tol = norm_tol(x[r], w, b, m, s) * 1.01 + half_step(y) * want.abs() * 1.01 + (2.0 ** -25 if yt == "fp16" else 0)
+        near(y[r], want, tol, "y")
+        size = x[r].double().abs().mean(1, keepdim=True)
+        near(mean[r].view(-1, 1), m, 65 * U * size + U * m.abs(), "mean")
+        near(rstd[r].view(-1, 1), s, 70 * U * s + s ** 3 * 65 * U * size ** 2, "rstd")
+
+
+@pytest.mark.parametrize("R,H,xt,dt", [(230000, 100, "fp32", "fp32"), (75000, 300, "fp32", "fp32"), (23000, 1001, "fp32", "fp32"), (22000, 1024, "fp32", "fp32"),
+                                       (11000, 2051, "fp32", "fp32"), (11000, 2048, "fp32", "fp32"), (2500, 9001, "fp32", "fp32"), (700000, 72, "bf16", "bf16"),
+                                       (150000, 301, "bf16", "bf16"), (45000, 1024, "bf16", "bf16"), (11000, 4099, "bf16", "bf16"), (3800, 9001, "bf16", "fp32")])
+def test_layer_norm_bwd_past_the_caches(ops, R, H, xt, dt):
+    x, dy, w = rows_on_device(R, H, xt, 510), rows_on_device(R, H, dt, 511), (1 + rnd(H, seed=512, scale=0.2)).to(DEV)
+    assert R * H * (2 * x.element_size() + dy.element_size()) > 256 << 20
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    ops.layer_norm(x, w, mean=mean, rstd=rstd)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    ww, wb, sw, sb = (torch.zeros(H, device=DEV, dtype=torch.float64) for _ in range(4))
+    step = (1 << 24) // H + 1
+    for i in range(0, R, step):
+        r = slice(i, min(R, i + step))
+        wx, pw, pb, hat, g = grad64(dy[r], x[r], mean[r], rstd[r], w)
+        near(dx[r], wx, grad_tol(dy[r], rstd[r], hat, g)[0] * 1.01 + half_step(dx) * wx.abs() * 1.01, "dx")
+        ww, wb, sw, sb = ww + pw, wb + pb, sw + (dy[r].double() * hat).abs().sum(0), sb + dy[r].double().abs().sum(0)
+    # grad_tol's bound over all rows: chains of the rows of a wave and the joins
+    near(dw, ww, (R / 64 + 68) * U * sw, "dweight")
+    near(db, wb, (R / 64 + 64) * U * sb, "dbias")
+
+
+def test_far_rows_of_the_backward(ops):
+    """column sums where the only rows that are not zero lie behind the 2^32-th byte: zeros add exactly, so the bound is that of these rows"""
+    H, ld = 1001, 40000
+    R = 2 ** 31 // ld + 100
+    far = torch.zeros(R, ld, device=DEV, dtype=torch.bfloat16)
+    last = rnd(50, H, seed=520).to(DEV).bfloat16()
+    far[-50:, 7:7 + H] = last
+    x, w = far[:, 7:7 + H], rnd(H, seed=521).to(DEV)
+    mean, rstd = torch.empty(R, device=DEV), torch.empty(R, device=DEV)
+    ops.layer_norm(x, w, mean=mean, rstd=rstd)
+    dx, dw, db = ops.layer_norm_bwd(x, x, mean, rstd, w)
+    args = [t.cpu() for t in (last, last, mean[-50:], rstd[-50:], w)]
+    wx, ww, wb, hat, g = grad64(*args)
+    tx, tw, tb = grad_tol(args[0], args[3], hat, g)
+    within(dx[-50:], wx, tx * 1.01 + half_step(dx) * wx.abs() * 1.01, "dx")
+    within(dw, ww, tw, "dweight")
+    within(db, wb, tb, "dbias")
+    assert not bool(dx[:-50].any())
