@@ -1,5 +1,7 @@
 """Tensor-level wrappers over the C ABI (one function per entry point of include/stdiff_hip.h).
-Tensors must live on the GPU; outputs are allocated with torch when not supplied."""
+Tensors must live on the GPU; outputs are allocated with torch when not supplied.
+Autograd does not see these functions: what they return never requires grad, whatever their inputs do, and a graph that leads
+through them ends there.  A torch.autograd.Function that calls the forward and the backward of an operator joins them to it."""
 import ctypes as C
 
 import torch
@@ -410,7 +412,8 @@ _bind.setup(_entries, L.StdiffError)
 def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, mean=None, rstd=None):
     """LayerNorm of the rows of x [R, H] with a weight and a bias per column (None: 1 and 0; one dtype for both).
     x and out: fp32 or a 16-bit type, any row stride, any H.  mean / rstd (fp32 [R], optional): receive the statistics
-    that layer_norm_bwd takes.  out may be x; else outputs share no memory with inputs or each other."""
+    that layer_norm_bwd takes.  out may be x; else outputs share no memory with inputs or each other.  Outside autograd: the
+    result does not require grad, whatever x, weight and bias do; layer_norm_bwd gives the gradients."""
     return _bind.layer_norm(x, weight, bias, eps, out, out_dtype, mean, rstd)
 
 

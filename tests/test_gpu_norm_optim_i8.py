@@ -1232,3 +1232,39 @@ def test_far_rows_of_the_backward(ops):
     within(dw, ww, tw, "dweight")
     within(db, wb, tb, "dbias")
     assert not bool(dx[:-50].any())
+
+
+def test_layer_norm_and_autograd(ops):
+    """by itself the call is outside autograd, as documented; both halves in an autograd.Function give autograd's gradients"""
+    R, H = 45, 130
+    x, w, b = rnd(R, H, seed=530), 1 + rnd(H, seed=531, scale=0.2), rnd(H, seed=532)
+    c = rnd(R, H, seed=533)
+    gpu = [t.to(DEV).requires_grad_() for t in (x, w, b)]
+    assert not ops.layer_norm(*gpu).requires_grad
+
+    class LayerNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias):
+            mean, rstd = (torch.empty(x.shape[0], device=x.device) for _ in range(2))
+            ctx.save_for_backward(x, mean, rstd, weight)
+            return ops.layer_norm(x, weight, bias, mean=mean, rstd=rstd)
+
+        @staticmethod
+        def backward(ctx, dy):
+            return ops.layer_norm_bwd(dy.contiguous(), *ctx.saved_tensors)     # a sum's gradient is one value, expanded
+    cpu = [t.double().requires_grad_() for t in (x, w, b)]
+    for _ in range(2):                                            # gradients of a second pass are added
+        y = LayerNorm.apply(*gpu)
+        assert y.requires_grad
+        (y * c.to(DEV)).sum().backward()
+        (norm64(*cpu, 1e-6)[0] * c.double()).sum().backward()
+    _, mean, rstd = norm64(x, None, None, 1e-6)
+    _, _, _, hat, g = grad64(c, x, mean, rstd, w)
+    tols = grad_tol(c, rstd, hat, g)
+    # twice the kernel's own bound, the sum of the two passes, and the statistics': mean and rstd are off by 70 u of themselves
+    stat = [70 * U * rstd * (g.abs() + hat.abs() * (g * hat).abs().mean(1, keepdim=True) * 3 + g.abs().mean(1, keepdim=True)),
+            70 * U * (c.double().abs() * (hat.abs() + rstd * (x.double().abs().mean(1, keepdim=True)))).sum(0), 0]
+    for got, want, tol, more in zip(gpu, cpu, tols, stat):
+        within(got.grad, want.grad, 2 * (tol + more) + U * want.grad.abs(), "gradient")
+    ones = torch.autograd.grad(LayerNorm.apply(*gpu).sum(), gpu[2])[0]
+    assert bool((ones == R).all())                                # a sum of ones is exact
