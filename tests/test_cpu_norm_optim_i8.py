@@ -401,3 +401,12 @@ def test_workspace_queries_refuse_what_an_int_cannot_hold():
         with pytest.raises(ValueError):
             ops.layer_norm_bwd_workspace(64, n, torch.float32)
     assert ops.layer_norm_bwd_workspace(2**31 - 1, 64, torch.float32) > 0 and ops.adamw_multi_workspace(2**31 - 1) > 2**31
+
+
+def test_build_compiles_what_is_built_already(monkeypatch):
+    """build() leaves no object of older sources or flags in place, whatever its time stamp says"""
+    import __graft_entry__ as G
+    ran = []
+    monkeypatch.setattr(G.subprocess, "run", lambda cmd, **kw: ran.append(cmd))
+    G.build()
+    assert len(ran) == 2 and all(cmd[0] == "make" and "-B" in cmd for cmd in ran)
