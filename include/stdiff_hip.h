@@ -522,7 +522,8 @@ int stdiff_layer_norm_bwd(const void* dy, long long lddy, int dy_dtype, const vo
  *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
  * state_bits 32: exp_avg / exp_avg_sq are fp32 [n].  state_bits 8: they are e4m3 codes [n], of m and of the ROOT of v, and every
  * 256 consecutive elements share exp_avg_scale / exp_avg_sq_scale (fp32 [ceil(n / 256)]): m = scale * code, sqrt v = scale *
- * code; all zeros is the state before the first step.  A block that holds an infinity or a NaN is NaN from the next step on.
+ * code; all zeros is the state before the first step.  A block that holds an infinity or a NaN is NaN from the next step on;
+ * one whose largest is below 1e-30 is held in units of 1e-30 / 448.
  * step_dev: int32 [1], the steps done before this call; incremented by it.  max_norm <= 0: no clipping.  norm (may be
  * NULL): receives the norm.  A norm that is NaN makes every parameter NaN.  The `tensors` array is read during the call
  * only; the tensors must not overlap; weight_decay >= 0.  workspace: stdiff_adamw_multi_workspace(n_tensors) bytes, 4-byte aligned. */

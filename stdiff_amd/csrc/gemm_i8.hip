@@ -5,8 +5,9 @@
 // scales are applied to the finished sum in fp32, the weight's first: sum * a_scale would overflow for activations above
 // 1e31 whose product with a weight is still a number.
 // Measured: quantisation of 65536 x 2048 bf16 71 us (5.6 TB/s), of 4 rows 2.1 us; product
-// of 4 x 4096 x 1024 3.8 us (a launch, one trip to memory and one barrier), of 65536 x 8192 x 2048 865 us (2.54 POP/s; 8192 x
-// 8192 x 8192 2.97): the matrix units are busy 69 % of the cycles, and the clock falls to 1.9 GHz.
+// of 4 x 4096 x 1024 3.7 us (a launch, one trip to memory and one barrier), of 65536 x 8192 x 2048 865 to 950 us (2.3 to 2.5 POP/s, by
+// what clock the card holds that day; 8192 x 8192 x 8192 up to 2.97): the matrix units are busy 69 % of the cycles, and the clock
+// falls to 1.9 GHz and below.
 #include "common.h"
 
 namespace {
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_tile_kernel(Params8 p, int ti
 // All of LDS is one array: with another for the scales the compiler lets every read wait for all DMA under way.
 // Measured per tile: 1.36 us for a slab (the instructions alone 1.1 at the clock that they leave), 5 us for C, half of it conversions and
 // scales.  The stores of C are under way during the next tile's first slab: the counted waits know how many they are.
-// PAST: C goes past the caches.  TAIL: K is no multiple of 16.  (A form of its own: the kernel uses all 256 registers, and the masks cost some.)
+// PAST: C goes past the caches.  TAIL: K is no multiple of 16.  (A form of its own: 229 to 233 registers without the masks, 248 to 251 with them, of 256.)
 template <typename TC, bool TAIL, bool PAST>
 __global__ __launch_bounds__(512, 1) void gemm_i8_256_kernel(Params8 p, int tiles_m, int tiles_n, int whole, int units) {
     constexpr int HALF = 128 * SLAB;
@@ -621,8 +622,11 @@ template <typename TC> int launch_gemm_i8(const Params8& p, hipStream_t st) {
         const int tail = (int)(t256 % cus);
         const int whole = tail && tail <= cus / 2 ? (int)t256 - tail : (int)t256, units = whole + 2 * ((int)t256 - whole);
         // Past the caches, but where rows begin inside cache lines and the caches hold most of C: its lines are whole before they leave
-        // (26628 x 3464 x 64 -> fp32, 369 MB: 101 us past the caches, 85 through them, -> bf16 63 and 43; 25055 x 5127 x 449 -> fp32,
-        // 514 MB: 171 and 176; whole lines, 131072 x 4096 x 128 -> bf16: 209 and 252).
+        // (us past the caches and through them: 26628 x 3464 x 128 -> fp32, 369 MB, 98 and 95, -> bf16 61 and 50; 25055 x 5127 x 449 ->
+        // fp32, 514 MB, 171 and 185).  Whole lines: 131072 x 4096 x 128 -> bf16 216 and 249, 65536 x 1024 x 256 -> bf16 34 and 45, 8192 x
+        // 8192 x 512 -> fp32 68 and 82, 65536 x 8192 x 2048 -> bf16 923 and 952, 2048 x 2560 x 2048 -> bf16 the same, but 8192 x 4096 x
+        // 1024 -> bf16 41 and 38.  With a kernel behind that reads C (quantize_rows): 547 and 549, 79 and 83, 141 and 133, 1200 and 1263,
+        // 28 and 28, 59 and 53: what the stores gain there is lost in part to reads that no cache serves, for C of 60 to 270 MB up to a tenth.
         const bool past = (((uintptr_t)p.C | (uintptr_t)(p.ldc * sizeof(TC))) & 127) == 0 || (long long)p.M * p.N * (long long)sizeof(TC) > (400ll << 20);
 #define TILES(TAIL, PAST)                                                                                                      \
     hipLaunchKernelGGL((gemm_i8_256_kernel<TC, TAIL, PAST>), dim3(std::min(units, cus)), dim3(512), 0, st, p, cdiv(p.M, 256),  \

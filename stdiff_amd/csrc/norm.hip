@@ -7,12 +7,14 @@
 // up to 128, 512 or 1024 elements (a wave holds 8, 2 or 1 of them), longer rows have a workgroup of ceil(H / 1024) waves,
 // up to 16384; beyond that (and below 8) the row is read again from the cache.  Small shares keep many rows in flight: with
 // one row per wave whatever its length, rows of 64 and 300 16-bit elements ran at 1.1 and 3.9 TB/s.
+// The kernels for rows beyond 16384 and below 8 are simple ones: 4096 x 20000 fp32 forward 215 us (3.1 TB/s), backward 402 (2.4), bf16 123 and
+// 245; rows below 8 leave nearly all lanes idle, 1000000 x 7 fp32 1.4 ms forward and 15 ms backward (64 threads walk down all rows).
 // The vector that the row's end cuts is moved left until it fits: its lane holds some of its neighbour's columns again, leaves
 // them out of the sums and stores them a second time with the same bits.  (Element by element, the 7 elements at the end
 // of rows of 999 cost 0.8 of the time of all others.)
 // Bound by memory where there are many rows, by launch and one trip to memory where there are few: forward of one row of
-// 1024 1.8 us, of 131072 x 1024 fp32 -> bf16 130 us (6.2 TB/s), backward of 32768 x 2048 fp32 135 + 5 us for the partial sums (5.8
-// TB/s), of 512 x 1024 bf16 3.5 us in one launch.
+// 1024 1.8 us, of 131072 x 1024 fp32 -> bf16 131 us (6.2 TB/s), backward of 32768 x 2048 fp32 135 + 6 us for the partial sums (5.7
+// TB/s), of 512 x 1024 bf16 3.8 us in one launch.
 // The variance is formed from the centred values (a second walk over the registers), so a row whose mean is far larger
 // than its spread keeps its digits.  All statistics and sums are fp32.
 #include "common.h"
@@ -473,17 +475,21 @@ inline bool in_registers(int H) { return H >= 8 && H <= IN_REGISTERS; }
 inline int norm_blocks(long long R, int rows_per_block, int per_cu) {
     return (int)std::min<long long>((R + rows_per_block - 1) / rows_per_block, (long long)per_cu * cu_count());
 }
-// A call that moves more than the memory-side cache holds (256 MB) goes past the caches: 131072 x 1024 fp32 -> bf16 131 against
-// 152 us, backward of 32768 x 2048 fp32 141 against 154, 262144 x 300 bf16 70 against 66.  Below that the next kernel finds the result in a
-// cache.
+// A call that moves more than the memory-side cache holds (256 MB) goes past the caches (us past them, through them): 131072 x 1024
+// fp32 -> bf16 133 and 152, 65536 x 2048 bf16 94 and 103, backward of 32768 x 2048 fp32 142 and 155, of 65536 x 1024 bf16 76 and 83, of
+// 32768 x 4096 bf16 144 and 147.  16-bit rows of 32 lanes gain nothing: 262144 x 300 bf16 75 and 75, its backward 101 and 98.  Below
+// that the next kernel finds the result in a cache.
 inline bool past_caches(long long bytes) { return bytes > (256ll << 20); }
 inline int lanes_of(int H) { return H <= 128 ? 8 : H <= 512 ? 32 : H <= 1024 ? 64 : BLOCK; }
 inline int threads_of(int H) { return H <= 1024 ? 256 : cdiv(H, 1024) * 64; }
 inline int rows_of_block(int H) { return H <= 1024 ? 256 / lanes_of(H) : 1; }
-// Few rows: the column sums walk down the rows in the launch that gives dx.  A workgroup reads 32 columns of all rows: up to 320 KB that is
-// better than the second launch, the workspace and the partial sums (us per call, one and two launches: 512 x 1024 bf16 5.6
-// and 9.5, 1024 x 1024 fp32 5.7 and 10.0, 1200 x 4096 bf16 10.7 and 16.2, 2500 x 1024 bf16 7.4 and 10.3; rows that begin anywhere,
-// 2077 x 1001 bf16, 10.6 and 9.8; behind the limit, 4096 x 1024 bf16, 21 and 11).
+// Few rows: the column sums walk down the rows in the launch that gives dx, without the second launch, the workspace and the
+// partial sums.  A workgroup reads 32 columns of all rows, 320 KB at most.  GPU us by one and by two launches, with operands that the
+// last call did not have: 512 x 1024 bf16 3.0 and 7.2, 1000 x 1024 5.1 and 8.1, 1500 x 1024 8.0 and 9.5, 1024 x 1024 fp32 7.9 and
+// 9.3, 1200 x 4096 bf16 11.0 and 15.2, fp32 15.6 and 16.8; rows that begin anywhere, 1000 x 1001 bf16 7.1 and 8.6, 1500 x 1001 9.3
+// and 10.1.  The limit suits operands that are still in the L2 (the same ones again, 2500 x 1024 bf16: 7.8 and 10.2); for others
+// two launches are better from about 250 KB on: 2000 x 1024 bf16 11.3 and 11.0, 2500 x 1024 13.6 and 10.7, 2077 x 1001 12.0 and
+// 10.2.  Behind the limit, 4096 x 1024 bf16: 21 and 11.
 inline bool one_launch(int R, int H, int x_size, int dy_size) {
     return (long long)R * 32 * (x_size + dy_size) <= 320 << 10 && H >= 8 && H <= 8192;
 }

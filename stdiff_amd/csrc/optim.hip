@@ -10,7 +10,9 @@
 // still under the slow decay of v.  The step itself uses m and v before they are rounded.
 // Bound by memory: 120 M parameters in 32 bits 82 us for the norm (5.8 TB/s) and 547 for the step (6.1 TB/s), 30 M with 8-bit states
 // 14 and 86 us (5.0 TB/s; 230 vector instructions per 256 elements keep the vector units busy 56 % of it), 479 M 1386 us together.  Small models are two launches
-// of 4.6 and 6.1 us: the table, the data, for the step also the partial sums, one trip to memory each.
+// of 4.5 and 6.2 us: the table, the data, for the step also the partial sums, one trip to memory each.  Without clipping one thread's
+// launch (the step count and two powers in 64 bits, 2.5 to 5 us) stands in the norm's place.  With 8-bit states the instructions are the
+// same for 16-bit parameters and gradients as for fp32 ones: 120 M of them 334 us instead of 358, at 10 bytes per element instead of 16.
 // A block that holds an infinity or a NaN gets a scale that is not finite: all its elements are NaN from the next step on.
 #include <float.h>
 
