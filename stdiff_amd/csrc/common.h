@@ -75,6 +75,13 @@ __device__ __forceinline__ unsigned pack2bf(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2_cv));
 }
 #endif
+// Conversions to 16 bits as IEEE has them, also in fp16: what the range does not hold becomes an infinity, a NaN stays one (the
+// clamping ones above make 65504 and -65504 of them).  For results whose overflow has to be seen, as by a loss scaler.
+__device__ __forceinline__ bf16_t to_h16(float f) { return __builtin_bit_cast(bf16_t, (h16)f); }
+__device__ __forceinline__ unsigned to_2h16(float a, float b) {
+    f32x2_cv v = {a, b};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2_cv));
+}
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {

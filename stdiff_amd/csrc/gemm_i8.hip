@@ -201,8 +201,10 @@ __device__ __forceinline__ f32x4 scaled(i32x4 sum, float as, f32x4 ws, f32x4 b) 
     for (int e = 0; e < 4; ++e) o[e] = (float)sum[e] * ws[e] * as + b[e];
     return o;
 }
+__device__ __forceinline__ void put1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put1(bf16_t* p, float v) { *p = to_h16(v); }
 __device__ __forceinline__ void put4(float* p, f32x4 v) { *(f32x4*)p = v; }
-__device__ __forceinline__ void put4(bf16_t* p, f32x4 v) { *(u32x2*)p = u32x2{pack2bf(v[0], v[1]), pack2bf(v[2], v[3])}; }
+__device__ __forceinline__ void put4(bf16_t* p, f32x4 v) { *(u32x2*)p = u32x2{to_2h16(v[0], v[1]), to_2h16(v[2], v[3])}; }
 // 16 bytes of a row of C, which may begin at any element and end inside the piece
 template <typename TC> __device__ __forceinline__ void store16(TC* row, int n, int N, u32x4 v) {
     constexpr int E = 16 / sizeof(TC);
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(512) void gemm_i8_rows_kernel(Params8 p) {
     TC* row = (TC*)p.C + m * p.ldc;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) Elem<TC>::st(row + n + e, v[e]);
+        if (n + e < p.N) put1(row + n + e, v[e]);
 }
 
 // ---- BM x BN tiles, one per workgroup of NW waves: both operands by LDS-DMA into a ring of four slabs, three ahead, one barrier

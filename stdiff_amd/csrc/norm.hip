@@ -55,15 +55,17 @@ template <int V, bool NT = false> __device__ __forceinline__ void stv(float* p, 
 }
 template <int V, bool NT = false> __device__ __forceinline__ void stv(bf16_t* p, const float* o) {
     if constexpr (V == 8) {
-        const u32x4 v = {pack2bf(o[0], o[1]), pack2bf(o[2], o[3]), pack2bf(o[4], o[5]), pack2bf(o[6], o[7])};
+        const u32x4 v = {to_2h16(o[0], o[1]), to_2h16(o[2], o[3]), to_2h16(o[4], o[5]), to_2h16(o[6], o[7])};
         if (NT) __builtin_nontemporal_store(v, (u32x4_u*)p);
         else *(u32x4_u*)p = v;
     } else {
-        const u32x2 v = {pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+        const u32x2 v = {to_2h16(o[0], o[1]), to_2h16(o[2], o[3])};
         if (NT) __builtin_nontemporal_store(v, (u32x2_u*)p);
         else *(u32x2_u*)p = v;
     }
 }
+__device__ __forceinline__ void st1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st1(bf16_t* p, float v) { *p = to_h16(v); }
 // V elements at column c of a row of H; what lies behind the row's end reads as `fill` and is not written
 template <int V, typename T> __device__ __forceinline__ void ld_edge(const T* row, int c, int H, float fill, float* o) {
     if (c + V <= H) return ldv<V>(row + c, o);
@@ -74,7 +76,7 @@ template <int V, typename T> __device__ __forceinline__ void st_edge(T* row, int
     if (c + V <= H) return stv<V>(row + c, o);
 #pragma unroll
     for (int j = 0; j < V; ++j)
-        if (c + j < H) Elem<T>::st(row + c + j, o[j]);
+        if (c + j < H) st1(row + c + j, o[j]);
 }
 
 // the columns of a lane's vector that begins at c in a row of H >= V
@@ -262,7 +264,7 @@ __device__ __forceinline__ void norm_bwd_rows(const TD* dy, long long lddy, cons
             } else if (ONCE && col[i].in()) {
 #pragma unroll
                 for (int j = 1; j < V; ++j)
-                    if (j >= col[i].skip) Elem<TX>::st(to + j, o[j]);
+                    if (j >= col[i].skip) st1(to + j, o[j]);
             }
         }
     }

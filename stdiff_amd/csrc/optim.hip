@@ -88,12 +88,12 @@ template <bool WHOLE> __device__ __forceinline__ void st4e(float* p, int k, f32x
 }
 template <bool WHOLE> __device__ __forceinline__ void st4e(bf16_t* p, int k, f32x4 o) {
     if (WHOLE || k >= 4) {
-        const u32x2 v = {pack2bf(o[0], o[1]), pack2bf(o[2], o[3])};
+        const u32x2 v = {to_2h16(o[0], o[1]), to_2h16(o[2], o[3])};
         __builtin_nontemporal_store(v, (u32x2_u*)p);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (j < k) p[j] = f2bf(o[j]);
+            if (j < k) p[j] = to_h16(o[j]);
     }
 }
 template <bool WHOLE> __device__ __forceinline__ unsigned ld_codes(const unsigned char* p, int k) {

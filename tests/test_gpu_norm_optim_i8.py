@@ -1268,3 +1268,75 @@ def test_layer_norm_and_autograd(ops):
         within(got.grad, want.grad, 2 * (tol + more) + U * want.grad.abs(), "gradient")
     ones = torch.autograd.grad(LayerNorm.apply(*gpu).sum(), gpu[2])[0]
     assert bool((ones == R).all())                                # a sum of ones is exact
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H", [5, 40, 300, 1000, 3000, 9000, 17000])
+def test_layer_norm_in_16_bits_beyond_the_range(ops, t, H):
+    """a NaN stays a NaN, what the type's range does not hold becomes an infinity of its sign, as a conversion has it"""
+    x = rnd(5, H, seed=540)
+    x[1, 3], x[2, 2], x[3, 1] = float("nan"), float("inf"), float("-inf")
+    x[0] += 10                                                   # no element close to the mean
+    x[0, ::2] -= 20
+    big = torch.full((H,), 3e38, device=DEV)
+    for src in (x.to(t), x):                                     # 16-bit and fp32 rows
+        y = ops.layer_norm(src.to(DEV), big, out_dtype=t).cpu()
+        assert y.dtype == t and bool(torch.isnan(y[1:4]).all())
+        off = src[0].double() - src[0].double().mean()           # about 10 in magnitude
+        assert bool((torch.sign(y[0].double()) == torch.sign(off)).all()) and bool((y[0].double().abs() > 1e37).all())
+        if t == torch.float16:
+            assert bool(torch.isinf(y[0]).all())
+        ok = ops.layer_norm(src.to(DEV), out_dtype=t).cpu()
+        assert bool(torch.isfinite(ok[0]).all()) and bool(torch.isfinite(ok[4]).all())
+    mean, rstd = torch.zeros(5, device=DEV), torch.full((5,), 1e6, device=DEV)
+    mean[0] = float("nan")
+    dy = rnd(5, H, seed=541).to(t).to(DEV)
+    for k in (1, 500):                                           # few rows in one launch, many in two
+        dx = ops.layer_norm_bwd(dy.repeat(k, 1), x.to(t).to(DEV).repeat(k, 1), mean.repeat(k), rstd.repeat(k), big * 1e-30)[0].cpu().view(k, 5, H)
+        assert bool(torch.isnan(dx[:, 0]).all()) and bool(torch.isnan(dx[:, 1]).all())
+        if t == torch.float16:
+            assert not bool((dx[:, 4].abs() == 65504).any()) and bool(torch.isinf(dx[:, 4]).any())
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", [(4, 100, 64), (300, 200, 200), (1600, 1700, 128), (5000, 4200, 128), (5000, 4200, 200)])
+def test_gemm_i8_in_16_bits_beyond_the_range(ops, t, M, N, K):
+    """every kernel of the product: scales that are not finite, and results that the type's range does not hold"""
+    A, W, _, _, _ = operands(M, N, K, seed=550)
+    A[:, :K], W[:, :K] = A[:, :K].abs().clamp_min(1), W[:, :K].abs().clamp_min(1)
+    sa, sw, b = torch.ones(M), torch.ones(N), torch.zeros(N)
+    sa[0], sa[M - 1], sa[M // 2], sa[1] = float("nan"), float("inf"), -1e35, 1e-3
+    sw[N // 3] = float("nan")
+    b[N - 1] = float("-inf")
+    y = ops.gemm_i8(A.to(DEV)[:, :K], sa.to(DEV), W.to(DEV)[:, :K], sw.to(DEV), b.to(DEV), out_dtype=t).cpu()
+    nan = torch.zeros(M, N, dtype=torch.bool)
+    nan[0], nan[:, N // 3], nan[M - 1, N - 1] = True, True, True
+    assert torch.equal(torch.isnan(y), nan)
+    assert bool((y[1:M - 1, N - 1] == -math.inf).all()) and bool(((y[M - 1] == math.inf) | nan[M - 1]).all())
+    assert bool(torch.isfinite(y[1, :N - 1])[~nan[1, :N - 1]].all())
+    if t == torch.float16:
+        assert bool(((y[M // 2] == -math.inf) | nan[M // 2]).all()) and not bool((y.abs() == 65504).any())
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [5, 1023, 300000])
+def test_adamw_multi_in_16_bits_beyond_the_range(ops, t, bits, n):
+    """a norm that is NaN makes every parameter NaN; without clipping a NaN or an infinite parameter stays where it is"""
+    for clip in (True, False):
+        p = torch.ones(n, device=DEV).to(t)
+        p[1], p[n - 1] = float("inf"), torch.finfo(t).max
+        g = torch.ones(n, device=DEV)
+        g[2] = float("nan")
+        g[n - 1] = -1.0
+        st = ops.adamw8_state(p) if bits == 8 else (torch.zeros(n, device=DEV), torch.zeros(n, device=DEV))
+        args = ops.adamw_multi_args([p], *[[v] for v in st])
+        ops.adamw_multi(args, [g], torch.zeros(1, device=DEV, dtype=torch.int32), torch.finfo(t).max / 8 if t == torch.float16 else 1e-3,
+                        max_norm=1.0 if clip else None)
+        q = p.cpu().float()
+        if clip:
+            assert bool(torch.isnan(q).all())
+            continue
+        assert math.isnan(q[2]) and int(torch.isnan(q).sum()) == 1 and math.isinf(q[1])
+        if t == torch.float16:                                   # 65504 + 8188
+            assert q[n - 1] == math.inf
