@@ -16,7 +16,9 @@
 // 1024 1.8 us, of 131072 x 1024 fp32 -> bf16 131 us (6.2 TB/s), backward of 32768 x 2048 fp32 135 + 6 us for the partial sums (5.7
 // TB/s), of 512 x 1024 bf16 3.8 us in one launch.
 // The variance is formed from the centred values (a second walk over the registers), so a row whose mean is far larger
-// than its spread keeps its digits.  All statistics and sums are fp32.
+// than its spread keeps its digits.  Statistics and sums are fp32; a thread's own sum of the rows beyond 16384, and of the columns of
+// those and of rows below 8, is held in 64 bits, since its terms may be millions (one row of 2^26 columns around 3.3 with a spread
+// of 0.01: the mean off by 2e-4 in fp32; the time does not change).
 #include "common.h"
 
 namespace {
@@ -175,20 +177,21 @@ __global__ __launch_bounds__(256) void layer_norm_long_kernel(const TX* x, long 
     for (long long row = blockIdx.x; row < R; row += gridDim.x, odd ^= 1) {
         const TX* xr = x + row * ldx;
         TY* yr = y + row * ldy;
-        float s = 0.f, q = 0.f;
+        double s = 0.0, q = 0.0;
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float v[4];
             ld_edge<4>(xr, c, H, 0.f, v);
             s += (v[0] + v[1]) + (v[2] + v[3]);
         }
-        const float mu = row_sum<BLOCK>(s, part[odd][0]) * inv;
+        const float mu = row_sum<BLOCK>((float)s, part[odd][0]) * inv;
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float v[4];
             ld_edge<4>(xr, c, H, mu, v);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q += (v[j] - mu) * (v[j] - mu);
+            for (int j = 0; j < 4; ++j) v[j] = (v[j] - mu) * (v[j] - mu);
+            q += (v[0] + v[1]) + (v[2] + v[3]);
         }
-        const float rs = 1.0f / sqrtf(row_sum<BLOCK>(q, part[odd][1]) * inv + eps);
+        const float rs = 1.0f / sqrtf(row_sum<BLOCK>((float)q, part[odd][1]) * inv + eps);
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float v[4], wv[4] = {1.f, 1.f, 1.f, 1.f}, bv[4] = {0.f, 0.f, 0.f, 0.f};
             ld_edge<4>(xr, c, H, 0.f, v);
@@ -390,7 +393,7 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_long_kernel(const TD* dy, 
     int odd = 0;
     for (long long row = blockIdx.x; row < R; row += gridDim.x, odd ^= 1) {
         const float mu = mean[row], rs = rstd[row];
-        float sg = 0.f, sgx = 0.f;
+        double sg = 0.0, sgx = 0.0;
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float d[4], v[4], wv[4] = {1.f, 1.f, 1.f, 1.f};
             ld_edge<4>(dy + row * lddy, c, H, 0.f, d);
@@ -398,12 +401,13 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_long_kernel(const TD* dy, 
             if (w) ld_edge<4>(w, c, H, 0.f, wv);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float g = d[j] * wv[j];
-                sg += g;
-                sgx += g * ((v[j] - mu) * rs);
+                d[j] *= wv[j];
+                v[j] = d[j] * ((v[j] - mu) * rs);
             }
+            sg += (d[0] + d[1]) + (d[2] + d[3]);
+            sgx += (v[0] + v[1]) + (v[2] + v[3]);
         }
-        const float mg = row_sum<BLOCK>(sg, part[odd][0]) * inv, mgx = row_sum<BLOCK>(sgx, part[odd][1]) * inv;
+        const float mg = row_sum<BLOCK>((float)sg, part[odd][0]) * inv, mgx = row_sum<BLOCK>((float)sgx, part[odd][1]) * inv;
         for (int c = threadIdx.x * 4; c < H; c += 1024) {
             float d[4], v[4], wv[4] = {1.f, 1.f, 1.f, 1.f};
             ld_edge<4>(dy + row * lddy, c, H, 0.f, d);
@@ -421,7 +425,7 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_columns_kernel(const TD* d
                                                                      const float* mean, const float* rstd, float* ws, int ldp,
                                                                      int R, int H) {
     const int c = (blockIdx.x * 256 + threadIdx.x) * 4;
-    float aw[4] = {0.f, 0.f, 0.f, 0.f}, ab[4] = {0.f, 0.f, 0.f, 0.f};
+    double sw[4] = {0.0, 0.0, 0.0, 0.0}, sb[4] = {0.0, 0.0, 0.0, 0.0};
     if (c >= H) return;
     for (long long row = blockIdx.y; row < R; row += gridDim.y) {
         float d[4], v[4];
@@ -430,10 +434,13 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_columns_kernel(const TD* d
         const float mu = mean[row], rs = rstd[row];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            aw[j] += d[j] * ((v[j] - mu) * rs);
-            ab[j] += d[j];
+            sw[j] += d[j] * ((v[j] - mu) * rs);
+            sb[j] += d[j];
         }
     }
+    float aw[4], ab[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { aw[j] = (float)sw[j]; ab[j] = (float)sb[j]; }
     float* out = ws + (size_t)blockIdx.y * 2 * ldp;
     st_edge<4>(out, c, H, aw);
     st_edge<4>(out + ldp, c, H, ab);

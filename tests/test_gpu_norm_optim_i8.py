@@ -1340,3 +1340,36 @@ def test_adamw_multi_in_16_bits_beyond_the_range(ops, t, bits, n):
         assert math.isnan(q[2]) and int(torch.isnan(q).sum()) == 1 and math.isinf(q[1])
         if t == torch.float16:                                   # 65504 + 8188
             assert q[n - 1] == math.inf
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_layer_norm_of_very_long_rows(ops, t):
+    """rows of 2^26 columns whose mean is far larger than their spread: sums of so many terms keep their digits, as the bounds of
+    short rows ask for it; the column sums of very many rows of three columns likewise"""
+    H = (1 << 26) + 5
+    gen = torch.Generator(DEV).manual_seed(560)
+    x = (3.3 + 0.01 * torch.randn(1, H, device=DEV, generator=gen)).to(t)
+    mean, rstd = torch.empty(1, device=DEV), torch.empty(1, device=DEV)
+    y = ops.layer_norm(x, mean=mean, rstd=rstd)
+    want, m, r = norm64(x, None, None, 1e-6)
+    size = x.double().abs().mean(1, keepdim=True)
+    near(mean.view(1, 1), m, 65 * U * size + U * m.abs(), "mean")
+    near(rstd.view(1, 1), r, 70 * U * r + r ** 3 * 65 * U * size ** 2, "rstd")
+    near(y, want, norm_tol(x, None, None, m, r) * 1.01 + half_step(y) * want.abs() * 1.01, "y")
+    dy = (0.1 + 0.01 * torch.randn(1, H, device=DEV, generator=gen)).to(t)
+    dx, _, db = ops.layer_norm_bwd(dy, x, mean, rstd, dbias=torch.empty(H, device=DEV))
+    wx, _, _, hat, g = grad64(dy, x, mean, rstd, None)
+    near(dx, wx, grad_tol(dy, rstd, hat, g)[0] * 1.01 + half_step(dx) * wx.abs() * 1.01, "dx")
+    assert torch.equal(db, dy[0].float())
+
+
+def test_layer_norm_bwd_of_very_many_short_rows(ops):
+    R, H = 3000001, 3
+    gen = torch.Generator(DEV).manual_seed(570)
+    x, dy = torch.randn(R, H, device=DEV, generator=gen), 0.1 + 1e-4 * torch.randn(R, H, device=DEV, generator=gen)
+    mean, rstd = x.double().mean(1).float(), torch.ones(R, device=DEV)
+    _, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, dweight=torch.empty(H, device=DEV), dbias=torch.empty(H, device=DEV))
+    _, ww, wb, hat, _ = grad64(dy, x, mean, rstd, None)
+    # products of three roundings; a share's sum is rounded once, 64 shares pass at most 2 additions of a slot and 5 of the tree
+    near(dw, ww, 11 * U * (dy.double() * hat).abs().sum(0), "dweight")
+    near(db, wb, 8 * U * dy.double().abs().sum(0), "dbias")
