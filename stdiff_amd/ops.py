@@ -420,9 +420,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, out=None, out_dtype=None, me
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, dx=None, dweight=None, dbias=None, accumulate=False, workspace=None):
     """Backward of layer_norm from its mean / rstd: (dx, dweight, dbias).  dx has x's dtype (allocated unless given; it may be
     dy or x).  dweight / dbias are fp32 [H]: with a weight both are allocated unless given, without one those that are
-    given are formed (else None); accumulate=True adds to what the given ones hold.  They are sums over the rows in a
-    fixed order: the same bits every run.  dy may be one row for all rows (an expanded tensor).  But for dx in the place of
-    dy or x, outputs and workspace share no memory with inputs or each other.
+    given are formed (else None); accumulate=True adds to what the given ones hold, and forms no others.  They are sums over
+    the rows in a fixed order: the same bits every run.  dy may be one row for all rows (an expanded tensor).  But for dx in the
+    place of dy or x, outputs and workspace share no memory with inputs or each other.
     workspace (fp32, at least layer_norm_bwd_workspace(R, H, ..) floats, none for few rows; allocated unless given):
     give one of its own to a call that is captured into an ops.Graph."""
     return _bind.layer_norm_bwd(dy, x, mean, rstd, weight, dx, dweight, dbias, accumulate, workspace)
