@@ -483,12 +483,14 @@ PyObject* adamw_multi(PyObject* const* a) {
         if (d->numel() != t->sizes[i] || !d->is_contiguous())
             refuse(PyExc_ValueError, "adamw_multi: gradient ", i, ": ", t->sizes[i], " contiguous elements are needed, got ", d->sizes(), " with strides ", d->strides());
         if (!d->is_cuda() || d->get_device() != t->device) refuse(PyExc_ValueError, "adamw_multi: gradient ", i, " is on ", d->device(), ", its parameter on device ", t->device);
-        const Area grad = flat(d, "gradient");
-        if (!apart(grad)) refuse(PyExc_ValueError, "adamw_multi: gradient ", i, " shares memory with a parameter or state");
-        for (const Area& c : cells)
-            if (meet(c, grad)) refuse(PyExc_ValueError, "adamw_multi: ", c.name, " and gradient ", i, " share memory");
         rows[i].grad = d->data_ptr();
         rows[i].grad_dtype = half.code(d->scalar_type());
+        const int64_t bytes = t->sizes[i] * (rows[i].grad_dtype == STDIFF_F32 ? 4 : 2);
+        const Area grad = {"gradient", (uintptr_t)rows[i].grad, bytes ? 1 : 0, bytes, bytes, ScalarType::Undefined};
+        if (!apart(grad)) refuse(PyExc_ValueError, "adamw_multi: gradient ", i, " shares memory with a parameter or state");
+        for (const Area& c : cells)
+            if (bytes && !c.empty() && c.at < grad.at + bytes && grad.at < c.end())
+                refuse(PyExc_ValueError, "adamw_multi: ", c.name, " and gradient ", i, " share memory");
     }
     Place here(step, {norm, ws_});
     if (n && here.device != t->device) refuse(PyExc_ValueError, "step_dev is on ", step.device(), ", the parameters on device ", t->device);
