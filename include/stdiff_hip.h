@@ -497,7 +497,8 @@ int stdiff_dit_backward(const stdiff_train_weights* w, const stdiff_train_acts* 
 /* ---------------------------------------------------------------- norm, optimizer and 8-bit product beside the DiT
  * (no counterpart in the reference, which leaves them to torch).  Rows may begin at any element and have any length
  * unless a function says otherwise; leading dimensions are 64-bit, and those of matrices that are only read may be smaller
- * than a row (0: one row for all).  None of them allocates; each may be captured.  Their conversions to 16 bits do not
+ * than a row (0: one row for all).  Outputs and workspaces share no memory with inputs or each other, but where in-place work is
+ * said to be possible; this is not checked here.  None of them allocates; each may be captured.  Their conversions to 16 bits do not
  * saturate in either build: what fp16 does not hold becomes an infinity, and a NaN stays one.
  *
  * LayerNorm over rows of H with a weight and a bias per column (either may be NULL: 1 and 0; both have w_dtype):
